@@ -47,6 +47,9 @@ EXPORTS = [
     "kdnn_b200_moe_route", "kdnn_b200_moe_workspace_bytes", "kdnn_b200_moe_ffn",
     "kdnn_b200_residual_rmsnorm", "kdnn_b200_dequant_to_dense", "kdnn_b200_quant_gemv_fp",
     "kdnn_b200_quant_gemv_host",
+
+    "kdnn_b200_kv_writes", "kdnn_b200_kv_plan", "kdnn_b200_kv_append", "kdnn_b200_kv_attention_workspace_bytes",
+    "kdnn_b200_kv_attention", "kdnn_b200_prompt_attention",
 ]
 
 
@@ -70,6 +73,11 @@ class GemvLayoutC(C.Structure):
 class MoeExchangeC(C.Structure):
     _fields_ = [("rank", C.c_int), ("world", C.c_int), ("regions", C.POINTER(C.c_void_p)),
                 ("wait_ns", C.c_ulonglong)]
+
+
+class KvCacheC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_size_t), ("kv_heads", C.c_size_t), ("page", C.c_size_t), ("dim", C.c_size_t)]
 
 
 KERNEL_AUTO, KERNEL_XREG, KERNEL_SMEM_WINDOW, KERNEL_ITEM_STREAM, KERNEL_PLAIN_LOADS = 0, 1, 2, 3, 4
@@ -159,6 +167,16 @@ def _load() -> C.CDLL:
     lib.kdnn_b200_read_probe.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]
     lib.kdnn_b200_residual_rmsnorm.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p,
                                                C.c_size_t, C.c_size_t, C.c_size_t, C.c_float, C.c_int, C.c_void_p]
+    P, Z = C.c_void_p, C.c_size_t
+    lib.kdnn_b200_kv_writes.restype = Z
+    lib.kdnn_b200_kv_writes.argtypes = [Z, Z, Z]
+    lib.kdnn_b200_kv_plan.argtypes = [P, P, Z, Z, Z, P, Z, Z, P, Z, P, P, P, P, P, P, P, Z, P]
+    lib.kdnn_b200_kv_append.argtypes = [P, Z, Z, P, Z, Z, C.c_int, Z, P, Z, C.POINTER(KvCacheC), P]
+    lib.kdnn_b200_kv_attention_workspace_bytes.restype = Z
+    lib.kdnn_b200_kv_attention_workspace_bytes.argtypes = [Z] * 5
+    lib.kdnn_b200_kv_attention.argtypes = [P, Z, Z, C.c_int, Z, Z, P, P, P, Z, P, Z, Z, C.POINTER(KvCacheC), P, Z, Z, C.c_float, Z,
+                                           P, Z, P]
+    lib.kdnn_b200_prompt_attention.argtypes = [P, Z, Z, P, Z, Z, P, Z, Z, C.c_int, Z, Z, Z, Z, P, Z, P, Z, Z, C.c_float, Z, P]
     return lib
 
 
@@ -745,6 +763,177 @@ def moe_block_routing(workspace: torch.Tensor, tokens_local: int, world: int, to
                                            tokens_local, world, top_k, H, F, n_experts, idx.data_ptr(), wts.data_ptr(),
                                            _stream()), "moe_block_routing")
     return idx, wts
+
+
+# ---------------------------------------------------------------------------
+# attention: paged 8-bit cache and packed prompts (src/KokkosDNN_Attention.hpp, src/KokkosDNN_KVCache.hpp)
+def _here(what: str, *tensors: torch.Tensor) -> None:
+    """Every tensor on the current CUDA device, where the launch goes."""
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if not t.is_cuda or t.device.index != dev:
+            raise ValueError(f"{what}: tensors must live on the current CUDA device")
+
+
+def _ints(what: str, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous int32")
+
+
+def _packed(what: str, name: str, t: torch.Tensor, heads: Optional[int], dim: Optional[int]):
+    """(row pitch, head pitch) of a [rows, heads, dim] tensor whose heads are contiguous rows."""
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{what}: {name} must be [rows, heads, dim]")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{what}: {name} must have unit stride in its last dimension")
+    hd = t.stride(1) if t.shape[1] > 1 else t.shape[2]
+    return (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] - 1) * hd + t.shape[2])), hd
+
+
+@dataclass
+class KvPlan:
+    """What kv_plan writes for one step: where its rows start, which positions and places of the cache they take.
+    ``lens`` and ``state`` are the sequences' lengths and the pool's state after the step."""
+    row_start: torch.Tensor   # int32 [seqs + 1]
+    first: torch.Tensor       # int32 [seqs]
+    lens: torch.Tensor        # int32 [seqs]
+    state: torch.Tensor       # int32 [4]: first free ring entry, free pages, rows without a slot, page writes
+    slots: torch.Tensor       # int32 [rows]
+    writes: torch.Tensor      # int32 [kv_writes(rows, seqs, page), 4]
+    page: int
+
+    @staticmethod
+    def empty(seqs: int, rows: int, page: int, device="cuda") -> "KvPlan":
+        def ints(*shape):
+            return torch.zeros(shape, dtype=torch.int32, device=device)
+        return KvPlan(ints(seqs + 1), ints(seqs), ints(seqs), ints(4), ints(rows), ints(kv_writes(rows, seqs, page), 4), page)
+
+    @property
+    def seqs(self) -> int:
+        return self.first.shape[0]
+
+    @property
+    def rows(self) -> int:
+        return self.slots.shape[0]
+
+
+@dataclass
+class KvCache:
+    """One layer's paged cache: int8 codes [pages, kv_heads, page, dim] and a power-of-two scale per page and head."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor     # float32 [pages, kv_heads]
+    v_scale: torch.Tensor
+
+    def __post_init__(self):
+        if self.k.dim() != 4 or self.k.shape != self.v.shape or self.k.dtype != torch.int8 or self.v.dtype != torch.int8:
+            raise ValueError("KvCache: codes must be int8 [pages, kv_heads, page, dim]")
+        if tuple(self.k_scale.shape) != tuple(self.k.shape[:2]) or self.v_scale.shape != self.k_scale.shape or \
+                self.k_scale.dtype != torch.float32 or self.v_scale.dtype != torch.float32:
+            raise ValueError("KvCache: scales must be float32 [pages, kv_heads]")
+        if not all(t.is_contiguous() for t in (self.k, self.v, self.k_scale, self.v_scale)):
+            raise ValueError("KvCache: tensors must be contiguous")
+        self.pages, self.kv_heads, self.page, self.dim = self.k.shape
+        self.c = KvCacheC(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.pages,
+                          self.kv_heads, self.page, self.dim)
+
+    @staticmethod
+    def empty(pages: int, kv_heads: int, page: int, dim: int, device="cuda") -> "KvCache":
+        codes = [torch.zeros((pages, kv_heads, page, dim), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+        return KvCache(*codes, *scales)
+
+
+def kv_writes(rows: int, seqs: int, page: int) -> int:
+    return int(lib.kdnn_b200_kv_writes(rows, seqs, page))
+
+
+def kv_plan(fresh: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, ring: torch.Tensor, state: torch.Tensor,
+            plan: KvPlan) -> None:
+    """Pages, slots and row offsets of one step into ``plan`` (see kdnn_b200_kv_plan): ``fresh[b]`` new tokens for every
+    sequence (negative: it has ended and gives its pages back), ``lens`` tokens cached, ``table`` [seqs, columns] the page
+    numbers, ``ring`` the pool's free pages and ``state`` its position. ``lens`` may be ``plan.lens`` and ``state``
+    ``plan.state``: then the call moves the pool from step to step in place."""
+    seqs, rows = plan.first.shape[0], plan.slots.shape[0]
+    if tuple(fresh.shape) != (seqs,) or tuple(lens.shape) != (seqs,) or table.dim() != 2 or table.shape[0] != seqs or \
+            tuple(plan.lens.shape) != (seqs,) or tuple(plan.row_start.shape) != (seqs + 1,) or state.numel() != 4 or \
+            plan.state.numel() != 4 or ring.dim() != 1 or plan.writes.dim() != 2 or plan.writes.shape[1] != 4:
+        raise ValueError("kv_plan: dimension mismatch")
+    _ints("kv_plan", fresh=fresh, lens=lens, ring=ring, state=state, row_start=plan.row_start, first=plan.first,
+          plan_lens=plan.lens, plan_state=plan.state, slots=plan.slots, writes=plan.writes)
+    if table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError("kv_plan: table must be int32 with unit stride in its last dimension")
+    _here("kv_plan", fresh, lens, table, ring, state, plan.row_start, plan.slots, plan.writes)
+    rc = lib.kdnn_b200_kv_plan(fresh.data_ptr(), lens.data_ptr(), seqs, plan.page, rows, table.data_ptr(),
+                               table.stride(0) if seqs > 1 else table.shape[1], table.shape[1], ring.data_ptr(), ring.shape[0],
+                               state.data_ptr(), plan.row_start.data_ptr(), plan.first.data_ptr(), plan.lens.data_ptr(),
+                               plan.state.data_ptr(), plan.slots.data_ptr(), plan.writes.data_ptr(), plan.writes.shape[0], _stream())
+    _check(rc, "kv_plan")
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, plan: KvPlan, cache: KvCache) -> None:
+    """The step's keys and values [rows, kv_heads, dim] into the places that ``plan`` gives them (see kdnn_b200_kv_append)."""
+    ldk, hdk = _packed("kv_append", "k", k, cache.kv_heads, cache.dim)
+    ldv, hdv = _packed("kv_append", "v", v, cache.kv_heads, cache.dim)
+    if k.shape[0] != plan.rows or v.shape[0] != plan.rows or k.dtype != v.dtype:
+        raise ValueError("kv_append: k and v must have the plan's rows and one Scalar")
+    if cache.page != plan.page:
+        raise ValueError("kv_append: cache and plan have pages of different size")
+    _ints("kv_append", writes=plan.writes)
+    _here("kv_append", k, v, plan.writes, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    _check(lib.kdnn_b200_kv_append(k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(k), k.shape[0], plan.writes.data_ptr(),
+                                   plan.writes.shape[0], C.byref(cache.c), _stream()), "kv_append")
+
+
+def kv_attention_workspace_bytes(rows: int, seqs: int, heads: int, kv_heads: int, dim: int) -> int:
+    return int(lib.kdnn_b200_kv_attention_workspace_bytes(rows, seqs, heads, kv_heads, dim))
+
+
+def kv_attention(q: torch.Tensor, plan: KvPlan, table: torch.Tensor, cache: KvCache, out: torch.Tensor, workspace: torch.Tensor,
+                 scale: Optional[float] = None, window: int = 0) -> None:
+    """Causal grouped attention of the step's rows over the cached tokens of their sequences, their own among them (see
+    kdnn_b200_kv_attention); ``scale`` defaults to dim ** -0.5, ``window`` 0 looks back without limit."""
+    ldq, hdq = _packed("kv_attention", "q", q, None, cache.dim)
+    rows, heads = q.shape[0], q.shape[1]
+    ldo, hdo = _packed("kv_attention", "out", out, heads, cache.dim)
+    seqs = plan.first.shape[0]
+    if out.shape[0] != rows or rows != plan.rows or out.dtype != q.dtype:
+        raise ValueError("kv_attention: q and out must have the plan's rows and one Scalar")
+    if table.dim() != 2 or table.shape[0] != seqs or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError("kv_attention: table must be int32 [seqs, columns] with unit stride in its last dimension")
+    if cache.page != plan.page or window < 0:
+        raise ValueError("kv_attention: cache and plan have pages of different size, or the window is negative")
+    _ints("kv_attention", row_start=plan.row_start, first=plan.first, lens=plan.lens)
+    _here("kv_attention", q, out, table, workspace, plan.row_start, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    _check(lib.kdnn_b200_kv_attention(q.data_ptr(), ldq, hdq, _scalar(q), rows, heads, plan.row_start.data_ptr(), plan.first.data_ptr(),
+                                      plan.lens.data_ptr(), seqs, table.data_ptr(), table.stride(0) if seqs > 1 else table.shape[1],
+                                      table.shape[1], C.byref(cache.c), out.data_ptr(), ldo, hdo,
+                                      cache.dim ** -0.5 if scale is None else float(scale), window, workspace.data_ptr(),
+                                      workspace.numel() * workspace.element_size(), _stream()), "kv_attention")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_start: torch.Tensor, out: torch.Tensor,
+                     scale: Optional[float] = None, window: int = 0) -> None:
+    """Causal grouped attention over packed prompts (see kdnn_b200_prompt_attention): q, out [rows, heads, dim], k, v
+    [rows, kv_heads, dim], ``row_start`` int32 [seqs + 1]; ``scale`` defaults to dim ** -0.5."""
+    what = "prompt_attention"
+    ldq, hdq = _packed(what, "q", q, None, None)
+    rows, heads, dim = q.shape
+    ldk, hdk = _packed(what, "k", k, None, dim)
+    kv_heads = k.shape[1]
+    ldv, hdv = _packed(what, "v", v, kv_heads, dim)
+    ldo, hdo = _packed(what, "out", out, heads, dim)
+    if k.shape[0] != rows or v.shape[0] != rows or out.shape[0] != rows or k.dtype != q.dtype or v.dtype != q.dtype or \
+            out.dtype != q.dtype:
+        raise ValueError(f"{what}: q, k, v and out must have the same rows and one Scalar")
+    if row_start.dim() != 1 or row_start.shape[0] < 1 or window < 0:
+        raise ValueError(f"{what}: row_start must be [seqs + 1] and the window not negative")
+    _ints(what, row_start=row_start)
+    _here(what, q, k, v, out, row_start)
+    _check(lib.kdnn_b200_prompt_attention(q.data_ptr(), ldq, hdq, k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(q), rows,
+                                          heads, kv_heads, dim, row_start.data_ptr(), row_start.shape[0] - 1, out.data_ptr(), ldo, hdo,
+                                          dim ** -0.5 if scale is None else float(scale), window, _stream()), what)
 
 
 def read_probe(buf: torch.Tensor, sink: torch.Tensor) -> None:

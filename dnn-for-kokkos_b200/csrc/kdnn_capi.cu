@@ -60,6 +60,14 @@ cudaError_t dequant_launch(uint32_t dt, const void* w, size_t rows, size_t cols,
                            cudaStream_t st);
 cudaError_t residual_rmsnorm_launch(const void* h, size_t ldh, const float* y, size_t ldy, void* out,
                                     size_t ldo, size_t T, size_t H, float eps, int scalar, cudaStream_t st);
+cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int32_t* state, int32_t* table, size_t ldt, size_t cols,
+                           int32_t* ring, size_t pages, size_t B, size_t page, size_t rows, int32_t* row_start, int32_t* first,
+                           int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t most, cudaStream_t st);
+cudaError_t kv_append_launch(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
+                             const int32_t* writes, size_t most, const kdnn_b200_kv_cache* c, cudaStream_t st);
+size_t kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t heads, size_t kv_heads, size_t dim);
+cudaError_t kv_attention_launch(const AttnArgs& a, const kdnn_b200_kv_cache* c, void* ws, cudaStream_t st);
+cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st);
 }  // namespace kdnn
 
 namespace {
@@ -116,6 +124,17 @@ void* mapped_host_pointer(const void* host) {
 // kdnn_b200_quant_gemv_host moves x and y with copy_bytes_kernel when the host buffers allow it
 // (measured on the three decode GEMVs: 1972 GB/s end to end against 1245 GB/s with the copy engine);
 // kdnn_b200_host_copy_by_kernel(0) keeps cudaMemcpyAsync for everything.
+bool page_ok(size_t page) { return page == 16 || page == 32 || page == 64 || page == 128; }
+// rows of `heads` heads of `dim` elements: nothing of a row lies behind its pitch
+bool heads_fit(size_t ld, size_t hd, size_t heads, size_t dim) { return heads > 0 && hd >= dim && (heads - 1) <= (ld - dim) / hd && ld >= dim; }
+const char* cache_fault(const kdnn_b200_kv_cache* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return "null cache";
+  if (!page_ok(c->page)) return "pages hold 16, 32, 64 or 128 tokens";
+  if (c->dim == 0 || c->dim % 16 != 0 || c->dim > 256) return "dim must be a multiple of 16 up to 256";
+  if (c->kv_heads == 0 || c->pages == 0 || c->pages > static_cast<size_t>(INT_MAX) / c->page) return "dimension mismatch";
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) return "codes are not 16-byte aligned";
+  return nullptr;
+}
 std::atomic<int> g_host_copy_kernel{1};
 bool host_copy_by_kernel() { return g_host_copy_kernel.load(std::memory_order_relaxed) != 0; }
 }  // namespace
@@ -555,6 +574,95 @@ int kdnn_b200_quant_gemv_fp(uint32_t ggml_type, const void* w, size_t rows, size
   return cuda_result(kdnn::gemv_fp_launch(ggml_type, w, rows, cols, x, x_scalar, y, y_scalar,
                                           static_cast<cudaStream_t>(stream)),
                      "quant_gemv_fp");
+}
+
+size_t kdnn_b200_kv_writes(size_t rows, size_t seqs, size_t page) {
+  if (page == 0) return 0;
+  const size_t most = rows / page + 2 * seqs < rows ? rows / page + 2 * seqs : rows;
+  return most ? most : 1;
+}
+
+int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, size_t page, size_t rows, int32_t* table, size_t ldt,
+                      size_t table_cols, int32_t* ring, size_t pages, const int32_t* state, int32_t* row_start, int32_t* first,
+                      int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t writes_entries, void* stream) {
+  if (!page_ok(page)) return fail(KDNN_ERR_INVALID, "kv_plan: pages hold 16, 32, 64 or 128 tokens");
+  if (seqs > 8192 || rows > static_cast<size_t>(INT_MAX) || pages == 0 || pages > static_cast<size_t>(INT_MAX) / page || table_cols == 0 ||
+      table_cols > static_cast<size_t>(INT_MAX) / page || ldt < table_cols)
+    return fail(KDNN_ERR_INVALID, "kv_plan: dimension mismatch");
+  if (seqs == 0) return fail(KDNN_ERR_INVALID, "kv_plan: no sequences");
+  if (!fresh || !lens || !table || !ring || !state || !row_start || !first || !lens_out || !state_out || (rows && !slots) || !writes ||
+      (reinterpret_cast<uintptr_t>(writes) & 15u))
+    return fail(KDNN_ERR_INVALID, "kv_plan: null or misaligned argument");
+  if (writes_entries < kdnn_b200_kv_writes(rows, seqs, page) || writes_entries > static_cast<size_t>(INT_MAX) / 4)
+    return fail(KDNN_ERR_INVALID, "kv_plan: writes holds fewer entries than kv_writes() says");
+  return cuda_result(kdnn::kv_plan_launch(fresh, lens, state, table, ldt, table_cols, ring, pages, seqs, page, rows, row_start, first,
+                                          lens_out, state_out, slots, writes, writes_entries, static_cast<cudaStream_t>(stream)),
+                     "kv_plan");
+}
+
+int kdnn_b200_kv_append(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
+                        const int32_t* writes, size_t writes_entries, const kdnn_b200_kv_cache* cache, void* stream) {
+  if (!scalar_ok(scalar)) return fail(KDNN_ERR_INVALID, "kv_append: scalar must be KDNN_F32 or KDNN_BF16");
+  if (const char* why = cache_fault(cache)) return fail(KDNN_ERR_INVALID, std::string("kv_append: ") + why);
+  if (rows == 0 || writes_entries == 0) return KDNN_OK;
+  if (!k || !v || !writes || (reinterpret_cast<uintptr_t>(writes) & 15u) || rows > static_cast<size_t>(INT_MAX) ||
+      writes_entries > static_cast<size_t>(INT_MAX))
+    return fail(KDNN_ERR_INVALID, "kv_append: bad argument");
+  if (cache->kv_heads > 65535 || !heads_fit(ldk, hdk, cache->kv_heads, cache->dim) || !heads_fit(ldv, hdv, cache->kv_heads, cache->dim))
+    return fail(KDNN_ERR_INVALID, "kv_append: dimension mismatch");
+  return cuda_result(kdnn::kv_append_launch(k, ldk, hdk, v, ldv, hdv, scalar, rows, writes, writes_entries, cache,
+                                            static_cast<cudaStream_t>(stream)),
+                     "kv_append");
+}
+
+size_t kdnn_b200_kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t heads, size_t kv_heads, size_t dim) {
+  return kdnn::kv_attention_workspace_bytes(rows, seqs, heads, kv_heads, dim);
+}
+
+int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, size_t rows, size_t heads, const int32_t* row_start,
+                           const int32_t* first, const int32_t* lens, size_t seqs, const int32_t* table, size_t ldt,
+                           size_t table_cols, const kdnn_b200_kv_cache* cache, void* out, size_t ldo, size_t hdo, float scale,
+                           size_t window, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!scalar_ok(scalar)) return fail(KDNN_ERR_INVALID, "kv_attention: scalar must be KDNN_F32 or KDNN_BF16");
+  if (const char* why = cache_fault(cache)) return fail(KDNN_ERR_INVALID, std::string("kv_attention: ") + why);
+  if (rows == 0 || seqs == 0 || heads == 0) return KDNN_OK;
+  if (heads % cache->kv_heads != 0 || heads > 65535 || !heads_fit(ldq, hdq, heads, cache->dim) || !heads_fit(ldo, hdo, heads, cache->dim))
+    return fail(KDNN_ERR_INVALID, "kv_attention: dimension mismatch");
+  if (rows > static_cast<size_t>(INT_MAX) / heads || seqs > 8192 || table_cols == 0 || ldt < table_cols ||
+      table_cols > static_cast<size_t>(INT_MAX) / cache->page)
+    return fail(KDNN_ERR_INVALID, "kv_attention: dimension mismatch");
+  if (!q || !row_start || !first || !lens || !table || !out || !workspace) return fail(KDNN_ERR_INVALID, "kv_attention: null argument");
+  if (workspace_bytes < kdnn::kv_attention_workspace_bytes(rows, seqs, heads, cache->kv_heads, cache->dim) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(KDNN_ERR_INVALID, "kv_attention: workspace too small or not 256-byte aligned");
+  kdnn::AttnArgs a{};
+  a.q = q; a.ldq = ldq; a.hdq = hdq; a.out = out; a.ldo = ldo; a.hdo = hdo; a.scalar = scalar;
+  a.rows = static_cast<int>(rows); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(cache->kv_heads);
+  a.dim = static_cast<int>(cache->dim); a.seqs = static_cast<int>(seqs);
+  a.row_start = row_start; a.first = first; a.lens = lens; a.table = table; a.ldt = ldt; a.cols = static_cast<int>(table_cols);
+  a.scale = scale; a.window = static_cast<int>(window > static_cast<size_t>(INT_MAX) ? 0 : window);
+  return cuda_result(kdnn::kv_attention_launch(a, cache, workspace, static_cast<cudaStream_t>(stream)), "kv_attention");
+}
+
+int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv,
+                               size_t hdv, int scalar, size_t rows, size_t heads, size_t kv_heads, size_t dim,
+                               const int32_t* row_start, size_t seqs, void* out, size_t ldo, size_t hdo, float scale, size_t window,
+                               void* stream) {
+  if (!scalar_ok(scalar)) return fail(KDNN_ERR_INVALID, "prompt_attention: scalar must be KDNN_F32 or KDNN_BF16");
+  if (dim == 0 || dim % 8 != 0 || dim > 256) return fail(KDNN_ERR_INVALID, "prompt_attention: dim must be a multiple of 8 up to 256");
+  if (rows == 0 || seqs == 0 || heads == 0) return KDNN_OK;
+  if (kv_heads == 0 || heads % kv_heads != 0 || heads > 65535 || !heads_fit(ldq, hdq, heads, dim) || !heads_fit(ldo, hdo, heads, dim) ||
+      !heads_fit(ldk, hdk, kv_heads, dim) || !heads_fit(ldv, hdv, kv_heads, dim))
+    return fail(KDNN_ERR_INVALID, "prompt_attention: dimension mismatch");
+  if (rows > static_cast<size_t>(INT_MAX) / heads || seqs > 8192) return fail(KDNN_ERR_INVALID, "prompt_attention: too many rows or sequences");
+  if (!q || !k || !v || !row_start || !out) return fail(KDNN_ERR_INVALID, "prompt_attention: null argument");
+  kdnn::AttnArgs a{};
+  a.q = q; a.ldq = ldq; a.hdq = hdq; a.k = k; a.ldk = ldk; a.hdk = hdk; a.v = v; a.ldv = ldv; a.hdv = hdv;
+  a.out = out; a.ldo = ldo; a.hdo = hdo; a.scalar = scalar;
+  a.rows = static_cast<int>(rows); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
+  a.dim = static_cast<int>(dim); a.seqs = static_cast<int>(seqs); a.row_start = row_start;
+  a.scale = scale; a.window = static_cast<int>(window > static_cast<size_t>(INT_MAX) ? 0 : window);
+  return cuda_result(kdnn::prompt_attention_launch(a, static_cast<cudaStream_t>(stream)), "prompt_attention");
 }
 
 }  // extern "C"

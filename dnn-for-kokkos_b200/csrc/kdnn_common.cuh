@@ -412,6 +412,18 @@ struct BlockArgs {
   void* ws;
 };
 
+// Arguments of one attention call (kdnn_capi.cu validates and fills them). Pitches in elements.
+struct AttnArgs {
+  const void* q; size_t ldq, hdq;
+  const void* k; size_t ldk, hdk;              // packed prompts alone
+  const void* v; size_t ldv, hdv;
+  void* out; size_t ldo, hdo;
+  int scalar, rows, heads, kv_heads, dim, seqs;
+  const int32_t *row_start, *first, *lens, *table;   // first, lens, table: the cache alone
+  size_t ldt; int cols;
+  float scale; int window;                     // window 0: none
+};
+
 // cudaFuncAttributeMaxDynamicSharedMemorySize belongs to the (kernel, device) pair, so a host thread that
 // moves to another device must set it there too: one bit per device, set on the first launch there.
 struct SmemAttrOnce {

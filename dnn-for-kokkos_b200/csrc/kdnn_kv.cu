@@ -1,0 +1,324 @@
+// The paged 8-bit key / value cache: page plan of a step (block table, slot map, page writes) and the write of new
+// rows. No counterpart in the reference's hot path; its int8 cache is src/KokkosDNN_KVCache.hpp.
+//
+// A page holds `page` tokens of every head as int8 codes [head][token][dim] and one power-of-two scale per head for
+// keys and one for values: x = code * scale. A power of two makes every operation of the cache exact but the rounding
+// of a code itself, so the same rows give the same cache on any machine, a page whose scale has to grow moves its
+// older codes by a shift, and the attention kernel applies scales without error.
+#include "kdnn_common.cuh"
+
+namespace kdnn {
+
+// ---- page plan ------------------------------------------------------------------------------------------
+// Per sequence b, cached tokens L, fresh tokens n (negative: the sequence has ended and gives its pages back):
+//   row_start = min(cumsum max(n, 0), rows), m = its difference; have = ceil(L / page);
+//   need = min(ceil((L + m) / page), cols) - have; pages are handed out in sequence order while there are any:
+//   got = clamp(available - sum of the needs before, 0, need); stored = min(m, (have + got) page - L).
+// Everything is a prefix sum over the sequences followed by independent entries, so each CTA of a small cluster
+// forms the sums for itself in shared memory and writes its share of the entries; the cluster barrier lies between the
+// last read of lens / state and their new values, which may go to the same arrays.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanCluster = 8;
+
+struct PlanArgs {
+  const int32_t *fresh, *lens, *state;
+  int32_t *table, *ring, *row_start, *first, *lens_out, *state_out, *slots;
+  int4* writes;
+  size_t ldt;
+  int B, page, rows, cols, pages, most;
+};
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+// Exclusive sum over the block's threads of one 64-bit value each; `total` comes back to everybody.
+__device__ __forceinline__ long long block_exclusive(long long v, long long* warps, long long& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();   // the sums of the call before have been read
+  if (lane == 31) warps[w] = inc;
+  __syncthreads();
+  long long base = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanThreads / 32; ++i) {
+    const long long s = warps[i];
+    if (i < w) base += s;
+    total += s;
+  }
+  return base + inc - v;
+}
+
+// Largest b with at[b] <= x, for at[0] = 0 <= x < at[n]
+__device__ __forceinline__ int upper_of(const int* at, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
+  pdl_chain_entry();
+  extern __shared__ int sm[];
+  __shared__ long long s_warps[kPlanThreads / 32];
+  const int B = a.B, page = a.page;
+  int* rs   = sm;              // [B + 1] first row of a sequence
+  int* tk   = rs + B + 1;      // [B + 1] pages taken before it
+  int* gv   = tk + B + 1;      // [B + 1] pages given back before it
+  int* wr   = gv + B + 1;      // [B + 1] page writes before it
+  int* len  = wr + B + 1;      // [B] tokens it holds (of an ended one: what it gives back)
+  int* stor = len + B;         // [B] fresh tokens that get a slot; -1: ended
+  const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(B, static_cast<int>(threadIdx.x) * per), b1 = min(B, b0 + per);
+  const int head = ((a.state[0] % a.pages) + a.pages) % a.pages, avail = max(0, min(a.pages, a.state[1]));
+
+  long long n = 0, total, all;
+  for (int b = b0; b < b1; ++b) {
+    const int f = a.fresh[b];
+    stor[b] = f;
+    len[b]  = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.cols) * page)));
+    n += max(f, 0);
+  }
+  long long at = block_exclusive(n, s_warps, all);
+  for (int b = b0; b < b1; ++b) {
+    rs[b] = static_cast<int>(min(at, static_cast<long long>(a.rows)));
+    at += max(stor[b], 0);
+  }
+  if (threadIdx.x == 0) rs[B] = static_cast<int>(min(all, static_cast<long long>(a.rows)));
+  __syncthreads();
+
+  auto held  = [&](int b) { return (len[b] + page - 1) / page; };
+  auto wants = [&](int b) {
+    if (stor[b] < 0) return 0;
+    const long long to = static_cast<long long>(len[b]) + (rs[b + 1] - rs[b]);
+    return static_cast<int>(min((to + page - 1) / page, static_cast<long long>(a.cols))) - held(b);
+  };
+  long long need = 0, back = 0;
+  for (int b = b0; b < b1; ++b) {
+    need += wants(b);
+    back += stor[b] < 0 ? held(b) : 0;
+  }
+  long long take = block_exclusive(need, s_warps, total), give = block_exclusive(back, s_warps, total);
+  const int given = static_cast<int>(min(total, static_cast<long long>(a.pages)));
+  long long put = 0, kept = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int w = wants(b), h = held(b);
+    const long long left = avail - take;
+    const int got = static_cast<int>(left <= 0 ? 0 : left < w ? left : w);
+    tk[b] = static_cast<int>(min(take, static_cast<long long>(avail)));
+    gv[b] = static_cast<int>(min(give, static_cast<long long>(a.pages)));
+    take += w;
+    if (stor[b] < 0) {
+      give += h;
+      continue;
+    }
+    const int st = static_cast<int>(min(static_cast<long long>(rs[b + 1] - rs[b]), static_cast<long long>(h + got) * page - len[b]));
+    stor[b] = st;
+    kept += st;
+    put += st > 0 ? (len[b] + st - 1) / page - len[b] / page + 1 : 0;
+  }
+  long long stored;
+  block_exclusive(kept, s_warps, stored);
+  long long w0 = block_exclusive(put, s_warps, total);
+  const int touched = static_cast<int>(min(total, static_cast<long long>(a.most)));
+  for (int b = b0; b < b1; ++b) {
+    wr[b] = static_cast<int>(min(w0, static_cast<long long>(a.most)));
+    w0 += stor[b] > 0 ? (len[b] + stor[b] - 1) / page - len[b] / page + 1 : 0;
+  }
+  if (threadIdx.x == kPlanThreads - 1) {
+    tk[B] = static_cast<int>(min(take, static_cast<long long>(avail)));
+    gv[B] = given;
+    wr[B] = touched;
+  }
+  __syncthreads();
+  const int taken = tk[B];
+
+  // the j-th page of sequence b: what the table holds, or the ring's next ones
+  auto page_of = [&](int b, int j) {
+    const int h = held(b);
+    return j < h ? a.table[static_cast<size_t>(b) * a.ldt + j]
+                 : a.ring[static_cast<int>((static_cast<long long>(head) + tk[b] + j - h) % a.pages)];
+  };
+  const int step = static_cast<int>(cluster_size()) * kPlanThreads, me = static_cast<int>(cluster_rank()) * kPlanThreads + threadIdx.x;
+  for (int p = me; p < taken; p += step) {
+    const int b = upper_of(tk, B, p);
+    a.table[static_cast<size_t>(b) * a.ldt + held(b) + p - tk[b]] = a.ring[static_cast<int>((static_cast<long long>(head) + p) % a.pages)];
+  }
+  for (int p = me; p < given; p += step) {
+    const int b = upper_of(gv, B, p);
+    a.ring[static_cast<int>((static_cast<long long>(head) + avail + p) % a.pages)] = a.table[static_cast<size_t>(b) * a.ldt + p - gv[b]];
+  }
+  for (int w = me; w < a.most; w += step) {
+    int4 e = make_int4(0, 0, 0, 0);
+    if (w < touched) {
+      const int b = upper_of(wr, B, w), j = len[b] / page + w - wr[b];
+      const int lo = max(j * page, len[b]);
+      const int hi = static_cast<int>(min((static_cast<long long>(j) + 1) * page, static_cast<long long>(len[b]) + stor[b]));
+      e = make_int4(rs[b] + lo - len[b], hi - lo, page_of(b, j), lo - j * page);
+    }
+    a.writes[w] = e;
+  }
+  const int rows = rs[B];
+  for (int r0 = me * 4; r0 < a.rows; r0 += step * 4) {   // four rows per search
+    int b = r0 < rows ? upper_of(rs, B, r0) : 0;
+    for (int r = r0; r < min(r0 + 4, a.rows); ++r) {
+      int slot = -1;
+      if (r < rows) {
+        while (r >= rs[b + 1]) ++b;
+        const int i = r - rs[b];
+        if (i < stor[b]) {
+          const int pos = len[b] + i, pg = page_of(b, pos / page);
+          if (pg >= 0 && pg < a.pages) slot = pg * page + pos % page;
+        }
+      }
+      a.slots[r] = slot;
+    }
+  }
+  if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
+  if (cluster_rank() == 0) {
+    for (int b = threadIdx.x; b < B; b += kPlanThreads) {
+      const bool ended = stor[b] < 0;
+      a.row_start[b] = rs[b];
+      a.first[b]     = ended ? 0 : len[b];
+      a.lens_out[b]  = ended ? 0 : len[b] + stor[b];
+    }
+    if (threadIdx.x == 0) {
+      a.row_start[B]   = rows;
+      a.state_out[0]   = (head + taken) % a.pages;
+      a.state_out[1]   = avail - taken + given;
+      a.state_out[2]   = static_cast<int>(min(all - stored, 0x7fffffffLL));
+      a.state_out[3]   = touched;
+    }
+  }
+}
+
+cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int32_t* state, int32_t* table, size_t ldt, size_t cols,
+                           int32_t* ring, size_t pages, size_t B, size_t page, size_t rows, int32_t* row_start, int32_t* first,
+                           int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t most, cudaStream_t st) {
+  PlanArgs a{fresh, lens, state, table, ring, row_start, first, lens_out, state_out, slots, reinterpret_cast<int4*>(writes), ldt,
+             static_cast<int>(B), static_cast<int>(page), static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
+             static_cast<int>(most)};
+  const int smem = static_cast<int>((6 * B + 4) * sizeof(int));
+  static SmemAttrOnce once;
+  cudaError_t e = set_max_smem_once(once, kv_plan_kernel, (6 * 8192 + 4) * 4);
+  if (e != cudaSuccess) return e;
+  // one CTA while its threads have a few rows each
+  const unsigned ctas = rows + most > 8 * kPlanThreads ? kPlanCluster : 1;
+  return launch_chained_cluster(kv_plan_kernel, dim3(ctas), dim3(kPlanThreads), smem, ctas, st, a);
+}
+
+// ---- new rows into the cache ---------------------------------------------------------------------------------
+struct AppendArgs {
+  const void* x[2];        // keys, values [rows][heads][dim]
+  size_t ld[2], hd[2];     // row and head pitch in elements
+  int8_t* codes[2];
+  float* scale[2];
+  const int4* writes;
+  int rows, pages, heads, page, dim;
+};
+
+// 2^e, -126 <= e <= 127
+__device__ __forceinline__ float pow2_of(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// The smallest power of two s with amax <= 127 s, at least 2^-100; 0 for 0. 127 / 128 of the next power of two is the
+// mantissa 0x7E0000.
+__device__ __forceinline__ float scale_for(float amax) {
+  if (!(amax > 0.0f)) return 0.0f;
+  const uint32_t u = __float_as_uint(amax);
+  const int e = static_cast<int>(u >> 23) - 127 - 6 + ((u & 0x7FFFFFu) > 0x7E0000u ? 1 : 0);
+  return pow2_of(max(e, -100));
+}
+// x / s for a power of two s (inv = 1 / s), to the nearest code; infinities are the largest code, NaN is 0.
+__device__ __forceinline__ int code_of(float x, float inv) {
+  const float q = rintf(__fmul_rn(x, inv));
+  return q != q ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
+}
+
+// One CTA per (page write, head, key or value).
+template <class XT>
+__global__ void __launch_bounds__(128) kv_append_kernel(AppendArgs a) {
+  pdl_chain_entry();
+  const int4 w = a.writes[blockIdx.x];
+  const int row0 = w.x, count = w.y, pg = w.z, off = w.w;
+  // an entry without rows, or one that does not name a place of the cache
+  if (count <= 0 || row0 < 0 || row0 > a.rows - count || pg < 0 || pg >= a.pages || off < 0 || off > a.page - count) return;
+  const int h = blockIdx.y, z = blockIdx.z, D = a.dim;
+  const XT* x = static_cast<const XT*>(a.x[z]) + static_cast<size_t>(row0) * a.ld[z] + static_cast<size_t>(h) * a.hd[z];
+  const size_t ld = a.ld[z];
+  const size_t ph = static_cast<size_t>(pg) * a.heads + h;
+  int8_t* codes = a.codes[z] + ph * a.page * D;
+  const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ld * sizeof(XT))) & 15u) == 0;
+  const int per_row = D / 8, work = count * per_row;
+  float amax = 0.0f;
+  for (int i = threadIdx.x; i < work; i += blockDim.x) {
+    float v[8];
+    load8<XT>(x + static_cast<size_t>(i / per_row) * ld, static_cast<size_t>(i % per_row) * 8, vec, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float m = fabsf(v[k]);
+      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values alone
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  __shared__ float s_max[4];
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+  const float old = off > 0 ? a.scale[z][ph] : 0.0f;
+  __syncthreads();
+  amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  const float s = fmaxf(old, scale_for(amax)), inv = s > 0.0f ? 1.0f / s : 0.0f;
+  if (off > 0 && old != s) {   // the page's scale grows: older codes follow
+    const float ratio = __fmul_rn(old, inv);
+    for (int i = threadIdx.x; i < off * D / 16; i += blockDim.x) {
+      uint4 w = reinterpret_cast<uint4*>(codes)[i];
+      uint32_t* u = &w.x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          r |= (static_cast<uint32_t>(code_of(static_cast<float>(static_cast<int8_t>(u[k] >> (8 * j))), ratio)) & 0xFFu) << (8 * j);
+        u[k] = r;
+      }
+      reinterpret_cast<uint4*>(codes)[i] = w;
+    }
+  }
+  int8_t* mine = codes + static_cast<size_t>(off) * D;
+  for (int i = threadIdx.x; i < work; i += blockDim.x) {
+    float v[8];
+    load8<XT>(x + static_cast<size_t>(i / per_row) * ld, static_cast<size_t>(i % per_row) * 8, vec, v);
+    uint32_t r[2] = {0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r[k >> 2] |= (static_cast<uint32_t>(code_of(v[k], inv)) & 0xFFu) << (8 * (k & 3));
+    reinterpret_cast<uint2*>(mine)[i] = make_uint2(r[0], r[1]);
+  }
+  if (threadIdx.x == 0) a.scale[z][ph] = s;
+}
+
+cudaError_t kv_append_launch(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
+                             const int32_t* writes, size_t most, const kdnn_b200_kv_cache* c, cudaStream_t st) {
+  AppendArgs a{{k, v}, {ldk, ldv}, {hdk, hdv}, {c->k, c->v}, {c->k_scale, c->v_scale}, reinterpret_cast<const int4*>(writes),
+               static_cast<int>(rows), static_cast<int>(c->pages), static_cast<int>(c->kv_heads), static_cast<int>(c->page),
+               static_cast<int>(c->dim)};
+  const dim3 grid(static_cast<unsigned>(most), static_cast<unsigned>(c->kv_heads), 2);
+  return scalar == KDNN_F32 ? launch_chained(kv_append_kernel<float>, grid, dim3(128), 0, st, a)
+                            : launch_chained(kv_append_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+}
+
+}  // namespace kdnn

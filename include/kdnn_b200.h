@@ -405,6 +405,73 @@ int kdnn_b200_dequant_to_dense(uint32_t ggml_type, const void* w, size_t rows, s
 int kdnn_b200_quant_gemv_fp(uint32_t ggml_type, const void* w, size_t rows, size_t cols, const void* x,
                             int x_scalar, void* y, int y_scalar, void* stream);
 
+/* ---- attention: paged 8-bit cache and packed prompts ---------------------------------------------------
+ * What stands between the projections of a decoder layer. Rows of a step are PACKED: the new tokens of sequence b are
+ * rows row_start[b] .. row_start[b + 1] of q, k, v and out, in order. Rows behind the last sequence are neither read nor
+ * written. Lengths, tables and plans live on the device; nothing here waits for the host, so a step can be captured into
+ * a graph once and replayed while lengths change. In the reference: src/KokkosDNN_Attention.hpp (causal grouped-query,
+ * sliding window, int8 cache), src/KokkosDNN_KVCache.hpp. */
+
+/* One layer's cache: `pages` pages of `page` tokens (16, 32, 64 or 128), int8 codes [pages][kv_heads][page][dim], one
+ * scale per page and head, float [pages][kv_heads], a power of two or 0. A cached value is code * scale.
+ * dim: a multiple of 16 up to 256; codes 16-byte aligned; pages * page <= INT_MAX. */
+typedef struct {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  size_t pages, kv_heads, page, dim;
+} kdnn_b200_kv_cache;
+
+/* Entries of kdnn_b200_kv_plan's `writes` that hold every plan of this size: min(rows, rows / page + 2 seqs), at least 1. */
+size_t kdnn_b200_kv_writes(size_t rows, size_t seqs, size_t page);
+
+/* Page plan of one step, on the GPU, in one launch. Free pages are a ring: state = {first free entry, free pages, tokens
+ * of the last call that got no slot, page writes of the last call}; ring[(state[0] + i) % pages], i < state[1], are free.
+ *   fresh[b] >= 0: sequence b (lens[b] tokens cached) gets that many new tokens; < 0: it has ended, its pages go back to
+ *   the ring (usable from the next call on) and its length becomes 0.
+ * Written: row_start[seqs + 1]; first[b] = position of b's first new row; lens_out[b] = its tokens after this step; new
+ * pages in table[b][..]; slots[r] = page * page_size + place of row r in the cache, -1 for a row without one;
+ * writes[i] = {first row, rows, page number, first token in the page}, one per page that new rows fall on, the rest zero.
+ * Pages go to the sequences in order. Where the ring runs out, or a sequence outgrows table_cols pages, the sequence's last
+ * tokens get no slot: lens_out counts what is stored, state_out[2] what is not. More fresh tokens than `rows` are cut at
+ * `rows` and counted there too. lens_out may be lens and state_out may be state. Calls that share a pool must not overlap.
+ * seqs <= 8192, pages * page <= INT_MAX, table_cols * page <= INT_MAX. */
+int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, size_t page, size_t rows, int32_t* table, size_t ldt,
+                      size_t table_cols, int32_t* ring, size_t pages, const int32_t* state, int32_t* row_start, int32_t* first,
+                      int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t writes_entries, void* stream);
+
+/* New rows into the cache: k, v [rows][kv_heads][dim] Scalar with row and head pitches in elements, places from a plan's
+ * `writes`. A page's scale becomes the smallest power of two s >= 2^-100 with max|x| <= 127 s over its new rows, or stays
+ * what it was where that is larger; new codes are rint(x / s); older codes of the page are rint(code * old scale / s).
+ * A page that is written from its first token on starts over. Infinities take the largest code, NaN takes 0, and neither
+ * counts for the scale. An entry of `writes` that names no place of the cache writes nothing. */
+int kdnn_b200_kv_append(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
+                        const int32_t* writes, size_t writes_entries, const kdnn_b200_kv_cache* cache, void* stream);
+
+/* Bytes of workspace of kdnn_b200_kv_attention on the current device (256-byte aligned, contents need not be kept). */
+size_t kdnn_b200_kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t heads, size_t kv_heads, size_t dim);
+
+/* out[r][h] = sum_j softmax_j(scale q[r][h] . k_j) v_j over the cached tokens j of row r's sequence, head h / (heads /
+ * kv_heads): 0 <= j < lens[b], j <= pos, and j > pos - window where window > 0; pos = first[b] + r - row_start[b]. A row
+ * with no such token gives 0. The new rows themselves are read from the cache: append before this call. Tokens on a page
+ * that the table does not hold (a number outside [0, pages), or beyond table_cols) are left out.
+ * q, out [rows][heads][dim] Scalar with row and head pitches; out may be q. heads is a multiple of kv_heads. */
+int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, size_t rows, size_t heads, const int32_t* row_start,
+                           const int32_t* first, const int32_t* lens, size_t seqs, const int32_t* table, size_t ldt,
+                           size_t table_cols, const kdnn_b200_kv_cache* cache, void* out, size_t ldo, size_t hdo, float scale,
+                           size_t window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal grouped attention over packed prompts: row r of sequence b attends to the rows row_start[b] .. r (with window > 0:
+ * the last `window` of them). q, out [rows][heads][dim], k, v [rows][kv_heads][dim] Scalar with row and head pitches in
+ * elements; dim a multiple of 8 up to 256. Values in masked places (later rows, other sequences) do not reach the result,
+ * infinities and NaN included. Rows outside [row_start[0], row_start[seqs]) are left as they were. out must not overlap
+ * k or v. */
+int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void* k, size_t ldk, size_t hdk, const void* v,
+                               size_t ldv, size_t hdv, int scalar, size_t rows, size_t heads, size_t kv_heads, size_t dim,
+                               const int32_t* row_start, size_t seqs, void* out, size_t ldo, size_t hdo, float scale,
+                               size_t window, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

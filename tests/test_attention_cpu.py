@@ -1,0 +1,122 @@
+"""Refusals of the attention operators: every check comes before the first launch, so fake pointers are never touched."""
+import ctypes as C
+
+import pytest
+import torch
+
+P = 0x10000
+
+
+def _cache(kd, **kw):
+    a = dict(k=P, v=P, k_scale=P, v_scale=P, pages=8, kv_heads=2, page=64, dim=128)
+    a.update(kw)
+    return kd.KvCacheC(*(a[f[0]] for f in kd.KvCacheC._fields_))
+
+
+def test_writes_hold_every_plan(kd):
+    assert kd.kv_writes(0, 4, 64) == 1
+    assert kd.kv_writes(3, 64, 64) == 3                 # no more pages than rows
+    assert kd.kv_writes(1000, 2, 16) == 62 + 4
+    # a sequence of n rows touches at most n / page + 2 pages
+    for page in (16, 32, 64, 128):
+        for n in range(1, 300):
+            most = max((off + n - 1) // page + 1 for off in range(page))
+            assert most <= kd.kv_writes(n, 1, page)
+
+
+def test_plan_refusals(kd):
+    ok = dict(fresh=P, lens=P, seqs=4, page=64, rows=4, table=P, ldt=8, cols=8, ring=P, pages=32, state=P, row_start=P, first=P,
+              lens_out=P, state_out=P, slots=P, writes=P, entries=8)
+
+    def call(**kw):
+        return kd.lib.kdnn_b200_kv_plan(*dict(ok, **kw).values(), None)
+
+    for kw in (dict(page=48), dict(page=0), dict(seqs=0), dict(seqs=8193), dict(cols=0), dict(ldt=7), dict(pages=0),
+               dict(pages=2 ** 31 // 64), dict(cols=2 ** 31 // 64, ldt=2 ** 31), dict(rows=2 ** 31), dict(entries=3), dict(writes=P + 4),
+               *({n: None} for n in ("fresh", "lens", "table", "ring", "state", "row_start", "first", "lens_out", "state_out", "slots",
+                                     "writes"))):
+        assert call(**kw) == kd.KDNN_ERR_INVALID, kw
+        assert "kv_plan" in kd.last_error()
+
+
+def test_append_refusals(kd):
+    ok = dict(k=P, ldk=256, hdk=128, v=P, ldv=256, hdv=128, scalar=1, rows=4, writes=P, entries=4, cache=_cache(kd))
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        a["cache"] = C.byref(a["cache"]) if a["cache"] is not None else None
+        return kd.lib.kdnn_b200_kv_append(*a.values(), None)
+
+    for kw in (dict(scalar=2), dict(cache=None), dict(k=None), dict(v=None), dict(writes=None), dict(writes=P + 8), dict(ldk=255),
+               dict(hdk=127), dict(hdv=129), dict(rows=2 ** 31), *(dict(cache=_cache(kd, **c)) for c in (
+                   dict(k=None), dict(v_scale=None), dict(k=P + 8), dict(page=24), dict(dim=24), dict(dim=272), dict(dim=0),
+                   dict(kv_heads=0), dict(pages=0), dict(pages=2 ** 25)))):
+        assert call(**kw) == kd.KDNN_ERR_INVALID, kw
+        assert "kv_append" in kd.last_error()
+    assert call(rows=0) == kd.KDNN_OK and call(entries=0) == kd.KDNN_OK
+
+
+def test_cache_attention_refusals(kd):
+    ok = dict(q=P, ldq=512, hdq=128, scalar=1, rows=4, heads=4, row_start=P, first=P, lens=P, seqs=2, table=P, ldt=8, cols=8,
+              cache=_cache(kd), out=P, ldo=512, hdo=128, scale=0.1, window=0, ws=P, ws_bytes=1 << 40)
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        a["cache"] = C.byref(a["cache"]) if a["cache"] is not None else None
+        return kd.lib.kdnn_b200_kv_attention(*a.values(), None)
+
+    for kw in (dict(scalar=7), dict(heads=3), dict(heads=65536 * 2), dict(ldq=511), dict(hdq=100), dict(ldo=400), dict(ldt=4), dict(cols=0),
+               dict(seqs=8193), dict(rows=2 ** 30), dict(ws=P + 16), dict(cols=2 ** 31 // 64, ldt=2 ** 31), dict(cache=None),
+               dict(cache=_cache(kd, dim=8)), *({n: None} for n in ("q", "row_start", "first", "lens", "table", "out", "ws"))):
+        assert call(**kw) == kd.KDNN_ERR_INVALID, kw
+        assert "kv_attention" in kd.last_error()
+    for kw in (dict(rows=0), dict(seqs=0), dict(heads=0)):
+        assert call(**kw) == kd.KDNN_OK, kw
+
+
+def test_prompt_attention_refusals(kd):
+    ok = dict(q=P, ldq=512, hdq=128, k=P, ldk=256, hdk=128, v=P, ldv=256, hdv=128, scalar=1, rows=4, heads=4, kv_heads=2, dim=128,
+              row_start=P, seqs=2, out=P, ldo=512, hdo=128, scale=0.1, window=0)
+
+    def call(**kw):
+        return kd.lib.kdnn_b200_prompt_attention(*dict(ok, **kw).values(), None)
+
+    for kw in (dict(scalar=-1), dict(dim=0), dict(dim=12), dict(dim=264), dict(kv_heads=0), dict(kv_heads=3), dict(ldq=500), dict(hdk=64),
+               dict(ldv=200), dict(hdo=120), dict(seqs=8193), dict(rows=2 ** 30),
+               *({n: None} for n in ("q", "k", "v", "row_start", "out"))):
+        assert call(**kw) == kd.KDNN_ERR_INVALID, kw
+        assert "prompt_attention" in kd.last_error()
+    for kw in (dict(rows=0), dict(seqs=0), dict(heads=0)):
+        assert call(**kw) == kd.KDNN_OK, kw
+
+
+def test_python_checks(kd):
+    """Shapes, types and places are checked before the library is called; nothing here has a CUDA device."""
+    i32 = dict(dtype=torch.int32)
+    plan = kd.KvPlan.empty(2, 5, 16, device="cpu")
+    assert plan.seqs == 2 and plan.rows == 5 and tuple(plan.writes.shape) == (4, 4)
+    fresh, lens, table, ring, state = (torch.zeros(2, **i32), torch.zeros(2, **i32), torch.zeros(2, 3, **i32), torch.zeros(6, **i32),
+                                       torch.zeros(4, **i32))
+    for bad in ((fresh[:1], lens, table, ring, state), (fresh, lens.long(), table, ring, state), (fresh, lens, table[0], ring, state),
+                (fresh, lens, table, ring, state[:3]), (fresh, lens, table.t().contiguous().t(), ring, state),
+                (fresh, lens, table, ring, state)):        # the last one is right but for its place
+        with pytest.raises(ValueError):
+            kd.kv_plan(*bad, plan)
+    with pytest.raises(ValueError):
+        kd.KvCache(torch.zeros(2, 1, 16, 64), torch.zeros(2, 1, 16, 64), torch.zeros(2, 1), torch.zeros(2, 1))
+    cache = kd.KvCache.empty(4, 2, 16, 64, device="cpu")
+    k = torch.zeros(5, 2, 64)
+    for a, b in ((k[:4], k), (k, k.double()), (k[:, :1], k), (k[..., :32], k[..., :32]), (k.transpose(1, 2), k), (k, k)):
+        with pytest.raises(ValueError):
+            kd.kv_append(a, b, plan, cache)
+    q = torch.zeros(5, 4, 64)
+    ws = torch.zeros(16, dtype=torch.uint8)
+    for args, kw in (((q[:3], plan, table, cache, q), {}), ((q, plan, table[:1], cache, q), {}), ((q, plan, table, cache, q.bfloat16()), {}),
+                     ((q, plan, table, cache, q), dict(window=-1)), ((q, plan, table, cache, q), {})):
+        with pytest.raises(ValueError):
+            kd.kv_attention(*args, ws, **kw)
+    rs = torch.zeros(3, **i32)
+    for args in ((q, k, k[:4], rs, q), (q, k, k, rs.long(), q), (q[0], k, k, rs, q), (q, k, k.bfloat16(), rs, q), (q, k, k, rs, q[:, :2]),
+                 (q, k, k, rs, q)):
+        with pytest.raises(ValueError):
+            kd.prompt_attention(*args)
