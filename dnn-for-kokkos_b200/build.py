@@ -8,7 +8,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["kdnn_gemv.cu", "kdnn_gemm.cu", "kdnn_moe.cu", "kdnn_dequant.cu", "kdnn_elementwise.cu", "kdnn_kv.cu", "kdnn_attn.cu",
+SOURCES = ["kdnn_gemv.cu", "kdnn_gemm.cu", "kdnn_moe.cu", "kdnn_dequant.cu", "kdnn_elementwise.cu", "kdnn_kv.cu", "kdnn_kvattn.cu", "kdnn_attn.cu",
            "kdnn_capi.cu"]
 HEADERS = ["kdnn_common.cuh", "kdnn_tile.cuh", "kdnn_grouped.cuh", "kdnn_mma.cuh", "kdnn_tc.cuh", "kdnn_split.cuh", "kdnn_rowmma.cuh", os.path.join("..", "..", "include", "kdnn_b200.h")]
 LIB = os.path.join(HERE, "libkdnn_b200.so")

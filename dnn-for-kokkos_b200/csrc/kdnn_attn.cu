@@ -100,8 +100,6 @@ static cudaError_t launch_rows(const AttnArgs& a, const kdnn_b200_kv_cache* c, c
                               : launch_chained(attn_row_kernel<__nv_bfloat16, PAGED>, grid, dim3(128), 0, st, a, k, v, ks, vs, pages, page);
 }
 
-size_t kv_attention_workspace_bytes(size_t, size_t, size_t, size_t, size_t) { return 256; }
-cudaError_t kv_attention_launch(const AttnArgs& a, const kdnn_b200_kv_cache* c, void*, cudaStream_t st) { return launch_rows<true>(a, c, st); }
 cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) { return launch_rows<false>(a, nullptr, st); }
 
 }  // namespace kdnn
