@@ -1,0 +1,715 @@
+// Causal grouped attention over packed prompts (kdnn_b200_prompt_attention).
+//
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2(e),  m a running reference.
+//
+// prompt_tc_kernel (bf16, heads of up to 128, 16-byte aligned rows): 128 query rows of one kv head, a few tokens times the
+// heads of the group, are the M of a tcgen05 product, so a group shares every key and value that is fetched and a short
+// prompt fills its tile. A CTA owns two such tiles and walks the keys 128 at a time: TMA brings keys and values (two stages
+// each), S = Q K^T lands in TMEM, a warpgroup per tile turns it into weights (a thread owns a row: no shuffles) and
+// writes them back as bf16 over the scores, O += P V accumulates in TMEM. While one tile's scores go through the exponentials,
+// the tensor cores work for the other. The reference m moves, and O is rescaled, only when a score passes it by 2^8.
+// Weights are rounded to bf16 (2^-8 each, averaged over the keys); sums and references are fp32.
+// A product reads masked values with weight 0, so infinities or NaN there would reach the sum: a row that does not come out finite is
+// computed again from its own keys alone.
+//
+// prompt_tile_kernel (fp32, larger heads, any alignment): 64 query rows against 64 keys in shared memory, fp32 FMA pairs.
+#include "kdnn_tc.cuh"
+
+#include "kdnn_ring.cuh"
+
+namespace kdnn {
+
+cudaError_t moe_status_ptr(int** out);
+
+// ---- one row from its own keys: a warp, lanes over channels -------------------------------------------------------
+template <class ST>
+__device__ __forceinline__ void row_alone(const AttnArgs& a, int row0, int i, int h) {
+  const int lane = threadIdx.x & 31, D = a.dim, g = h / (a.heads / a.kv_heads);
+  const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(row0 + i) * a.ldq + static_cast<size_t>(h) * a.hdq;
+  float qv[8], o[8], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    qv[e] = e * 32 + lane < D ? to_f32(q[e * 32 + lane]) : 0.0f;
+    o[e] = 0.0f;
+  }
+  for (int j = a.window > 0 ? max(0, i - a.window + 1) : 0; j <= i; ++j) {
+    const ST* k = static_cast<const ST*>(a.k) + static_cast<size_t>(row0 + j) * a.ldk + static_cast<size_t>(g) * a.hdk;
+    const ST* v = static_cast<const ST*>(a.v) + static_cast<size_t>(row0 + j) * a.ldv + static_cast<size_t>(g) * a.hdv;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e * 32 + lane < D) s += qv[e] * to_f32(k[e * 32 + lane]);
+    s = warp_sum(s) * a.scale;
+    const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - (mn == -INFINITY ? 0.0f : mn));
+    l = l * f + p;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e * 32 + lane < D) o[e] = o[e] * f + p * to_f32(v[e * 32 + lane]);
+    m = mn;
+  }
+  ST* out = static_cast<ST*>(a.out) + static_cast<size_t>(row0 + i) * a.ldo + static_cast<size_t>(h) * a.hdo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e * 32 + lane < D) store_scalar(out + e * 32 + lane, o[e] / l);
+}
+
+// ---- which sequence and which part of it a CTA works on ---------------------------------------------------------------
+struct PromptItem {
+  int row0, n, part;   // first row and rows of the sequence, index of the part (the last parts, with the most keys, come first)
+};
+// `per`: rows of a part; item: this CTA's. All THREADS threads; false: there is no such item.
+template <int THREADS>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int item, PromptItem& it) {
+  __shared__ int s_warp[THREADS / 32];
+  __shared__ int4 s_found;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long left = item;
+  for (int b0 = 0; b0 < a.seqs; b0 += THREADS) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    int row0 = 0, n = 0;
+    if (b < a.seqs) {
+      row0 = max(a.row_start[b], 0);
+      n = max(min(a.row_start[b + 1], a.rows) - row0, 0);
+    }
+    const int parts = static_cast<int>((n + per - 1) / per);
+    int inc = parts;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) s_warp[w] = inc;
+    __syncthreads();
+    int base = 0, total = 0;
+    for (int k = 0; k < THREADS / 32; ++k) {
+      if (k < w) base += s_warp[k];
+      total += s_warp[k];
+    }
+    const long long at = left - (base + inc - parts);
+    if (at >= 0 && at < parts) s_found = make_int4(row0, n, parts - 1 - static_cast<int>(at), 0);
+    __syncthreads();
+    if (left < total) {
+      const int4 f = s_found;
+      it = PromptItem{f.x, f.y, f.z};
+      return true;
+    }
+    left -= total;
+  }
+  return false;
+}
+
+// ---- fp32 tiles -----------------------------------------------------------------------------------------------------------
+constexpr int kTileM = 64, kTileN = 64;
+template <int DM>
+struct TileShape {
+  static constexpr int kPitch = DM + 4, kPPitch = kTileN + 4;
+  static constexpr int kFloats = (kTileM + kTileN) * kPitch + kTileN * DM + kTileM * kPPitch;
+};
+
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) { return ffma2(a, b, c); }
+
+// Four channels of a row; channels behind D are 0.
+template <class ST>
+__device__ __forceinline__ float4 four_of(const ST* p, int d, int D, bool vec) {
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (d < D) load4<ST>(p, static_cast<size_t>(d), vec, v);
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Thread (ty, tx) of 16 x 16 holds rows 4 ty .. + 3 against keys tx + 16 i, and channels 4 tx + 64 i of the result.
+template <class ST, int DM>
+__global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(AttnArgs a) {
+  using S = TileShape<DM>;
+  pdl_chain_entry();
+  extern __shared__ __align__(16) float sf[];
+  float *sq = sf, *sk = sq + kTileM * S::kPitch, *sv = sk + kTileN * S::kPitch, *sp = sv + kTileN * DM;
+  const int g = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads, D = a.dim;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  PromptItem it;
+  // a part of a sequence: the tokens whose query rows (token, head of the group) fill a tile, or one token of a larger group
+  const int tokens = max(kTileM / G, 1), splits = (tokens * G + kTileM - 1) / kTileM;
+  const int idx = blockIdx.x / a.kv_heads;
+  if (!find_item<256>(a, tokens, idx / splits, it)) return;
+  const int f0 = (idx % splits) * kTileM;             // first flattened row inside the part
+  const int tok0 = it.part * tokens;
+  const int fn = min(min(tokens, it.n - tok0) * G - f0, kTileM);
+  if (fn <= 0) return;
+
+  auto q_at = [&](int r) { return f0 + min(r, fn - 1); };
+  for (int i = threadIdx.x; i < kTileM * (DM / 4); i += 256) {
+    const int r = i / (DM / 4), d = (i % (DM / 4)) * 4, f = q_at(r), t = f / G;
+    const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldq + static_cast<size_t>(g * G + f - t * G) * a.hdq;
+    *reinterpret_cast<float4*>(sq + r * S::kPitch + d) = four_of<ST>(q, d, D, (reinterpret_cast<uintptr_t>(q) & (4 * sizeof(ST) - 1)) == 0);
+  }
+  int hi[4], lo[4];
+  float m[4], l[4];
+  float4 o[4][DM / 64];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int pos = tok0 + q_at(4 * ty + r) / G;
+    hi[r] = pos + 1;
+    lo[r] = a.window > 0 ? pos - a.window + 1 : 0;
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DM / 64; ++i) o[r][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  const int p_lo = tok0 + f0 / G, p_hi = tok0 + (f0 + fn - 1) / G;
+  const int k_beg = a.window > 0 ? max(0, p_lo - a.window + 1) : 0, k_end = p_hi + 1;
+  const float c = a.scale * 1.4426950408889634f;
+  for (int k0 = k_beg; k0 < k_end; k0 += kTileN) {
+    __syncthreads();      // the tile before has been used
+    bool odd = false;     // a value that is not finite
+    for (int i = threadIdx.x; i < kTileN * (DM / 4); i += 256) {
+      const int r = i / (DM / 4), d = (i % (DM / 4)) * 4;
+      float4 kv = make_float4(0, 0, 0, 0), vv = kv;
+      if (k0 + r < k_end) {
+        const size_t row = static_cast<size_t>(it.row0) + k0 + r;
+        const ST* k = static_cast<const ST*>(a.k) + row * a.ldk + static_cast<size_t>(g) * a.hdk;
+        const ST* v = static_cast<const ST*>(a.v) + row * a.ldv + static_cast<size_t>(g) * a.hdv;
+        kv = four_of<ST>(k, d, D, (reinterpret_cast<uintptr_t>(k) & (4 * sizeof(ST) - 1)) == 0);
+        vv = four_of<ST>(v, d, D, (reinterpret_cast<uintptr_t>(v) & (4 * sizeof(ST) - 1)) == 0);
+      }
+      *reinterpret_cast<float4*>(sk + r * S::kPitch + d) = kv;
+      *reinterpret_cast<float4*>(sv + r * DM + d) = vv;
+      odd |= !(fmaxf(fmaxf(fabsf(vv.x), fabsf(vv.y)), fmaxf(fabsf(vv.z), fabsf(vv.w))) < INFINITY) || vv.x != vv.x || vv.y != vv.y ||
+             vv.z != vv.z || vv.w != vv.w;
+    }
+    odd = __syncthreads_or(odd);
+    float2 s2[4][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s2[r][i] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int d = 0; d < DM; d += 4) {
+      float4 qv[4], kv[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) qv[r] = *reinterpret_cast<const float4*>(sq + (4 * ty + r) * S::kPitch + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(sk + (tx + 16 * i) * S::kPitch + d);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s2[r][i] = fma_pair(make_float2(qv[r].x, qv[r].y), make_float2(kv[i].x, kv[i].y), s2[r][i]);
+          s2[r][i] = fma_pair(make_float2(qv[r].z, qv[r].w), make_float2(kv[i].z, kv[i].w), s2[r][i]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float s[4], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = k0 + tx + 16 * i;
+        s[i] = key < hi[r] && key >= lo[r] ? (s2[r][i].x + s2[r][i].y) * c : -INFINITY;
+        top = fmaxf(top, s[i]);
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float nm = fmaxf(m[r], top), ref = nm == -INFINITY ? 0.0f : nm, f = exp2f(m[r] - ref);
+      m[r] = nm;
+      l[r] *= f;
+#pragma unroll
+      for (int i = 0; i < DM / 64; ++i) {
+        o[r][i].x *= f; o[r][i].y *= f; o[r][i].z *= f; o[r][i].w *= f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = exp2f(s[i] - ref);
+        l[r] += p;
+        sp[(4 * ty + r) * S::kPPitch + tx + 16 * i] = p;
+      }
+    }
+    __syncthreads();
+    for (int k = 0; k < kTileN; k += 4) {
+      float pv[4][4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(pv[r]) = *reinterpret_cast<const float4*>(sp + (4 * ty + r) * S::kPPitch + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < DM / 64; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + (k + e) * DM + 64 * i + 4 * tx);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float4 u = v;
+            if (odd && pv[r][e] == 0.0f) u = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a masked value does not enter
+            const float2 pp = make_float2(pv[r][e], pv[r][e]);
+            const float2 x = fma_pair(pp, make_float2(u.x, u.y), make_float2(o[r][i].x, o[r][i].y));
+            const float2 y = fma_pair(pp, make_float2(u.z, u.w), make_float2(o[r][i].z, o[r][i].w));
+            o[r][i] = make_float4(x.x, x.y, y.x, y.y);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+    if (4 * ty + r >= fn) continue;
+    const int f = f0 + 4 * ty + r, t = f / G;
+    ST* out = static_cast<ST*>(a.out) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldo + static_cast<size_t>(g * G + f - t * G) * a.hdo;
+#pragma unroll
+    for (int i = 0; i < DM / 64; ++i) {
+      const int d = 64 * i + 4 * tx;
+      if (d >= D) continue;
+      store_scalar(out + d, o[r][i].x / l[r]);
+      store_scalar(out + d + 1, o[r][i].y / l[r]);
+      store_scalar(out + d + 2, o[r][i].z / l[r]);
+      store_scalar(out + d + 3, o[r][i].w / l[r]);
+    }
+  }
+}
+
+template <class ST, int DM>
+static cudaError_t launch_tile(const AttnArgs& a, cudaStream_t st) {
+  const int smem = TileShape<DM>::kFloats * 4, G = a.heads / a.kv_heads;
+  static SmemAttrOnce once;
+  const cudaError_t e = set_max_smem_once(once, prompt_tile_kernel<ST, DM>, smem);
+  if (e != cudaSuccess) return e;
+  const long long tokens = std::max(kTileM / G, 1), splits = (tokens * G + kTileM - 1) / kTileM;
+  const long long parts = std::min<long long>(a.rows, a.rows / tokens + a.seqs);
+  const long long ctas = parts * splits * a.kv_heads;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  return launch_chained(prompt_tile_kernel<ST, DM>, dim3(static_cast<unsigned>(ctas)), dim3(256), smem, st, a);
+}
+template <class ST>
+static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
+  if (a.dim <= 64) return launch_tile<ST, 64>(a, st);
+  return a.dim <= 128 ? launch_tile<ST, 128>(a, st) : launch_tile<ST, 256>(a, st);
+}
+
+// ---- tcgen05 tiles ----------------------------------------------------------------------------------------------------------
+constexpr int kPtThreads = 384, kPtWarpTma = 8, kPtWarpMma = 9, kPtKeys = 128, kPtStages = 2;
+constexpr uint32_t kPtHalf = 128 * 128;     // 128 rows of 64 channels, 128-byte swizzle
+
+template <int DM>
+struct PtLayout {
+  static constexpr uint32_t kOperand = (DM / 64) * kPtHalf;     // 128 rows x DM channels
+  static constexpr uint32_t q = 0, k = q + 2 * kOperand, v = k + kPtStages * kOperand, bar = v + kPtStages * kOperand;
+  static constexpr uint32_t total = bar + 256 + 1024;           // + slack for the 1024-byte alignment of the base
+};
+// TMEM columns: scores of the two tiles (the weights take the first half of the same columns), then their sums
+constexpr uint32_t kPtS = 0, kPtO = 256;
+
+struct alignas(64) PromptParams {
+  CUtensorMap q, k, v;
+  AttnArgs a;
+  int G, tokens;     // heads of a group; tokens of a tile (tokens * G <= 128 rows)
+  float c;           // scale * log2(e), not negative
+  int* status;
+};
+
+__device__ __forceinline__ void pt_load(uint32_t dst, const CUtensorMap* map, int d, int h, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(d), "r"(h), "r"(row), "r"(bar)
+      : "memory");
+}
+// rows of 128 bytes, 128-byte swizzle, eight rows per 1024-byte atom: K-major operand (channels inner, reduced) ...
+__device__ __forceinline__ uint64_t pt_desc_k(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// ... and MN-major (channels inner, keys reduced): the next 64 channels one half further, the next eight keys one atom further
+__device__ __forceinline__ uint64_t pt_desc_mn(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t(kPtHalf >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// D = F32, A = B = bf16, M = 128
+__device__ __forceinline__ constexpr uint32_t pt_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void pt_ld32(uint32_t t, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(t));
+}
+__device__ __forceinline__ void pt_st32(uint32_t t, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool pt_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ float pt_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pt_bf2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int DM>
+__global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptParams p) {
+  using L = PtLayout<DM>;
+  extern __shared__ __align__(1024) uint8_t pt_raw[];
+  const uint32_t base = (smem_u32(pt_raw) + 1023u) & ~1023u;
+  uint8_t* smem = pt_raw + (base - smem_u32(pt_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AttnArgs& a = p.a;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = blockIdx.x % a.kv_heads;
+  PromptItem it;
+  if (!find_item<kPtThreads>(a, 2 * p.tokens, blockIdx.x / a.kv_heads, it)) return;
+  // tokens [t0, t0 + tokens) and [t0 + tokens, ...) of the sequence; keys from `beg` on, 128 at a time
+  const int t0 = it.part * 2 * p.tokens;
+  const int beg = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
+  const int end0 = min(it.n, t0 + p.tokens), end1 = min(it.n, t0 + 2 * p.tokens);
+  const int n0 = (end0 - beg + kPtKeys - 1) / kPtKeys, n1 = end1 > end0 ? (end1 - beg + kPtKeys - 1) / kPtKeys : 0;
+  const int steps = max(n0, n1);
+
+  const uint32_t bars = base + L::bar;
+  auto q_full  = [&](int x) { return bars + 8u * x; };
+  auto k_full  = [&](int s) { return bars + 16u + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 32u + 8u * s; };
+  auto v_full  = [&](int s) { return bars + 48u + 8u * s; };
+  auto v_empty = [&](int s) { return bars + 64u + 8u * s; };
+  auto s_full  = [&](int x) { return bars + 80u + 8u * x; };
+  auto p_full  = [&](int x) { return bars + 96u + 8u * x; };
+  auto o_full  = [&](int x) { return bars + 112u + 8u * x; };
+  const uint32_t mma_end = bars + 128u;
+  uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 144);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 148);
+  RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 152);   // what the TMA warp armed last
+
+  if (warp == kPtWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full(i), 1);
+      mbar_init(k_full(i), 1);
+      mbar_init(k_empty(i), 1);
+      mbar_init(v_full(i), 1);
+      mbar_init(v_empty(i), 1);
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), 4);
+      mbar_init(o_full(i), 1);
+    }
+    mbar_init(mma_end, 1);
+    *abort_flag = 0;
+    *ring_end = RingArmed();
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  constexpr uint32_t tmem = 0;     // all 512 columns are ours: the allocation starts at column 0
+  if (*tmem_slot != tmem) *abort_flag = 1;   // (cannot happen; every wait below then gives up)
+
+  // Bounded wait of a whole warp; the vote makes the verdict uniform.
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    for (uint32_t i = 0; i < (1u << 21); ++i) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      if ((i & 31u) == 31u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    }
+    *abort_flag = 1;
+    return false;
+  };
+  bool ok = true;
+
+  // Registers go where the scores are: 2 x 128 threads of 224 and 128 of 40 are 62464 of the 64512 that the launch holds.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ------------------------------------------------------------------ scores -> weights (a thread owns a row)
+    const int x = warp >> 2, row = (warp & 3) * 32 + lane, n = x ? n1 : n0;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + kPtS + x * 128, to = tmem + lanes + kPtO + x * 128;
+    if (n > 0) {
+      const int t = row / p.G, h = row - t * p.G, first = t0 + x * p.tokens;
+      const int last = (x ? end1 : end0) - 1;
+      const bool live = t < p.tokens && first + t <= last;
+      const int pos = min(first + t, last);
+      const int hi = pos + 1, lo = a.window > 0 ? pos - a.window + 1 : 0;
+      const int in_hi = first + 1, in_lo = a.window > 0 ? last - a.window + 1 : 0;   // seen by every row
+      const float c = p.c;
+      float m = -INFINITY;
+      float2 l2 = make_float2(0.0f, 0.0f);
+      for (int j = 0; j < n && ok; ++j) {
+        if (!(ok = wait(s_full(x), j & 1))) break;
+        tc_after();
+        float s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pt_ld32(ts + 32 * i, s[i]);
+        tc_wait_ld();
+        const int k0 = beg + j * kPtKeys;
+        if (k0 + kPtKeys > in_hi || k0 < in_lo) {
+          const int rh = hi - k0, rl = lo - k0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * i + e >= rh || 32 * i + e < rl) s[i][e] = -INFINITY;
+        }
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          top[i] = s[i][0];
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) top[i] = fmaxf(fmaxf(top[i], s[i][e]), s[i][e + 1]);
+          top[i] = fmaxf(top[i], s[i][31]);
+        }
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool moves = m == -INFINITY ? mx != -INFINITY : (mx - m) * c > 8.0f;
+        if (__any_sync(0xffffffffu, moves)) {
+          const float f = moves ? (m == -INFINITY ? 0.0f : pt_ex2((m - mx) * c)) : 1.0f;
+          if (moves) m = mx;
+          l2.x *= f;
+          l2.y *= f;
+          if (j > 0) {      // (the product of step j - 1 came before the scores of this one)
+#pragma unroll
+            for (int i = 0; i < DM / 32; ++i) {
+              float o[32];
+              pt_ld32(to + 32 * i, o);
+              tc_wait_ld();
+              uint32_t u[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
+              pt_st32(to + 32 * i, u);
+            }
+          }
+        }
+        const float nm = m == -INFINITY ? 0.0f : -m * c;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 y = ffma2(make_float2(s[2 * i + (e >> 4)][2 * (e & 15)], s[2 * i + (e >> 4)][2 * (e & 15) + 1]), make_float2(c, c), make_float2(nm, nm));
+            const float2 pr = make_float2(pt_ex2(y.x), pt_ex2(y.y));
+            l2 = fadd2(l2, pr);
+            w[e] = pt_bf2(pr.x, pr.y);
+          }
+          pt_st32(ts + 32 * i, w);
+        }
+        pt_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(x));
+      }
+      if (ok) ok = wait(o_full(x), 0);
+      if (ok) {
+        tc_after();
+        const float l = l2.x + l2.y, inv = 1.0f / l;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(it.row0 + pos) * a.ldo + static_cast<size_t>(g * p.G + h) * a.hdo;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < DM / 32; ++i) {
+          float o[32];
+          pt_ld32(to + 32 * i, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float y0 = o[e + 2 * k] * inv, y1 = o[e + 2 * k + 1] * inv;
+              bad |= !(fabsf(y0) < INFINITY) || !(fabsf(y1) < INFINITY);
+              w[k] = pt_bf2(y0, y1);
+            }
+            if (live && 32 * i + e < a.dim) *reinterpret_cast<uint4*>(out + 32 * i + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        // rows that did not come out finite, one after the other
+        for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo != 0; todo &= todo - 1) {
+          const int src = __ffs(todo) - 1;
+          __syncwarp();
+          row_alone<__nv_bfloat16>(a, it.row0, __shfl_sync(0xffffffffu, pos, src), g * p.G + __shfl_sync(0xffffffffu, h, src));
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  }
+  if (warp == kPtWarpTma) {
+    // ------------------------------------------------------------------ queries, then keys and values
+    if (lane == 0) {
+      RingArmed armed;
+      auto wait1 = [&](uint32_t bar, uint32_t parity) -> bool {
+        for (uint32_t i = 0; i < (1u << 21); ++i) {
+          if (mbar_try_wait(bar, parity)) return true;
+          if ((i & 31u) == 31u && *abort_flag != 0) return false;
+        }
+        *abort_flag = 1;
+        return false;
+      };
+      auto load = [&](uint32_t dst, const CUtensorMap* map, int head, int row, uint32_t bytes, uint32_t bar) {
+        mbar_expect_tx(bar, bytes * (DM / 64));
+        for (int d = 0; d < DM; d += 64) pt_load(dst + (d / 64) * kPtHalf, map, d, head, row, bar);
+      };
+      const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128u;
+      load(base + L::q, &p.q, g * p.G, it.row0 + t0, q_bytes, q_full(0));
+      armed.arm(4, 0);
+      for (int j = 0; j < steps && ok; ++j) {
+        const int s = j & 1;
+        const uint32_t ph = (j >> 1) & 1;
+        if (!(ok = wait1(k_empty(s), ph ^ 1u))) break;
+        load(base + L::k + s * L::kOperand, &p.k, g, it.row0 + beg + j * kPtKeys, kPtHalf, k_full(s));
+        armed.arm(s, ph);
+        if (j == 0 && n1 > 0) {
+          load(base + L::q + L::kOperand, &p.q, g * p.G, it.row0 + t0 + p.tokens, q_bytes, q_full(1));
+          armed.arm(5, 0);
+        }
+        if (!(ok = wait1(v_empty(s), ph ^ 1u))) break;
+        load(base + L::v + s * L::kOperand, &p.v, g, it.row0 + beg + j * kPtKeys, kPtHalf, v_full(s));
+        armed.arm(2 + s, ph);
+      }
+      *ring_end = armed;
+    }
+    __syncwarp();
+  } else if (warp == kPtWarpMma) {
+    // ------------------------------------------------------------------ products
+    auto scores = [&](int x, int j) {
+      if (pt_elect()) {
+        const uint32_t qa = base + L::q + x * L::kOperand, ka = base + L::k + (j & 1) * L::kOperand;
+#pragma unroll
+        for (int k = 0; k < DM / 16; ++k)
+          pt_mma_ss(tmem + kPtS + x * 128, pt_desc_k(qa + (k >> 2) * kPtHalf + (k & 3) * 32), pt_desc_k(ka + (k >> 2) * kPtHalf + (k & 3) * 32),
+                    pt_idesc(kPtKeys, false), k != 0);
+        tc_commit(s_full(x));
+      }
+      __syncwarp();
+    };
+    auto sums = [&](int x, int j, bool last) {
+      if (pt_elect()) {
+        const uint32_t va = base + L::v + (j & 1) * L::kOperand;
+#pragma unroll
+        for (int k = 0; k < kPtKeys / 16; ++k)
+          pt_mma_ts(tmem + kPtO + x * 128, tmem + kPtS + x * 128 + 8 * k, pt_desc_mn(va + k * 2048), pt_idesc(DM, true), j != 0 || k != 0);
+        if (last) tc_commit(o_full(x));
+      }
+      __syncwarp();
+    };
+    auto done = [&](uint32_t bar) {
+      if (pt_elect()) tc_commit(bar);
+      __syncwarp();
+    };
+    ok = wait(k_full(0), 0) && wait(q_full(0), 0);
+    if (ok) {
+      tc_after();
+      scores(0, 0);
+      if (n1 > 0) {
+        ok = wait(q_full(1), 0);
+        if (ok) scores(1, 0);
+      }
+      done(k_empty(0));
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      const uint32_t ph = (j >> 1) & 1;
+      if (!(ok = wait(v_full(j & 1), ph))) break;
+      bool keys = false;       // the next step's keys are there
+      for (int x = 0; x < 2 && ok; ++x) {
+        const int n = x ? n1 : n0;
+        if (j >= n) continue;
+        if (!(ok = wait(p_full(x), j & 1))) break;
+        tc_after();
+        sums(x, j, j + 1 == n);
+        if (j + 1 < n) {
+          if (!keys && !(ok = wait(k_full((j + 1) & 1), ((j + 1) >> 1) & 1))) break;
+          keys = true;
+          scores(x, j + 1);
+        }
+      }
+      if (!ok) break;
+      done(v_empty(j & 1));
+      if (keys) done(k_empty((j + 1) & 1));
+    }
+  }
+  if (!ok && lane == 0) atomicExch(p.status, KDNN_ERR_DEVICE_WAIT);
+  tc_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // some role gave up: the copies and products still in flight end (bounded) before the CTA gives its memory back
+    if (warp == kPtWarpTma && lane == 0)
+      ring_drain(*ring_end, 6, 1u << 14, [&](int s, uint32_t parity) {
+        return mbar_try_wait(s < 2 ? k_full(s) : s < 4 ? v_full(s - 2) : q_full(s - 4), parity); });
+    if (warp == kPtWarpMma && pt_elect()) {
+      tc_commit(mma_end);
+      mbar_wait_bounded(mma_end, 0u, 1u << 16);
+    }
+    __syncthreads();
+  }
+  if (warp == kPtWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
+}
+
+static bool encode_heads(CUtensorMap* map, const void* x, size_t ld, size_t hd, int rows, int heads, int dim, int box_heads, int box_rows) {
+  TcEncodeFn fn = tc_encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3]    = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(hd) * 2, static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[3]     = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[3]    = {1u, 1u, 1u};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DM>
+static cudaError_t launch_tc(const PromptParams& p, cudaStream_t st) {
+  static SmemAttrOnce once;
+  const cudaError_t e = set_max_smem_once(once, prompt_tc_kernel<DM>, static_cast<int>(PtLayout<DM>::total));
+  if (e != cudaSuccess) return e;
+  const long long parts = std::min<long long>(p.a.rows, p.a.rows / (2 * p.tokens) + p.a.seqs), ctas = parts * p.a.kv_heads;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  return launch_chained(prompt_tc_kernel<DM>, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads), PtLayout<DM>::total, st, p);
+}
+
+cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
+  if (a.scalar == KDNN_F32) return launch_tiles<float>(a, st);
+  const int G = a.heads / a.kv_heads;
+  const size_t pitches = a.ldq | a.hdq | a.ldk | a.hdk | a.ldv | a.hdv | a.ldo | a.hdo;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                          reinterpret_cast<uintptr_t>(a.out);
+  // TMA wants 16-byte pitches; a reference for the largest score needs a scale that is not negative
+  if (a.dim <= 128 && G <= 128 && pitches % 8 == 0 && bases % 16 == 0 && a.scale >= 0.0f && a.scale < 1e30f) {
+    PromptParams p;
+    p.a = a;
+    p.G = G;
+    p.tokens = 128 / G;
+    p.c = a.scale * 1.4426950408889634f;
+    const cudaError_t e = moe_status_ptr(&p.status);
+    if (e != cudaSuccess) return e;
+    if (encode_heads(&p.q, a.q, a.ldq, a.hdq, a.rows, a.heads, a.dim, G, p.tokens) &&
+        encode_heads(&p.k, a.k, a.ldk, a.hdk, a.rows, a.kv_heads, a.dim, 1, kPtKeys) &&
+        encode_heads(&p.v, a.v, a.ldv, a.hdv, a.rows, a.kv_heads, a.dim, 1, kPtKeys))
+      return a.dim <= 64 ? launch_tc<64>(p, st) : launch_tc<128>(p, st);
+  }
+  return launch_tiles<__nv_bfloat16>(a, st);
+}
+
+}  // namespace kdnn
