@@ -209,7 +209,13 @@ def _scalar(t: torch.Tensor) -> int:
     raise ValueError(f"Scalar must be float32 or bfloat16, got {t.dtype}")
 
 
+# the current stream's handle without a Stream object around it (a microsecond less per call), where torch has the call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -767,41 +773,66 @@ def moe_block_routing(workspace: torch.Tensor, tokens_local: int, world: int, to
 
 # ---------------------------------------------------------------------------
 # attention: paged 8-bit cache and packed prompts (src/KokkosDNN_Attention.hpp, src/KokkosDNN_KVCache.hpp)
+_I32 = torch.int32
+
+
 def _here(what: str, *tensors: torch.Tensor) -> None:
     """Every tensor on the current CUDA device, where the launch goes."""
-    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    dev = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda or t.device.index != dev:
+        if t.get_device() != dev or dev < 0:
             raise ValueError(f"{what}: tensors must live on the current CUDA device")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors must live on the current CUDA device")
 
 
-def _ints(what: str, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous int32")
-
-
-def _packed(what: str, name: str, t: torch.Tensor, heads: Optional[int], dim: Optional[int]):
+def _packed(what: str, name: str, t: torch.Tensor, rows: int, heads: int, dim: int):
     """(row pitch, head pitch) of a [rows, heads, dim] tensor whose heads are contiguous rows."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{what}: {name} must be [rows, heads, dim]")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    if t.shape != (rows, heads, dim):
+        raise ValueError(f"{what}: {name} must be [rows, heads, dim] = {(rows, heads, dim)}, got {tuple(t.shape)}")
+    ld, hd, one = t.stride()
+    if one != 1 and dim > 1:
         raise ValueError(f"{what}: {name} must have unit stride in its last dimension")
-    hd = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    return (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] - 1) * hd + t.shape[2])), hd
+    if heads == 1:
+        hd = dim
+    return (ld if rows > 1 else max(ld, (heads - 1) * hd + dim)), hd
 
 
 @dataclass
 class KvPlan:
     """What kv_plan writes for one step: where its rows start, which positions and places of the cache they take.
-    ``lens`` and ``state`` are the sequences' lengths and the pool's state after the step."""
-    row_start: torch.Tensor   # int32 [seqs + 1]
-    first: torch.Tensor       # int32 [seqs]
-    lens: torch.Tensor        # int32 [seqs]
-    state: torch.Tensor       # int32 [4]: first free ring entry, free pages, rows without a slot, page writes
-    slots: torch.Tensor       # int32 [rows]
-    writes: torch.Tensor      # int32 [kv_writes(rows, seqs, page), 4]
+    ``lens`` and ``state`` are the sequences' lengths and the pool's state after the step. Tensors are checked where they are
+    set: contiguous int32 of the shapes below, on one device."""
+    row_start: torch.Tensor   # [seqs + 1]
+    first: torch.Tensor       # [seqs]
+    lens: torch.Tensor        # [seqs]
+    state: torch.Tensor       # [4]: first free ring entry, free pages, rows without a slot, page writes
+    slots: torch.Tensor       # [rows]
+    writes: torch.Tensor      # [at least kv_writes(rows, seqs, page), 4]
     page: int
+
+    def __post_init__(self):
+        self._check()
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if hasattr(self, "seqs"):      # complete: a tensor put in later is checked as the first ones were
+            self._check()
+
+    def _check(self):
+        tensors = (self.row_start, self.first, self.lens, self.state, self.slots, self.writes)
+        dev = self.first.device
+        for t in tensors:
+            if t.dtype != _I32 or not t.is_contiguous() or t.device != dev:
+                raise ValueError("KvPlan: tensors must be contiguous int32 on one device")
+        if self.slots.dim() != 1 or self.first.dim() != 1:
+            raise ValueError("KvPlan: first is [seqs] and slots [rows]")
+        seqs, rows = self.first.shape[0], self.slots.shape[0]
+        if self.row_start.shape != (seqs + 1,) or self.lens.shape != (seqs,) or self.state.shape != (4,) or \
+                self.writes.dim() != 2 or self.writes.shape[1] != 4 or self.writes.shape[0] < kv_writes(rows, seqs, self.page):
+            raise ValueError("KvPlan: dimension mismatch")
+        for name, value in (("seqs", seqs), ("rows", rows)):
+            object.__setattr__(self, name, value)
 
     @staticmethod
     def empty(seqs: int, rows: int, page: int, device="cuda") -> "KvPlan":
@@ -809,16 +840,8 @@ class KvPlan:
             return torch.zeros(shape, dtype=torch.int32, device=device)
         return KvPlan(ints(seqs + 1), ints(seqs), ints(seqs), ints(4), ints(rows), ints(kv_writes(rows, seqs, page), 4), page)
 
-    @property
-    def seqs(self) -> int:
-        return self.first.shape[0]
 
-    @property
-    def rows(self) -> int:
-        return self.slots.shape[0]
-
-
-@dataclass
+@dataclass(frozen=True)
 class KvCache:
     """One layer's paged cache: int8 codes [pages, kv_heads, page, dim] and a power-of-two scale per page and head."""
     k: torch.Tensor
@@ -827,22 +850,34 @@ class KvCache:
     v_scale: torch.Tensor
 
     def __post_init__(self):
-        if self.k.dim() != 4 or self.k.shape != self.v.shape or self.k.dtype != torch.int8 or self.v.dtype != torch.int8:
+        k = self.k
+        if k.dim() != 4 or k.shape != self.v.shape or k.dtype != torch.int8 or self.v.dtype != torch.int8:
             raise ValueError("KvCache: codes must be int8 [pages, kv_heads, page, dim]")
-        if tuple(self.k_scale.shape) != tuple(self.k.shape[:2]) or self.v_scale.shape != self.k_scale.shape or \
+        if self.k_scale.shape != k.shape[:2] or self.v_scale.shape != k.shape[:2] or \
                 self.k_scale.dtype != torch.float32 or self.v_scale.dtype != torch.float32:
             raise ValueError("KvCache: scales must be float32 [pages, kv_heads]")
-        if not all(t.is_contiguous() for t in (self.k, self.v, self.k_scale, self.v_scale)):
-            raise ValueError("KvCache: tensors must be contiguous")
-        self.pages, self.kv_heads, self.page, self.dim = self.k.shape
-        self.c = KvCacheC(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.pages,
-                          self.kv_heads, self.page, self.dim)
+        for t in (k, self.v, self.k_scale, self.v_scale):
+            if not t.is_contiguous() or t.device != k.device:
+                raise ValueError("KvCache: tensors must be contiguous, on one device")
+        for name, value in zip(("pages", "kv_heads", "page", "dim"), k.shape):
+            object.__setattr__(self, name, value)
+
+    def c_struct(self) -> KvCacheC:
+        return KvCacheC(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.pages,
+                        self.kv_heads, self.page, self.dim)
 
     @staticmethod
     def empty(pages: int, kv_heads: int, page: int, dim: int, device="cuda") -> "KvCache":
         codes = [torch.zeros((pages, kv_heads, page, dim), dtype=torch.int8, device=device) for _ in range(2)]
         scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
         return KvCache(*codes, *scales)
+
+
+def _table(what: str, table: torch.Tensor, seqs: int) -> int:
+    """Row pitch of a block table [seqs, columns]."""
+    if table.dim() != 2 or table.shape[0] != seqs or table.dtype != _I32 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise ValueError(f"{what}: table must be int32 [seqs, columns] with unit stride in its last dimension")
+    return table.stride(0) if seqs > 1 else table.shape[1]
 
 
 def kv_writes(rows: int, seqs: int, page: int) -> int:
@@ -855,35 +890,33 @@ def kv_plan(fresh: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, ring: 
     sequence (negative: it has ended and gives its pages back), ``lens`` tokens cached, ``table`` [seqs, columns] the page
     numbers, ``ring`` the pool's free pages and ``state`` its position. ``lens`` may be ``plan.lens`` and ``state``
     ``plan.state``: then the call moves the pool from step to step in place."""
-    seqs, rows = plan.first.shape[0], plan.slots.shape[0]
-    if tuple(fresh.shape) != (seqs,) or tuple(lens.shape) != (seqs,) or table.dim() != 2 or table.shape[0] != seqs or \
-            tuple(plan.lens.shape) != (seqs,) or tuple(plan.row_start.shape) != (seqs + 1,) or state.numel() != 4 or \
-            plan.state.numel() != 4 or ring.dim() != 1 or plan.writes.dim() != 2 or plan.writes.shape[1] != 4:
+    seqs, one = plan.seqs, (plan.seqs,)
+    if fresh.shape != one or lens.shape != one or state.shape != (4,) or ring.dim() != 1:
         raise ValueError("kv_plan: dimension mismatch")
-    _ints("kv_plan", fresh=fresh, lens=lens, ring=ring, state=state, row_start=plan.row_start, first=plan.first,
-          plan_lens=plan.lens, plan_state=plan.state, slots=plan.slots, writes=plan.writes)
-    if table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError("kv_plan: table must be int32 with unit stride in its last dimension")
-    _here("kv_plan", fresh, lens, table, ring, state, plan.row_start, plan.slots, plan.writes)
-    rc = lib.kdnn_b200_kv_plan(fresh.data_ptr(), lens.data_ptr(), seqs, plan.page, rows, table.data_ptr(),
-                               table.stride(0) if seqs > 1 else table.shape[1], table.shape[1], ring.data_ptr(), ring.shape[0],
-                               state.data_ptr(), plan.row_start.data_ptr(), plan.first.data_ptr(), plan.lens.data_ptr(),
-                               plan.state.data_ptr(), plan.slots.data_ptr(), plan.writes.data_ptr(), plan.writes.shape[0], _stream())
+    for t in (fresh, lens, ring, state):
+        if t.dtype != _I32 or not t.is_contiguous():
+            raise ValueError("kv_plan: fresh, lens, ring and state must be contiguous int32")
+    ldt = _table("kv_plan", table, seqs)
+    _here("kv_plan", fresh, lens, table, ring, state, plan.first)
+    rc = lib.kdnn_b200_kv_plan(fresh.data_ptr(), lens.data_ptr(), seqs, plan.page, plan.rows, table.data_ptr(), ldt, table.shape[1],
+                               ring.data_ptr(), ring.shape[0], state.data_ptr(), plan.row_start.data_ptr(), plan.first.data_ptr(),
+                               plan.lens.data_ptr(), plan.state.data_ptr(), plan.slots.data_ptr(), plan.writes.data_ptr(),
+                               plan.writes.shape[0], _stream())
     _check(rc, "kv_plan")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, plan: KvPlan, cache: KvCache) -> None:
     """The step's keys and values [rows, kv_heads, dim] into the places that ``plan`` gives them (see kdnn_b200_kv_append)."""
-    ldk, hdk = _packed("kv_append", "k", k, cache.kv_heads, cache.dim)
-    ldv, hdv = _packed("kv_append", "v", v, cache.kv_heads, cache.dim)
-    if k.shape[0] != plan.rows or v.shape[0] != plan.rows or k.dtype != v.dtype:
-        raise ValueError("kv_append: k and v must have the plan's rows and one Scalar")
+    rows, heads, dim = plan.rows, cache.kv_heads, cache.dim
+    ldk, hdk = _packed("kv_append", "k", k, rows, heads, dim)
+    ldv, hdv = _packed("kv_append", "v", v, rows, heads, dim)
+    if k.dtype != v.dtype:
+        raise ValueError("kv_append: k and v must share one Scalar")
     if cache.page != plan.page:
         raise ValueError("kv_append: cache and plan have pages of different size")
-    _ints("kv_append", writes=plan.writes)
-    _here("kv_append", k, v, plan.writes, cache.k, cache.v, cache.k_scale, cache.v_scale)
-    _check(lib.kdnn_b200_kv_append(k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(k), k.shape[0], plan.writes.data_ptr(),
-                                   plan.writes.shape[0], C.byref(cache.c), _stream()), "kv_append")
+    _here("kv_append", k, v, plan.first, cache.k)
+    _check(lib.kdnn_b200_kv_append(k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(k), rows, plan.writes.data_ptr(),
+                                   plan.writes.shape[0], C.byref(cache.c_struct()), _stream()), "kv_append")
 
 
 def kv_attention_workspace_bytes(rows: int, seqs: int, heads: int, kv_heads: int, dim: int) -> int:
@@ -894,23 +927,21 @@ def kv_attention(q: torch.Tensor, plan: KvPlan, table: torch.Tensor, cache: KvCa
                  scale: Optional[float] = None, window: int = 0) -> None:
     """Causal grouped attention of the step's rows over the cached tokens of their sequences, their own among them (see
     kdnn_b200_kv_attention); ``scale`` defaults to dim ** -0.5, ``window`` 0 looks back without limit."""
-    ldq, hdq = _packed("kv_attention", "q", q, None, cache.dim)
-    rows, heads = q.shape[0], q.shape[1]
-    ldo, hdo = _packed("kv_attention", "out", out, heads, cache.dim)
-    seqs = plan.first.shape[0]
-    if out.shape[0] != rows or rows != plan.rows or out.dtype != q.dtype:
-        raise ValueError("kv_attention: q and out must have the plan's rows and one Scalar")
-    if table.dim() != 2 or table.shape[0] != seqs or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError("kv_attention: table must be int32 [seqs, columns] with unit stride in its last dimension")
+    if q.dim() != 3:
+        raise ValueError("kv_attention: q must be [rows, heads, dim]")
+    rows, heads, dim, seqs = plan.rows, q.shape[1], cache.dim, plan.seqs
+    ldq, hdq = _packed("kv_attention", "q", q, rows, heads, dim)
+    ldo, hdo = _packed("kv_attention", "out", out, rows, heads, dim)
+    if out.dtype != q.dtype:
+        raise ValueError("kv_attention: q and out must share one Scalar")
+    ldt = _table("kv_attention", table, seqs)
     if cache.page != plan.page or window < 0:
         raise ValueError("kv_attention: cache and plan have pages of different size, or the window is negative")
-    _ints("kv_attention", row_start=plan.row_start, first=plan.first, lens=plan.lens)
-    _here("kv_attention", q, out, table, workspace, plan.row_start, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    _here("kv_attention", q, out, table, workspace, plan.first, cache.k)
     _check(lib.kdnn_b200_kv_attention(q.data_ptr(), ldq, hdq, _scalar(q), rows, heads, plan.row_start.data_ptr(), plan.first.data_ptr(),
-                                      plan.lens.data_ptr(), seqs, table.data_ptr(), table.stride(0) if seqs > 1 else table.shape[1],
-                                      table.shape[1], C.byref(cache.c), out.data_ptr(), ldo, hdo,
-                                      cache.dim ** -0.5 if scale is None else float(scale), window, workspace.data_ptr(),
-                                      workspace.numel() * workspace.element_size(), _stream()), "kv_attention")
+                                      plan.lens.data_ptr(), seqs, table.data_ptr(), ldt, table.shape[1], C.byref(cache.c_struct()),
+                                      out.data_ptr(), ldo, hdo, dim ** -0.5 if scale is None else float(scale), window,
+                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()), "kv_attention")
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_start: torch.Tensor, out: torch.Tensor,
@@ -918,18 +949,18 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_star
     """Causal grouped attention over packed prompts (see kdnn_b200_prompt_attention): q, out [rows, heads, dim], k, v
     [rows, kv_heads, dim], ``row_start`` int32 [seqs + 1]; ``scale`` defaults to dim ** -0.5."""
     what = "prompt_attention"
-    ldq, hdq = _packed(what, "q", q, None, None)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"{what}: q and k must be [rows, heads, dim]")
     rows, heads, dim = q.shape
-    ldk, hdk = _packed(what, "k", k, None, dim)
-    kv_heads = k.shape[1]
-    ldv, hdv = _packed(what, "v", v, kv_heads, dim)
-    ldo, hdo = _packed(what, "out", out, heads, dim)
-    if k.shape[0] != rows or v.shape[0] != rows or out.shape[0] != rows or k.dtype != q.dtype or v.dtype != q.dtype or \
-            out.dtype != q.dtype:
-        raise ValueError(f"{what}: q, k, v and out must have the same rows and one Scalar")
-    if row_start.dim() != 1 or row_start.shape[0] < 1 or window < 0:
-        raise ValueError(f"{what}: row_start must be [seqs + 1] and the window not negative")
-    _ints(what, row_start=row_start)
+    kv_heads, dtype = k.shape[1], q.dtype
+    ldq, hdq = _packed(what, "q", q, rows, heads, dim)
+    ldk, hdk = _packed(what, "k", k, rows, kv_heads, dim)
+    ldv, hdv = _packed(what, "v", v, rows, kv_heads, dim)
+    ldo, hdo = _packed(what, "out", out, rows, heads, dim)
+    if k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
+        raise ValueError(f"{what}: q, k, v and out must share one Scalar")
+    if row_start.dim() != 1 or row_start.shape[0] < 1 or row_start.dtype != _I32 or not row_start.is_contiguous() or window < 0:
+        raise ValueError(f"{what}: row_start must be contiguous int32 [seqs + 1] and the window not negative")
     _here(what, q, k, v, out, row_start)
     _check(lib.kdnn_b200_prompt_attention(q.data_ptr(), ldq, hdq, k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(q), rows,
                                           heads, kv_heads, dim, row_start.data_ptr(), row_start.shape[0] - 1, out.data_ptr(), ldo, hdo,

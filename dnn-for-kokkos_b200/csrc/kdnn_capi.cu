@@ -586,7 +586,7 @@ int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, si
                       size_t table_cols, int32_t* ring, size_t pages, const int32_t* state, int32_t* row_start, int32_t* first,
                       int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t writes_entries, void* stream) {
   if (!page_ok(page)) return fail(KDNN_ERR_INVALID, "kv_plan: pages hold 16, 32, 64 or 128 tokens");
-  if (seqs > 8192 || rows > static_cast<size_t>(INT_MAX) || pages == 0 || pages > static_cast<size_t>(INT_MAX) / page || table_cols == 0 ||
+  if (seqs > 8192 || rows > (size_t(1) << 30) || pages == 0 || pages > static_cast<size_t>(INT_MAX) / page || table_cols == 0 ||
       table_cols > static_cast<size_t>(INT_MAX) / page || ldt < table_cols)
     return fail(KDNN_ERR_INVALID, "kv_plan: dimension mismatch");
   if (seqs == 0) return fail(KDNN_ERR_INVALID, "kv_plan: no sequences");

@@ -17,7 +17,7 @@ namespace kdnn {
 // Everything is a prefix sum over the sequences followed by independent entries, so each CTA of a small cluster
 // forms the sums for itself in shared memory and writes its share of the entries; the cluster barrier lies between the
 // last read of lens / state and their new values, which may go to the same arrays.
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
 constexpr int kPlanCluster = 8;
 
 struct PlanArgs {
@@ -25,7 +25,7 @@ struct PlanArgs {
   int32_t *table, *ring, *row_start, *first, *lens_out, *state_out, *slots;
   int4* writes;
   size_t ldt;
-  int B, page, rows, cols, pages, most;
+  int B, shift, rows, cols, pages, most;   // pages of 1 << shift tokens
 };
 
 __device__ __forceinline__ void cluster_sync_all() {
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   pdl_chain_entry();
   extern __shared__ int sm[];
   __shared__ long long s_warps[kPlanThreads / 32];
-  const int B = a.B, page = a.page;
+  const int B = a.B, shift = a.shift, page = 1 << shift;
   int* rs   = sm;              // [B + 1] first row of a sequence
   int* tk   = rs + B + 1;      // [B + 1] pages taken before it
   int* gv   = tk + B + 1;      // [B + 1] pages given back before it
@@ -87,7 +87,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   int* len  = wr + B + 1;      // [B] tokens it holds (of an ended one: what it gives back)
   int* stor = len + B;         // [B] fresh tokens that get a slot; -1: ended
   const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(B, static_cast<int>(threadIdx.x) * per), b1 = min(B, b0 + per);
-  const int head = ((a.state[0] % a.pages) + a.pages) % a.pages, avail = max(0, min(a.pages, a.state[1]));
+  int head = a.state[0];
+  const int avail = max(0, min(a.pages, a.state[1]));
+  if (head < 0 || head >= a.pages) head = ((head % a.pages) + a.pages) % a.pages;
+  const int tail = head + avail >= a.pages ? head + avail - a.pages : head + avail;
 
   long long n = 0, total, all;
   for (int b = b0; b < b1; ++b) {
@@ -104,11 +107,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   if (threadIdx.x == 0) rs[B] = static_cast<int>(min(all, static_cast<long long>(a.rows)));
   __syncthreads();
 
-  auto held  = [&](int b) { return (len[b] + page - 1) / page; };
+  auto held  = [&](int b) { return (len[b] + page - 1) >> shift; };
   auto wants = [&](int b) {
     if (stor[b] < 0) return 0;
     const long long to = static_cast<long long>(len[b]) + (rs[b + 1] - rs[b]);
-    return static_cast<int>(min((to + page - 1) / page, static_cast<long long>(a.cols))) - held(b);
+    return static_cast<int>(min((to + page - 1) >> shift, static_cast<long long>(a.cols))) - held(b);
   };
   long long need = 0, back = 0;
   for (int b = b0; b < b1; ++b) {
@@ -132,7 +135,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     const int st = static_cast<int>(min(static_cast<long long>(rs[b + 1] - rs[b]), static_cast<long long>(h + got) * page - len[b]));
     stor[b] = st;
     kept += st;
-    put += st > 0 ? (len[b] + st - 1) / page - len[b] / page + 1 : 0;
+    put += st > 0 ? ((len[b] + st - 1) >> shift) - (len[b] >> shift) + 1 : 0;
   }
   long long stored;
   block_exclusive(kept, s_warps, stored);
@@ -140,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   const int touched = static_cast<int>(min(total, static_cast<long long>(a.most)));
   for (int b = b0; b < b1; ++b) {
     wr[b] = static_cast<int>(min(w0, static_cast<long long>(a.most)));
-    w0 += stor[b] > 0 ? (len[b] + stor[b] - 1) / page - len[b] / page + 1 : 0;
+    w0 += stor[b] > 0 ? ((len[b] + stor[b] - 1) >> shift) - (len[b] >> shift) + 1 : 0;
   }
   if (threadIdx.x == kPlanThreads - 1) {
     tk[B] = static_cast<int>(min(take, static_cast<long long>(avail)));
@@ -150,46 +153,58 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   __syncthreads();
   const int taken = tk[B];
 
+  auto ring_at = [&](int from, int i) { return from + i >= a.pages ? from + i - a.pages : from + i; };   // i <= pages
   // the j-th page of sequence b: what the table holds, or the ring's next ones
   auto page_of = [&](int b, int j) {
     const int h = held(b);
-    return j < h ? a.table[static_cast<size_t>(b) * a.ldt + j]
-                 : a.ring[static_cast<int>((static_cast<long long>(head) + tk[b] + j - h) % a.pages)];
+    return j < h ? a.table[static_cast<size_t>(b) * a.ldt + j] : a.ring[ring_at(head, tk[b] + j - h)];
   };
   const int step = static_cast<int>(cluster_size()) * kPlanThreads, me = static_cast<int>(cluster_rank()) * kPlanThreads + threadIdx.x;
-  for (int p = me; p < taken; p += step) {
-    const int b = upper_of(tk, B, p);
-    a.table[static_cast<size_t>(b) * a.ldt + held(b) + p - tk[b]] = a.ring[static_cast<int>((static_cast<long long>(head) + p) % a.pages)];
-  }
-  for (int p = me; p < given; p += step) {
-    const int b = upper_of(gv, B, p);
-    a.ring[static_cast<int>((static_cast<long long>(head) + avail + p) % a.pages)] = a.table[static_cast<size_t>(b) * a.ldt + p - gv[b]];
+  const int rows = rs[B];
+  // four rows per search; a page is looked up where it changes
+  const bool wide = (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0;
+  for (int r0 = me * 4; r0 < a.rows; r0 += step * 4) {
+    int out[4] = {-1, -1, -1, -1};
+    if (r0 < rows) {
+      int b = upper_of(rs, B, r0), at_b = -1, at_j = -1, pg = -1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = r0 + k;
+        if (r >= rows) break;
+        while (r >= rs[b + 1]) ++b;
+        const int i = r - rs[b];
+        if (i < stor[b]) {
+          const int pos = len[b] + i, j = pos >> shift;
+          if (b != at_b || j != at_j) {
+            pg = page_of(b, j);
+            at_b = b;
+            at_j = j;
+          }
+          if (pg >= 0 && pg < a.pages) out[k] = (pg << shift) + (pos & (page - 1));
+        }
+      }
+    }
+    if (wide && r0 + 4 <= a.rows) *reinterpret_cast<int4*>(a.slots + r0) = make_int4(out[0], out[1], out[2], out[3]);
+    else
+      for (int k = 0; k < 4 && r0 + k < a.rows; ++k) a.slots[r0 + k] = out[k];
   }
   for (int w = me; w < a.most; w += step) {
     int4 e = make_int4(0, 0, 0, 0);
     if (w < touched) {
-      const int b = upper_of(wr, B, w), j = len[b] / page + w - wr[b];
-      const int lo = max(j * page, len[b]);
-      const int hi = static_cast<int>(min((static_cast<long long>(j) + 1) * page, static_cast<long long>(len[b]) + stor[b]));
-      e = make_int4(rs[b] + lo - len[b], hi - lo, page_of(b, j), lo - j * page);
+      const int b = upper_of(wr, B, w), j = (len[b] >> shift) + w - wr[b];
+      const int lo = max(j << shift, len[b]);
+      const int hi = static_cast<int>(min((static_cast<long long>(j) + 1) << shift, static_cast<long long>(len[b]) + stor[b]));
+      e = make_int4(rs[b] + lo - len[b], hi - lo, page_of(b, j), lo - (j << shift));
     }
     a.writes[w] = e;
   }
-  const int rows = rs[B];
-  for (int r0 = me * 4; r0 < a.rows; r0 += step * 4) {   // four rows per search
-    int b = r0 < rows ? upper_of(rs, B, r0) : 0;
-    for (int r = r0; r < min(r0 + 4, a.rows); ++r) {
-      int slot = -1;
-      if (r < rows) {
-        while (r >= rs[b + 1]) ++b;
-        const int i = r - rs[b];
-        if (i < stor[b]) {
-          const int pos = len[b] + i, pg = page_of(b, pos / page);
-          if (pg >= 0 && pg < a.pages) slot = pg * page + pos % page;
-        }
-      }
-      a.slots[r] = slot;
-    }
+  for (int p = me; p < taken; p += step) {
+    const int b = upper_of(tk, B, p);
+    a.table[static_cast<size_t>(b) * a.ldt + held(b) + p - tk[b]] = a.ring[ring_at(head, p)];
+  }
+  for (int p = me; p < given; p += step) {
+    const int b = upper_of(gv, B, p);
+    a.ring[ring_at(tail, p)] = a.table[static_cast<size_t>(b) * a.ldt + p - gv[b]];
   }
   if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
   if (cluster_rank() == 0) {
@@ -201,7 +216,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     }
     if (threadIdx.x == 0) {
       a.row_start[B]   = rows;
-      a.state_out[0]   = (head + taken) % a.pages;
+      a.state_out[0]   = ring_at(head, taken) % a.pages;
       a.state_out[1]   = avail - taken + given;
       a.state_out[2]   = static_cast<int>(min(all - stored, 0x7fffffffLL));
       a.state_out[3]   = touched;
@@ -212,15 +227,17 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
 cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int32_t* state, int32_t* table, size_t ldt, size_t cols,
                            int32_t* ring, size_t pages, size_t B, size_t page, size_t rows, int32_t* row_start, int32_t* first,
                            int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t most, cudaStream_t st) {
+  int shift = 4;
+  while ((size_t(1) << shift) < page) ++shift;
   PlanArgs a{fresh, lens, state, table, ring, row_start, first, lens_out, state_out, slots, reinterpret_cast<int4*>(writes), ldt,
-             static_cast<int>(B), static_cast<int>(page), static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
+             static_cast<int>(B), shift, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
              static_cast<int>(most)};
   const int smem = static_cast<int>((6 * B + 4) * sizeof(int));
   static SmemAttrOnce once;
   cudaError_t e = set_max_smem_once(once, kv_plan_kernel, (6 * 8192 + 4) * 4);
   if (e != cudaSuccess) return e;
   // one CTA while its threads have a few rows each
-  const unsigned ctas = rows + most > 8 * kPlanThreads ? kPlanCluster : 1;
+  const unsigned ctas = rows / 4 + most > 2 * kPlanThreads ? kPlanCluster : 1;
   return launch_chained_cluster(kv_plan_kernel, dim3(ctas), dim3(kPlanThreads), smem, ctas, st, a);
 }
 

@@ -7,17 +7,21 @@
 //    The tiles of all units form one line; each warp takes an equal run of it, so a long context is split over as many
 //    warps as a batch of short ones. Runs that end inside a unit leave partial sums, joined in a fixed order: within a
 //    CTA through shared memory, between CTAs by kv_join_kernel.
-//  * A lane fetches exactly the 16-byte pieces that its own matrix fragments come from, with cp.async into its own slots
-//    of shared memory: deep queues without registers, no barriers, no bank conflicts, cache layout untouched.
+//  * Each warp has its own queue of tiles in shared memory, filled by cp.async: bytes in flight without registers, no barrier
+//    between warps, no bank conflicts, and the cache keeps plain rows. What a fetch instruction covers matters: eight neighbouring lanes
+//    a whole 128-byte line is the fast form (lanes of a quarter warp on four rows took 1.3 times as long for the same bytes).
 //  * S^T = K q^T and O^T = V^T P^T on mma.sync m16n8k16 (fp16 in, fp32 sums): tokens, then channels, are the 16 rows, the
-//    query rows the 8 columns, so a group of 8 heads wastes nothing. Codes become fp16 exactly (1024 + code + 128 by a
-//    byte permutation, minus 1152); k order and channel order are permuted the same way on both sides of a product.
+//    query rows the 8 columns, so a group of 8 heads wastes nothing. For S a code + 128 is an fp16 number by its bits alone (a
+//    multiple of 2^-24), and the sums start from -128 sum(q); for O, whose sums run over the whole context, codes become
+//    fp16 exactly (1024 + code + 128 by a byte permutation, minus 1152). k order and channel order are permuted the same way on both sides of a product.
 //  * Weights: 2^(s + log2 b - m), one running reference for the values and one for the sum of weights, so that scales
 //    that lie far apart lose neither. References are whole numbers and move only when a score passes them by 8 (weights
 //    stay below 2^15 in fp16; every rescale is exact).
 //  * fp32 activations: q and the weights enter as two fp16 parts each (22 bits), and every tile's product is added to the sums
 //    by fp32 additions (the tensor core cuts instead of rounding).
 #include "kdnn_common.cuh"
+
+#include <string.h>
 
 #include <algorithm>
 
@@ -26,20 +30,31 @@ namespace kdnn {
 constexpr int kKvWarps = 8;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kTop = 7.0f;        // weights are 2^(kTop + s - m): at most 2^15
-constexpr int kLeast = 4;           // tiles that a warp takes at least
+constexpr int kSwitch = 4;          // what going to another unit costs a warp, in tiles: each unit's place in the line is that much longer
+constexpr int kKnown = 1024;        // sequences whose lengths a CTA keeps in shared memory
+constexpr int kLeast = 2;           // tiles that a warp takes at least
 
+// A stage of a warp's queue: 16 tokens x DM codes of K, then of V, fetched as 16-byte pieces, eight neighbouring lanes a
+// 128-byte line. Pieces are placed so that neither the writes nor the fragment reads (lane = 4 g + c) meet in a bank:
+//   K, DM >= 128: piece ^ 4 (row & 1), read as pieces c + 4 k of the rows tau(g), tau(g) + 2
+//   V, DM >= 128: piece ^ 2 (row / 4 % 4), read as pieces g + 8 k of the rows 4 c + i
+//   V, DM = 64: row ^ (row / 4 % 2), piece ^ 2 (row / 8), read as 8 bytes at 8 g of the rows 4 c + i
 template <int DM>
 struct KvShape {
-  static constexpr int kKInstr = 2 * (DM / 64);                       // 16-byte pieces of K per lane and tile
-  static constexpr int kVInstr = 4 * (DM >= 128 ? DM / 128 : 1);      // pieces of V (8 bytes for DM = 64)
-  static constexpr int kVPiece = DM == 64 ? 8 : 16;
-  static constexpr int kStageBytes = kKInstr * 512 + kVInstr * 32 * kVPiece;
+  static constexpr int kPieces = DM / 16, kRows = 32 / kPieces, kInstr = 16 / kRows;   // pieces of a row; rows of a fetch; fetches of K
+  static constexpr int kStageBytes = 2 * 16 * DM;
+  static __device__ __forceinline__ uint32_t k_put(int row, int piece) {
+    return row * DM + (DM >= 128 ? piece ^ ((row & 1) << 2) : piece) * 16;
+  }
+  static __device__ __forceinline__ uint32_t v_put(int row, int piece) {
+    return DM >= 128 ? row * DM + (piece ^ (((row >> 2) & 3) << 1)) * 16 : (row ^ ((row >> 2) & 1)) * DM + (piece ^ (((row >> 3) & 1) << 1)) * 16;
+  }
 };
-// one partial sum: O [8 NT][DM], then m (values), m (sum), sum per row
+// one partial sum: the accumulators of O^T in register order ([NT][DM / 16] x 32 lanes x 4), then per row {m (values), m (sum), sum, 0}
 template <int DM, int NT>
 struct KvPart {
-  static constexpr int kRows = 8 * NT;
-  static constexpr int kFloats = kRows * (DM + 4);
+  static constexpr int kTiles = NT * DM / 16;
+  static constexpr int kRefs = kTiles * 128, kFloats = kRefs + 8 * NT * 4;
 };
 
 struct KvArgs {
@@ -47,7 +62,7 @@ struct KvArgs {
   const int8_t *k, *v;
   const float *ks, *vs;
   int pages, pshift;
-  float* parts;      // [CTA][2 kKvWarps + 2][KvPart::kFloats]: its warps' pieces, then its own two
+  float* parts;      // [CTA][kKvWarps + 2][KvPart::kFloats]: pieces that its warps put down before the end of their runs, then its own two
   int4* joins;       // [CTA]: the unit that begins in this CTA and ends in a later one: {CTAs that follow, b, unit, 0}
 };
 
@@ -81,12 +96,8 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
 }
 __device__ __forceinline__ float half_low(uint32_t v) { return __half2float(__ushort_as_half(static_cast<unsigned short>(v & 0xFFFFu))); }
 __device__ __forceinline__ float half_high(uint32_t v) { return __half2float(__ushort_as_half(static_cast<unsigned short>(v >> 16))); }
-template <int N>
 __device__ __forceinline__ void fetch(uint32_t dst, const void* src, int bytes) {   // bytes 0: zeros
-  if (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -102,36 +113,41 @@ __device__ __forceinline__ uint2 lds64(uint32_t p) {
   return v;
 }
 
-// What sequence b asks for: rows, token tiles [lo, hi) that some row of it can see (at least one, so that every row is written).
+// What sequence b asks for: rows, token tiles [lo, lo + tiles) that some row of it can see (at least one, so that every row is
+// written); `line` is a unit's length in the line of tiles.
 struct SeqWork {
-  int row0, n, first, len, lo, tiles, row_tiles;
+  int row0, n, first, len, lo, tiles, line, row_tiles;
 };
+__device__ __forceinline__ int4 seq_lengths(const AttnArgs& a, int pshift, int b) {
+  const int row0 = max(a.row_start[b], 0);
+  return make_int4(row0, max(min(a.row_start[b + 1], a.rows) - row0, 0), min(max(a.first[b], 0), 0x7fffffff - a.rows),
+                   min(max(a.lens[b], 0), a.cols << pshift));      // nothing lies behind the table's pages
+}
 template <int NT>
-__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int pshift, int b) {
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int G, int4 v) {
   SeqWork s;
-  s.row0  = max(a.row_start[b], 0);
-  s.n     = max(min(a.row_start[b + 1], a.rows) - s.row0, 0);
-  s.first = min(max(a.first[b], 0), 0x7fffffff - a.rows);
-  s.len   = min(max(a.lens[b], 0), a.cols << pshift);   // nothing lies behind the table's pages
-  const int end = static_cast<int>(min(static_cast<long long>(s.len), static_cast<long long>(s.first) + s.n));
+  s.row0 = v.x; s.n = v.y; s.first = v.z; s.len = v.w;
+  const int end = min(s.len, s.first + s.n);      // (first <= INT_MAX - rows)
   s.lo = a.window > 0 ? max(s.first - a.window + 1, 0) >> 4 : 0;
   s.tiles = s.n > 0 ? max(((end + 15) >> 4) - s.lo, 1) : 0;
-  const int G = a.heads / a.kv_heads;
+  s.line = s.tiles + kSwitch;
   s.row_tiles = static_cast<int>((static_cast<long long>(s.n) * G + 8 * NT - 1) / (8 * NT));
   return s;
 }
 
-// Tiles of the sequences before each one, for all threads of the CTA; at[seqs] is their sum.
+// The line before each sequence, for all threads of the CTA; at[seqs] is all of it. The first sequences' lengths stay in `known`.
 template <int NT>
-__device__ __forceinline__ void line_of(const AttnArgs& a, int pshift, long long* at) {
+__device__ __forceinline__ void line_of(const AttnArgs& a, int G, int pshift, long long* at, int4* known) {
   __shared__ long long s_warp[kKvWarps];
   const int T = kKvWarps * 32, per = (a.seqs + T - 1) / T, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int b0 = min(a.seqs, static_cast<int>(threadIdx.x) * per), b1 = min(a.seqs, b0 + per);
   long long sum = 0;
   for (int b = b0; b < b1; ++b) {
-    const SeqWork s = seq_work<NT>(a, pshift, b);
+    const int4 v = seq_lengths(a, pshift, b);
+    if (b < kKnown) known[b] = v;
+    const SeqWork s = seq_work<NT>(a, G, v);
     at[b] = sum;
-    sum += static_cast<long long>(s.tiles) * s.row_tiles * a.kv_heads;
+    sum += static_cast<long long>(s.line) * s.row_tiles * a.kv_heads;
   }
   long long inc = sum;
 #pragma unroll
@@ -152,95 +168,135 @@ __device__ __forceinline__ void line_of(const AttnArgs& a, int pshift, long long
   __syncthreads();
 }
 
-// One warp, query row r of a unit: the n partial sums that of(k) names (nullptr: none) as one, in that order; to the result, or as a
-// partial sum to `to`.
-template <class ST, int DM, int NT, class Of>
-__device__ __forceinline__ void join_row(const AttnArgs& a, const SeqWork& s, int unit, int r, int lane, int n, Of of, float* to) {
-  using Pt = KvPart<DM, NT>;
-  constexpr int W = DM >= 128 ? 4 : 2, V = DM / (32 * W);     // W neighbouring channels per lane, V times
-  float mz = kLowest, ml = kLowest, l = 0.0f, o[V][W];
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < W; ++e) o[i][e] = 0.0f;
-#pragma unroll 4
-  for (int k = 0; k < n; ++k) {
-    const float* part = of(k);
-    if (part == nullptr) continue;
-    const float4 m = __ldcg(reinterpret_cast<const float4*>(part + Pt::kRows * DM + r * 4));
-    float x[V][W];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (W == 4) *reinterpret_cast<float4*>(x[i]) = __ldcg(reinterpret_cast<const float4*>(part + r * DM + 128 * i + 4 * lane));
-      else *reinterpret_cast<float2*>(x[i]) = __ldcg(reinterpret_cast<const float2*>(part + r * DM + 2 * lane));
-    }
-    const float nz = fmaxf(mz, m.x), nl = fmaxf(ml, m.y);
-    const float f0 = ex2(mz - nz), f1 = ex2(m.x - nz);
-    l = l * ex2(ml - nl) + m.z * ex2(m.y - nl);
-    mz = nz;
-    ml = nl;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int e = 0; e < W; ++e) o[i][e] = o[i][e] * f0 + x[i][e] * f1;
-  }
-  if (to != nullptr) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (W == 4) *reinterpret_cast<float4*>(to + r * DM + 128 * i + 4 * lane) = *reinterpret_cast<float4*>(o[i]);
-      else *reinterpret_cast<float2*>(to + r * DM + 2 * lane) = *reinterpret_cast<float2*>(o[i]);
-    }
-    if (lane == 0) *reinterpret_cast<float4*>(to + Pt::kRows * DM + r * 4) = make_float4(mz, ml, l, 0.0f);
-    return;
-  }
-  const int G = a.heads / a.kv_heads, kvh = unit / s.row_tiles, f = (unit - kvh * s.row_tiles) * 8 * NT + r;
-  if (f >= s.n * G) return;
-  const int i0 = f / G;
-  ST* out = static_cast<ST*>(a.out) + static_cast<size_t>(s.row0 + i0) * a.ldo + static_cast<size_t>(kvh * G + f - i0 * G) * a.hdo;
-  const float y = l != 0.0f ? ex2(mz - ml - kTop) / l : 0.0f;
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      const int d = 128 * i + W * lane + e;
-      if (d < a.dim) store_scalar(out + d, y != 0.0f ? o[i][e] * y : 0.0f);
-    }
+// at[seqs + 1], known[min(seqs, kKnown)]
+__host__ __device__ inline uint32_t kv_lists_bytes(int seqs) {
+  return (((static_cast<uint32_t>(seqs + 1) * 8 + 15) & ~15u) + static_cast<uint32_t>(seqs < kKnown ? seqs : kKnown) * 16 + 127) & ~127u;
 }
 
-template <class ST, int DM, int NT, int STAGES>
+// First channel of m tile j of O^T for a lane: its accumulators are channels d (0, 1) and d + 1 (2, 3) of the rows 2 c (0, 2), 2 c + 1 (1, 3).
+template <int DM>
+__device__ __forceinline__ int channel_of(int j, int g) {
+  return DM == 64 ? 8 * g + 2 * j : 128 * (j >> 3) + 16 * g + 2 * (j & 7);
+}
+// Where row fr of a unit (first flattened row f0) goes.
+template <class ST>
+__device__ __forceinline__ ST* out_row(const AttnArgs& a, const SeqWork& s, int kvh, int G, int f) {
+  const int i = f / G;
+  return static_cast<ST*>(a.out) + static_cast<size_t>(s.row0 + i) * a.ldo + static_cast<size_t>(kvh * G + f - i * G) * a.hdo;
+}
+__device__ __forceinline__ void store_pair(float* p, float x, float y) { p[0] = x; p[1] = y; }
+__device__ __forceinline__ void store_pair(__nv_bfloat16* p, float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  if ((reinterpret_cast<uintptr_t>(p) & 3u) == 0) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = v;
+  } else {
+    p[0] = v.x;
+    p[1] = v.y;
+  }
+}
+
+// One warp, m tile j of row tile nt of a unit: its n partial sums (of(k) names the k-th) as one, in that order; to the result, or
+// as a partial sum to `to`. Loads of eight pieces are in flight at once.
+template <class ST, int DM, int NT, bool HERE, class Of>
+__device__ __forceinline__ void join_tile(const AttnArgs& a, const SeqWork& s, int unit, int nt, int j, int n, Of of, float* to) {
+  using Pt = KvPart<DM, NT>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int at = ((nt * (DM / 16) + j) * 32 + lane) * 4, ref = Pt::kRefs + (nt * 8 + 2 * c) * 4;
+  float mz[2] = {kLowest, kLowest}, ml[2] = {kLowest, kLowest}, l[2] = {0.0f, 0.0f};
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int k0 = 0; k0 < n; k0 += 8) {
+    float4 x[8], m[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float* part = of(min(k0 + k, n - 1));
+      auto get = [&](int i) {       // pieces of this CTA may lie in shared memory
+        return HERE ? *reinterpret_cast<const float4*>(part + i) : __ldcg(reinterpret_cast<const float4*>(part + i)); };
+      x[k] = get(at);
+      m[k][0] = get(ref);
+      m[k][1] = get(ref + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= n) break;
+      float f0[2], f1[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float nz = fmaxf(mz[h], m[k][h].x), nl = fmaxf(ml[h], m[k][h].y);
+        f0[h] = ex2(mz[h] - nz);
+        f1[h] = ex2(m[k][h].x - nz);
+        l[h] = l[h] * ex2(ml[h] - nl) + m[k][h].z * ex2(m[k][h].y - nl);
+        mz[h] = nz;
+        ml[h] = nl;
+      }
+      o.x = o.x * f0[0] + x[k].x * f1[0];
+      o.y = o.y * f0[1] + x[k].y * f1[1];
+      o.z = o.z * f0[0] + x[k].z * f1[0];
+      o.w = o.w * f0[1] + x[k].w * f1[1];
+    }
+  }
+  if (to != nullptr) {
+    *reinterpret_cast<float4*>(to + at) = o;
+    if (j == 0 && g == 0) {
+      *reinterpret_cast<float4*>(to + ref) = make_float4(mz[0], ml[0], l[0], 0.0f);
+      *reinterpret_cast<float4*>(to + ref + 4) = make_float4(mz[1], ml[1], l[1], 0.0f);
+    }
+    return;
+  }
+  const int G = a.heads / a.kv_heads, kvh = unit / s.row_tiles, f = (unit - kvh * s.row_tiles) * 8 * NT + nt * 8 + 2 * c;
+  const int d = channel_of<DM>(j, g);
+  if (d >= a.dim) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (f + h >= s.n * G) continue;
+    const float y = l[h] != 0.0f ? ex2(mz[h] - ml[h] - kTop) / l[h] : 0.0f;
+    const float u = h ? o.y : o.x, v = h ? o.w : o.z;
+    store_pair(out_row<ST>(a, s, kvh, G, f + h) + d, y != 0.0f ? u * y : 0.0f, y != 0.0f ? v * y : 0.0f);
+  }
+}
+
+// FULL: dim == DM (piece addresses are immediate offsets).
+template <class ST, int DM, int NT, int STAGES, bool FULL>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) kv_attention_kernel(KvArgs p) {
   using Sh = KvShape<DM>;
   using Pt = KvPart<DM, NT>;
   constexpr int PARTS = sizeof(ST) == 4 ? 2 : 1;
   constexpr int KS = DM / 16;                       // k steps of S, and m tiles of O
+  static_assert(Pt::kFloats * 4 <= STAGES * Sh::kStageBytes, "a piece fits where the queue was");
   pdl_chain_entry();
   extern __shared__ __align__(16) uint8_t sm[];
   const AttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int G = a.heads / a.kv_heads, D = a.dim, page = 1 << p.pshift;
+  const int G = a.heads / a.kv_heads, D = FULL ? DM : a.dim, page = 1 << p.pshift;
   long long* at = reinterpret_cast<long long*>(sm);
-  uint8_t* ring = sm + ((static_cast<size_t>(a.seqs + 1) * 8 + 127) & ~size_t(127));
-  __shared__ float4 s_meta[kKvWarps][STAGES];
-  __shared__ int4 s_seg[2 * kKvWarps];              // pieces of this CTA's warps: {b, unit, 1, .}; z 0: none
-  line_of<NT>(a, p.pshift, at);
+  int4* known = reinterpret_cast<int4*>(sm + ((static_cast<uint32_t>(a.seqs + 1) * 8 + 15) & ~15u));
+  const uint32_t ring = smem_u32(sm) + kv_lists_bytes(a.seqs);
+  __shared__ int s_order[kKvWarps][2 * kKvWarps];
+  __shared__ int4 s_seg[2 * kKvWarps];              // pieces of this CTA's warps: {b, unit, 1, in the queue's place}; z 0: none
+  line_of<NT>(a, G, p.pshift, at, known);
+  auto work_of = [&](int b) { return seq_work<NT>(a, G, b < kKnown ? known[b] : seq_lengths(a, p.pshift, b)); };
   const long long total = at[a.seqs];
-  // warps that take a run: all of a CTA's where there is enough for them, else fewer in every CTA
-  const int ctas = gridDim.x;
-  const int wpc  = static_cast<int>(max(1LL, min(static_cast<long long>(kKvWarps), (total + static_cast<long long>(kLeast) * ctas - 1) / (static_cast<long long>(kLeast) * ctas))));
-  const long long workers = max(1LL, min(static_cast<long long>(wpc) * ctas, (total + kLeast - 1) / kLeast));
-  auto start_of = [&](long long i) { return i >= workers ? total : total * i / workers; };
-  const long long my0 = static_cast<long long>(blockIdx.x) * wpc;
-  const long long cta0 = start_of(my0), cta1 = start_of(my0 + wpc);
-  long long pos = w < wpc ? start_of(my0 + w) : 0;
-  const long long end = w < wpc ? start_of(my0 + w + 1) : 0, begin = pos;
+  // every warp takes a run while there are kLeast tiles for it; with fewer, the first CTAs' warps do. (Several runs per warp, the later
+  // ones by CTAs that follow on the SMs that finish early, cost more than the SMs' different bandwidths: 122 us against 98 for
+  // three contexts of 131071.)
+  const int workers = static_cast<int>(max(1LL, min(static_cast<long long>(kKvWarps) * gridDim.x, (total + kLeast - 1) / kLeast)));
+  const long long share = total < 0x7fffffffLL ? static_cast<int>(total) / workers : total / workers;
+  const int longer = static_cast<int>(total - share * workers);      // the first ones take one tile more
+  auto start_of = [&](int i) { return i >= workers ? total : share * i + min(i, longer); };
+  const int my0 = blockIdx.x * kKvWarps;
+  const long long cta0 = start_of(my0), cta1 = start_of(my0 + kKvWarps);
+  long long pos = start_of(my0 + w);
+  const long long end = start_of(my0 + w + 1), begin = pos;
   if (lane < 2) s_seg[2 * w + lane] = make_int4(0, 0, 0, 0);
 
-  const uint32_t my_ring = smem_u32(ring) + static_cast<uint32_t>(w) * STAGES * Sh::kStageBytes;
-  const uint32_t my_k = my_ring + lane * 16, my_v = my_ring + Sh::kKInstr * 512 + lane * Sh::kVPiece;
+  const uint32_t my_ring = ring + static_cast<uint32_t>(w) * STAGES * Sh::kStageBytes;
+  // the pieces this lane fetches: row lr + i kRows, piece lc; and where it reads
+  const int lr = lane / Sh::kPieces, lc = lane % Sh::kPieces;
+  const int lane_at = lr * D + (FULL || lc * 16 < D ? lc * 16 : 0), lane_bytes = FULL || lc * 16 < D ? 16 : 0;
+  const int tau = 4 * (g >> 1) + (g & 1), dk = 16 * c;
 
-  float acc[NT][KS][4];        // O^T: m tile t = 2 word + half of word: rows d = 16 g + 2 t + {0 (c0, c1), 1 (c2, c3)}
+  float acc[NT][KS][4];
   float mz[NT][2], ml[NT][2], l[NT][2];
-  // where a lane's channels lie: DM = 64: 8 g + 2 t; 128: 16 g + 2 t; 256: 16 g + 2 t (t < 8), 128 + 16 g + 2 (t - 8)
+
   int b = 0;
   SeqWork s{};
   long long in_b = 0;          // tiles of sequence b before pos
@@ -251,108 +307,148 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
       if (at[mid] <= pos) lo = mid; else hi = mid;
     }
     b = lo;
-    s = seq_work<NT>(a, p.pshift, b);
+    s = work_of(b);
     in_b = pos - at[b];
   }
   while (pos < end) {
-    while (in_b >= static_cast<long long>(s.tiles) * s.row_tiles * a.kv_heads) {
+    while (in_b >= static_cast<long long>(s.line) * s.row_tiles * a.kv_heads) {
       in_b = 0;
-      s = seq_work<NT>(a, p.pshift, ++b);
+      s = work_of(++b);
     }
-    const int unit = static_cast<int>(in_b / s.tiles), tile = static_cast<int>(in_b - static_cast<long long>(unit) * s.tiles);
-    const int take = static_cast<int>(min(static_cast<long long>(s.tiles - tile), end - pos));
-    const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
+    const int unit = in_b < 0x7fffffffLL ? static_cast<int>(in_b) / s.line : static_cast<int>(in_b / s.line);
+    const int place = static_cast<int>(in_b - static_cast<long long>(unit) * s.line);
+    const int run = static_cast<int>(min(static_cast<long long>(s.line - place), end - pos));
+    const bool first_of_run = pos == begin;
+    pos += run;
+    in_b += run;
+    const int tile = max(place - kSwitch, 0), take = place + run - kSwitch - tile;
+    if (take <= 0) continue;      // the run ends before the unit's first tile
+    const int kvh = s.row_tiles == 1 ? unit : unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
     const int f0 = rt * 8 * NT, fn = min(8 * NT, s.n * G - f0);            // query rows of the unit: token f / G, head f % G
     // tiles that some row of the unit sees
     const int p_lo = s.first + f0 / G, p_hi = s.first + (f0 + fn - 1) / G;
     const int u_hi = min(s.len, p_hi + 1), u_lo = a.window > 0 ? max(p_lo - a.window + 1, 0) : 0;
     const int t_beg = max(s.lo + tile, u_lo >> 4), t_end = min(s.lo + tile + take, (u_hi + 15) >> 4);
 
-    // ---- queue of tiles
-    int chunk = -1, c_pg = -1;
-    float c_ks = 0.0f, c_ev = -INFINITY;
-    auto issue = [&](int t) {
-      if (t < t_end) {
-        const int j = (t << 4) >> p.pshift;
-        if (chunk < 0 || j - chunk >= 32) {       // the next 32 pages: a page and its scales per lane
-          chunk = j;
-          const int jj = j + lane;
-          c_pg = -1;
-          if (jj < a.cols && (static_cast<long long>(jj) << p.pshift) < u_hi) c_pg = a.table[static_cast<size_t>(b) * a.ldt + jj];
-          if (c_pg >= p.pages) c_pg = -1;
-          if (c_pg >= 0) {
-            const size_t ph = static_cast<size_t>(c_pg) * a.kv_heads + kvh;
-            c_ks = p.ks[ph];
-            const uint32_t vb = __float_as_uint(p.vs[ph]);
-            c_ev = vb == 0u ? -INFINITY : static_cast<float>(static_cast<int>((vb >> 23) & 0xFFu) - 127);
+    // ---- the unit's query rows are requested
+    constexpr int QW = DM / 4 * sizeof(ST) / 16;      // 16-byte words of a lane's share of a row
+    uint4 raw[NT][QW];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int f = min(nt * 8 + g, fn - 1) + f0, i = f / G;
+      const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(s.row0 + i) * a.ldq + static_cast<size_t>(kvh * G + f - i * G) * a.hdq;
+      constexpr int PER = 16 / sizeof(ST);            // elements of a word
+      const bool vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
+#pragma unroll
+      for (int k = 0; k < QW; ++k) {
+        const int d = 64 * (k / (16 / PER)) + dk + PER * (k % (16 / PER));
+        raw[nt][k] = make_uint4(0u, 0u, 0u, 0u);
+        if (d < D) {
+          if (vec) {
+            raw[nt][k] = *reinterpret_cast<const uint4*>(q + d);
+          } else {
+            ST v[PER];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[e] = q[d + e];
+            memcpy(&raw[nt][k], v, 16);
           }
         }
-        const int pg = __shfl_sync(0xffffffffu, c_pg, j - chunk);
-        const float ks = __shfl_sync(0xffffffffu, c_ks, j - chunk), ev = __shfl_sync(0xffffffffu, c_ev, j - chunk);
-        const int st = t % STAGES;
-        if (lane == 0) s_meta[w][st] = make_float4(ks, ev, pg >= 0 ? 1.0f : 0.0f, 0.0f);
-        const size_t base = ((static_cast<size_t>(max(pg, 0)) * a.kv_heads + kvh) * page + ((t << 4) & (page - 1))) * D;
-        const bool there = pg >= 0;
-        const uint32_t kd = my_k + st * Sh::kStageBytes, vd = my_v + st * Sh::kStageBytes;
-#pragma unroll
-        for (int i = 0; i < Sh::kKInstr; ++i) {
-          const int tok = 4 * (g >> 1) + (g & 1) + 2 * (i & 1), d = 16 * c + 64 * (i >> 1);
-          fetch<16>(kd + i * 512, p.k + base + tok * D + (d < D ? d : 0), there && d < D ? 16 : 0);
+      }
+    }
+
+    // ---- queue of tiles. The next 32 pages and their scales are held one per lane; those of the 32 before stay for the
+    // tiles that are still in the queue.
+    int chunk = -32, c_pg = -1, o_chunk = -32, o_pg = -1;
+    float c_ks = 0.0f, c_vs = 0.0f, o_ks = 0.0f, o_vs = 0.0f;
+    const int8_t *kp = p.k, *vp = p.v;
+    int there = 0, in_stage = 0;
+    auto issue = [&](int t) {
+      if (t < t_end) {
+        const int off = (t << 4) & (page - 1);
+        if (off == 0 || t == t_beg) {
+          const int j = (t << 4) >> p.pshift;
+          if (j - chunk >= 32) {
+            o_chunk = chunk; o_pg = c_pg; o_ks = c_ks; o_vs = c_vs;
+            chunk = j;
+            const int jj = j + lane;
+            c_pg = -1;
+            if (jj < a.cols && (static_cast<long long>(jj) << p.pshift) < u_hi) c_pg = a.table[static_cast<size_t>(b) * a.ldt + jj];
+            if (c_pg >= p.pages || c_pg < 0) {
+              c_pg = -1;
+            } else {
+              const size_t ph = static_cast<size_t>(c_pg) * a.kv_heads + kvh;
+              c_ks = p.ks[ph];
+              c_vs = p.vs[ph];
+            }
+          }
+          const int pg = __shfl_sync(0xffffffffu, c_pg, j - chunk);
+          there = pg >= 0 ? lane_bytes : 0;
+          const size_t base = ((static_cast<size_t>(max(pg, 0)) * a.kv_heads + kvh) * page + off) * D + lane_at;
+          kp = p.k + base;
+          vp = p.v + base;
+        } else {
+          kp += 16 * D;
+          vp += 16 * D;
         }
+        const uint32_t kd = my_ring + in_stage * Sh::kStageBytes, vd = kd + 16 * DM;
 #pragma unroll
-        for (int i = 0; i < Sh::kVInstr; ++i) {
-          const int tok = 4 * c + (i & 3), d = DM == 64 ? 8 * g : 16 * g + 128 * (i >> 2);
-          fetch<Sh::kVPiece>(vd + i * 32 * Sh::kVPiece, p.v + base + tok * D + (d < D ? d : 0), there && d < D ? Sh::kVPiece : 0);
-        }
+        for (int i = 0; i < Sh::kInstr; ++i) fetch(kd + Sh::k_put(lr + i * Sh::kRows, lc), kp + i * Sh::kRows * D, there);
+#pragma unroll
+        for (int i = 0; i < Sh::kInstr; ++i) fetch(vd + Sh::v_put(lr + i * Sh::kRows, lc), vp + i * Sh::kRows * D, there);
       }
       fetch_commit();
+      if (++in_stage == STAGES) in_stage = 0;
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(t_beg + i);
 
-    // ---- the unit's query rows
+    // ---- query rows as fp16 fragments
     uint32_t qf[PARTS][NT][KS][2];
-    float rsc[NT][2];
+    float rsc[NT][2], bias[NT][2];      // factor of a row's scores; 128 sum(q) in their units: products are with code + 128
     int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int f = min(nt * 8 + g, fn - 1) + f0;
-      const int i = f / G;
-      const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(s.row0 + i) * a.ldq + static_cast<size_t>(kvh * G + f - i * G) * a.hdq;
-      const bool vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
       float x[DM / 4];
       float amax = 0.0f;
 #pragma unroll
-      for (int k = 0; k < DM / 64; ++k)
+      for (int k = 0; k < QW; ++k) {
+        constexpr int PER = 16 / sizeof(ST);
+        ST v[PER];
+        memcpy(v, &raw[nt][k], 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          const int d = 64 * k + 16 * c + 8 * h;
-          if (d < D) load8<ST>(q, static_cast<size_t>(d), vec, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[k * 16 + h * 8 + e] = t[e];
-            amax = fmaxf(amax, fabsf(t[e]));
-          }
+        for (int e = 0; e < PER; ++e) {
+          x[k * PER + e] = to_f32(v[e]);
+          amax = fmaxf(amax, fabsf(x[k * PER + e]));
         }
+      }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // the row's largest value is taken to [2^7, 2^8)
       const int e = amax > 0.0f ? max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100) : 0;
       const float to = __uint_as_float(static_cast<uint32_t>(7 - e + 127) << 23);
       const float back = __uint_as_float(static_cast<uint32_t>(e - 7 + 127) << 23);
+      float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < KS; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float v0 = x[4 * j + 2 * h] * to, v1 = x[4 * j + 2 * h + 1] * to;
-          qf[0][nt][j][h] = half_pair(v0, v1);
-          if (PARTS == 2) qf[PARTS - 1][nt][j][h] = half_pair(v0 - half_low(qf[0][nt][j][h]), v1 - half_high(qf[0][nt][j][h]));
+          const uint32_t u = half_pair(v0, v1);
+          qf[0][nt][j][h] = u;
+          sum += half_low(u) + half_high(u);
+          if (PARTS == 2) {
+            const uint32_t r = half_pair(v0 - half_low(u), v1 - half_high(u));
+            qf[PARTS - 1][nt][j][h] = r;
+            sum += half_low(r) + half_high(r);
+          }
         }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       const float r = a.scale * 1.4426950408889634f * back;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        rsc[nt][h] = __shfl_sync(0xffffffffu, r, (2 * c + h) * 4);
+        rsc[nt][h]  = __shfl_sync(0xffffffffu, r, (2 * c + h) * 4) * 16777216.0f;
+        bias[nt][h] = __shfl_sync(0xffffffffu, sum, (2 * c + h) * 4) * -0x1p-17f;
         const int fr = f0 + min(nt * 8 + 2 * c + h, fn - 1), ps = s.first + fr / G;
         hi[nt][h] = min(s.len, ps + 1);
         lo[nt][h] = a.window > 0 ? ps - a.window + 1 : 0;
@@ -364,27 +460,57 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
 #pragma unroll
         for (int e2 = 0; e2 < 4; ++e2) acc[nt][j][e2] = 0.0f;
     }
-    // tokens below in_hi and from in_lo on are seen by every row
-    const int in_hi = min(s.len, p_lo + 1), in_lo = a.window > 0 ? p_hi - a.window + 1 : 0;
+    // tiles [in_lo, in_hi) are seen whole by every row
+    const int in_hi = min(s.len, p_lo + 1) >> 4, in_lo = a.window > 0 ? (max(p_hi - a.window + 1, 0) + 15) >> 4 : 0;
 
+    int stage = 0;
+    bool gone = false;                                   // the page is not there
+    float ev = 0.0f;                                     // log2 of its value scale
+    float rk[NT][2], az[NT][2], lim[NT][2];              // score factor, exponent offset of the weights, where a reference moves
+    auto refs = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          az[nt][h]  = ev + kTop - mz[nt][h];
+          lim[nt][h] = fminf(ml[nt][h], mz[nt][h] - ev) + 8.0f;
+        }
+    };
     for (int t = t_beg; t < t_end; ++t) {
+      __syncwarp();             // the stage that the next fetch goes to has been read
       issue(t + STAGES - 1);
       fetch_wait<STAGES - 1>();
-      __syncwarp();
-      const int st = t % STAGES;
-      const float4 meta = s_meta[w][st];
-      // ---- S^T
+      __syncwarp();             // everybody's pieces are there
+      if (((t << 4) & (page - 1)) == 0 || t == t_beg) {   // another page
+        const int j = (t << 4) >> p.pshift;
+        const bool old = j < chunk;
+        const int src = j - (old ? o_chunk : chunk);
+        gone = __shfl_sync(0xffffffffu, old ? o_pg : c_pg, src) < 0;
+        const float ks = __shfl_sync(0xffffffffu, old ? o_ks : c_ks, src);
+        const uint32_t vb = __float_as_uint(__shfl_sync(0xffffffffu, old ? o_vs : c_vs, src));
+        ev = vb == 0u ? -INFINITY : static_cast<float>(static_cast<int>((vb >> 23) & 0xFFu) - 127);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) rk[nt][h] = rsc[nt][h] * ks;
+        refs();
+      }
+      const uint32_t kd = my_ring + stage * Sh::kStageBytes, vd = kd + 16 * DM;
+      if (++stage == STAGES) stage = 0;
+      // ---- S^T: codes + 128 as fp16 by their bits (whole multiples of 2^-24)
       float sc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[nt][e] = bias[nt][e & 1];
 #pragma unroll
       for (int k = 0; k < DM / 64; ++k) {
-        const uint4 k0 = lds128(my_k + st * Sh::kStageBytes + (2 * k) * 512), k1 = lds128(my_k + st * Sh::kStageBytes + (2 * k + 1) * 512);
+        const uint4 k0 = lds128(kd + Sh::k_put(tau, c + 4 * k)), k1 = lds128(kd + Sh::k_put(tau + 2, c + 4 * k));
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
-          const uint32_t a0 = code_pair(u0, 0x4140), a2 = code_pair(u0, 0x4342), a1 = code_pair(u1, 0x4140), a3 = code_pair(u1, 0x4342);
+          const uint32_t a0 = prmt(u0, 0u, 0x4140), a2 = prmt(u0, 0u, 0x4342), a1 = prmt(u1, 0u, 0x4140), a3 = prmt(u1, 0u, 0x4342);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -392,21 +518,26 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
         }
       }
       // ---- scores: token tau(g) (e = 0, 1) and tau(g) + 2 (e = 2, 3) against the rows 2 c, 2 c + 1
-      const int t0 = (t << 4) + 4 * (g >> 1) + (g & 1);
-      const bool edge = (t << 4) + 16 > in_hi || (t << 4) < in_lo || meta.z == 0.0f;
+      const bool edge = t >= in_hi || t < in_lo || gone;
       bool over = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = sc[nt][e] * rsc[nt][e & 1] * meta.x;
-          if (edge) {
+        for (int e = 0; e < 4; ++e) sc[nt][e] *= rk[nt][e & 1];
+      if (edge) {
+        const int t0 = (t << 4) + 4 * (g >> 1) + (g & 1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
             const int tok = t0 + (e & 2);
-            if (tok >= hi[nt][e & 1] || tok < lo[nt][e & 1] || meta.z == 0.0f) v = -INFINITY;
+            if (tok >= hi[nt][e & 1] || tok < lo[nt][e & 1] || gone) sc[nt][e] = -INFINITY;
           }
-          sc[nt][e] = v;
-          over |= v > ml[nt][e & 1] + 8.0f || v + meta.y > mz[nt][e & 1] + 8.0f;
-        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) over |= fmaxf(sc[nt][h], sc[nt][2 + h]) > lim[nt][h];
       if (__any_sync(0xffffffffu, over)) {     // a reference moves: both, for every row
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -416,7 +547,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float nl = fmaxf(ml[nt][h], ceilf(top)), nz = fmaxf(mz[nt][h], ceilf(top) + meta.y);
+            const float nl = fmaxf(ml[nt][h], ceilf(top)), nz = fmaxf(mz[nt][h], ceilf(top) + ev);
             l[nt][h] *= ex2(ml[nt][h] - nl);
             const float f = ex2(mz[nt][h] - nz);
             ml[nt][h] = nl;
@@ -427,6 +558,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
               acc[nt][j][2 + h] *= f;
             }
           }
+        refs();
       }
       uint32_t pf[PARTS][NT][2];
 #pragma unroll
@@ -435,7 +567,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           l[nt][e & 1] += ex2(sc[nt][e] - ml[nt][e & 1]);
-          wv[e] = ex2(sc[nt][e] + (meta.y + kTop) - mz[nt][e & 1]);
+          wv[e] = ex2(sc[nt][e] + az[nt][e & 1]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -450,7 +582,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
         uint32_t v[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t ad = my_v + st * Sh::kStageBytes + (4 * k + i) * 32 * Sh::kVPiece;
+          const uint32_t ad = vd + Sh::v_put(4 * c + i, DM == 64 ? g >> 1 : g + 8 * k) + (DM == 64 ? 8 * (g & 1) : 0);
           if (DM == 64) {
             const uint2 x = lds64(ad);
             v[i][0] = x.x; v[i][1] = x.y; v[i][2] = v[i][3] = 0u;
@@ -495,105 +627,100 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
         l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 8);
         l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 16);
       }
-    const bool whole = take == s.tiles;
-    if (whole) {
+    if (take == s.tiles) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int fr = nt * 8 + 2 * c + h;
           if (fr >= fn) continue;
-          const int i = (f0 + fr) / G;
-          ST* o = static_cast<ST*>(a.out) + static_cast<size_t>(s.row0 + i) * a.ldo + static_cast<size_t>(kvh * G + f0 + fr - i * G) * a.hdo;
+          ST* o = out_row<ST>(a, s, kvh, G, f0 + fr);
           const float f = l[nt][h] != 0.0f ? ex2(mz[nt][h] - ml[nt][h] - kTop) / l[nt][h] : 0.0f;
 #pragma unroll
-          for (int j = 0; j < KS; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = DM == 64 ? 8 * g + 2 * j + e : 128 * (j >> 3) + 16 * g + 2 * (j & 7) + e;
-              if (d < D) store_scalar(o + d, f != 0.0f ? acc[nt][j][2 * e + h] * f : 0.0f);
-            }
+          for (int j = 0; j < KS; ++j) {
+            const int d = channel_of<DM>(j, g);
+            if (FULL || d < D) store_pair(o + d, f != 0.0f ? acc[nt][j][h] * f : 0.0f, f != 0.0f ? acc[nt][j][2 + h] * f : 0.0f);
+          }
         }
     } else {
       // at most two pieces in a run: of a unit that began before it (or at its start), and of one that goes on behind it
-      const int slot = 2 * w + (pos == begin ? 0 : 1);
-      float* part = p.parts + (static_cast<size_t>(blockIdx.x) * (2 * kKvWarps + 2) + slot) * Pt::kFloats;
+      // (the last one lies where the warp's queue was)
+      const int slot = 2 * w + (first_of_run ? 0 : 1);
+      float* part = pos == end ? reinterpret_cast<float*>(sm + (my_ring - smem_u32(sm)))
+                               : p.parts + (static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) + w) * Pt::kFloats;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int fr = nt * 8 + 2 * c + h;
+        for (int j = 0; j < KS; ++j)
+          *reinterpret_cast<float4*>(part + ((nt * KS + j) * 32 + lane) * 4) = make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
+        if (g == 0) {
 #pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            const int d = DM == 64 ? 8 * g + 2 * j : 128 * (j >> 3) + 16 * g + 2 * (j & 7);
-            *reinterpret_cast<float2*>(part + fr * DM + d) = make_float2(acc[nt][j][h], acc[nt][j][2 + h]);
-          }
-          if (g == 0) *reinterpret_cast<float4*>(part + Pt::kRows * DM + fr * 4) = make_float4(mz[nt][h], ml[nt][h], l[nt][h], 0.0f);
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float4*>(part + Pt::kRefs + (nt * 8 + 2 * c + h) * 4) = make_float4(mz[nt][h], ml[nt][h], l[nt][h], 0.0f);
         }
-      if (lane == 0) s_seg[slot] = make_int4(b, unit, 1, 0);
+      }
+      if (lane == 0) s_seg[slot] = make_int4(b, unit, 1, pos == end);
     }
-    pos += take;
-    in_b += take;
   }
 
-  // ---- pieces of one unit that this CTA's warps hold are joined, a row per warp
+  // ---- pieces of one unit that this CTA's warps hold are joined, an m tile per warp
   __syncthreads();
-  const float* mine = p.parts + static_cast<size_t>(blockIdx.x) * (2 * kKvWarps + 2) * Pt::kFloats;
+  const float* mine = p.parts + static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) * Pt::kFloats;
+  const float* queues = reinterpret_cast<const float*>(sm + (ring - smem_u32(sm)));
   int4 goes_on = make_int4(0, 0, 0, 0);
-  for (int i = 0; i < 2 * kKvWarps;) {
-    const int4 seg = s_seg[i];
-    if (seg.z == 0) {
-      ++i;
-      continue;
+  const int4 seg = lane < 2 * kKvWarps ? s_seg[lane] : make_int4(0, 0, 0, 0);
+  for (unsigned left = __ballot_sync(0xffffffffu, seg.z != 0); left != 0;) {
+    const int i = __ffs(left) - 1, ub = __shfl_sync(0xffffffffu, seg.x, i), uu = __shfl_sync(0xffffffffu, seg.y, i);
+    const unsigned group = __ballot_sync(0xffffffffu, seg.z != 0 && seg.x == ub && seg.y == uu);
+    left &= ~group;
+    if ((group >> lane) & 1u) s_order[w][__popc(group & ((1u << lane) - 1u))] = lane;
+    __syncwarp();
+    const SeqWork u = work_of(ub);
+    const long long u1 = at[ub] + static_cast<long long>(uu + 1) * u.line, u0 = u1 - u.tiles;
+    float* to = p.parts + (static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) + kKvWarps + (u0 < cta0 ? 0 : 1)) * Pt::kFloats;
+    for (int x = w; x < Pt::kTiles; x += kKvWarps)
+      join_tile<ST, DM, NT, true>(a, u, uu, x / KS, x % KS, __popc(group), [&](int k) {
+        const int at = s_order[w][k];
+        return s_seg[at].w ? queues + (at >> 1) * (STAGES * Sh::kStageBytes / 4) : mine + (at >> 1) * Pt::kFloats; },
+                            u0 >= cta0 && u1 <= cta1 ? nullptr : to);
+    if (u0 >= cta0 && u1 > cta1) {      // how many CTAs further its last tile is
+      const long long x = u1 - 1, cut = (share + 1) * longer;
+      const int in = static_cast<int>(x < cut ? x / (share + 1) : longer + (x - cut) / share);
+      goes_on = make_int4(in / kKvWarps - static_cast<int>(blockIdx.x), ub, uu, 0);
     }
-    int n = i + 1;      // the unit's pieces follow one another, with unused places between them
-    for (int k = i + 1; k < 2 * kKvWarps; ++k) {
-      const int4 o = s_seg[k];
-      if (o.z != 0 && (o.x != seg.x || o.y != seg.y)) break;
-      if (o.z != 0) n = k + 1;
-    }
-    const SeqWork u = seq_work<NT>(a, p.pshift, seg.x);
-    const long long u0 = at[seg.x] + static_cast<long long>(seg.y) * u.tiles, u1 = u0 + u.tiles;
-    const bool whole = u0 >= cta0 && u1 <= cta1;
-    float* to = p.parts + (static_cast<size_t>(blockIdx.x) * (2 * kKvWarps + 2) + 2 * kKvWarps + (u0 < cta0 ? 0 : 1)) * Pt::kFloats;
-    for (int r = w; r < 8 * NT; r += kKvWarps)
-      join_row<ST, DM, NT>(a, u, seg.y, r, lane, n - i, [&](int k) {
-        return s_seg[i + k].z != 0 ? mine + static_cast<size_t>(i + k) * Pt::kFloats : nullptr; }, whole ? nullptr : to);
-    if (u0 >= cta0 && u1 > cta1) {      // the CTA of its last tile
-      long long x = (u1 - 1) * workers / total;
-      while (start_of(x + 1) <= u1 - 1) ++x;
-      while (start_of(x) > u1 - 1) --x;
-      goes_on = make_int4(static_cast<int>(x / wpc) - static_cast<int>(blockIdx.x), seg.x, seg.y, 0);
-    }
-    i = n;
+    __syncwarp();
   }
   if (threadIdx.x == 0) p.joins[blockIdx.x] = goes_on;
 }
 
-// Units that several CTAs share, joined by the one they begin in: a row per warp.
+// Units that several CTAs share, joined by the one they begin in: an m tile per warp.
 template <class ST, int DM, int NT>
-__global__ void __launch_bounds__(NT * 256) kv_join_kernel(KvArgs p) {
+__global__ void __launch_bounds__(NT * DM * 2) kv_join_kernel(KvArgs p) {
   using Pt = KvPart<DM, NT>;
   pdl_chain_entry();
-  const int4 job = p.joins[blockIdx.x];
+  const int4 job = __ldcg(p.joins + blockIdx.x);
   if (job.x <= 0) return;
-  const SeqWork u = seq_work<NT>(p.a, p.pshift, job.y);
-  const int first = blockIdx.x;
-  join_row<ST, DM, NT>(p.a, u, job.z, threadIdx.x >> 5, threadIdx.x & 31, job.x + 1, [&](int k) {
-    return p.parts + (static_cast<size_t>(first + k) * (2 * kKvWarps + 2) + 2 * kKvWarps + (k == 0 ? 1 : 0)) * Pt::kFloats; },
-    nullptr);
+  const SeqWork u = seq_work<NT>(p.a, p.a.heads / p.a.kv_heads, seq_lengths(p.a, p.pshift, job.y));
+  const float* first = p.parts + (static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) + kKvWarps) * Pt::kFloats;
+  const int w = threadIdx.x >> 5;
+  join_tile<ST, DM, NT, false>(p.a, u, job.z, w / (DM / 16), w % (DM / 16), job.x + 1, [&](int k) {
+    return first + (static_cast<size_t>(k) * (kKvWarps + 2) + (k == 0 ? 1 : 0)) * Pt::kFloats; }, nullptr);
 }
 
-template <class ST, int DM, int NT, int STAGES>
+template <class ST, int DM, int NT, int STAGES, bool FULL>
 static cudaError_t launch_kv(const KvArgs& p, int ctas, cudaStream_t st) {
   const size_t ring = static_cast<size_t>(kKvWarps) * STAGES * KvShape<DM>::kStageBytes;
-  const size_t smem = ((static_cast<size_t>(p.a.seqs + 1) * 8 + 127) & ~size_t(127)) + ring;
+  const size_t smem = kv_lists_bytes(p.a.seqs) + ring;
   static SmemAttrOnce once;
-  cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, NT, STAGES>, static_cast<int>(ring + 8193 * 8 + 128));
+  cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, NT, STAGES, FULL>, static_cast<int>(ring + kv_lists_bytes(8192)));
   if (e == cudaSuccess)
-    e = launch_chained(kv_attention_kernel<ST, DM, NT, STAGES>, dim3(ctas), dim3(kKvWarps * 32), smem, st, p);
-  if (e == cudaSuccess) e = launch_chained(kv_join_kernel<ST, DM, NT>, dim3(ctas), dim3(NT * 256), 0, st, p);
+    e = launch_chained(kv_attention_kernel<ST, DM, NT, STAGES, FULL>, dim3(ctas), dim3(kKvWarps * 32), smem, st, p);
+  if (e == cudaSuccess) e = launch_chained(kv_join_kernel<ST, DM, NT>, dim3(ctas), dim3(NT * DM * 2), 0, st, p);
   return e;
+}
+template <class ST, int DM, int NT, int STAGES>
+static cudaError_t launch_kv_dim(const KvArgs& p, int ctas, cudaStream_t st) {
+  return p.a.dim == DM ? launch_kv<ST, DM, NT, STAGES, true>(p, ctas, st) : launch_kv<ST, DM, NT, STAGES, false>(p, ctas, st);
 }
 
 int device_sm_count();
@@ -604,7 +731,7 @@ static int kv_nt(size_t rows, size_t seqs, size_t heads, size_t kv_heads, int dm
   return dm == 256 || (rows + seqs - 1) / seqs * (heads / kv_heads) <= 8 ? 1 : 2;
 }
 static int kv_ctas(int nt, int dm) { return device_sm_count() * (nt == 1 && dm <= 128 ? 2 : 1); }
-static size_t kv_part_floats(int nt, int dm) { return static_cast<size_t>(8 * nt) * (dm + 4); }
+static size_t kv_part_floats(int nt, int dm) { return static_cast<size_t>(8 * nt) * (dm + 4); }   // KvPart::kFloats
 
 // The same for every number of rows: the workspace of a prompt serves the decode steps behind it.
 size_t kv_attention_workspace_bytes(size_t, size_t, size_t, size_t, size_t dim) {
@@ -612,7 +739,7 @@ size_t kv_attention_workspace_bytes(size_t, size_t, size_t, size_t, size_t dim) 
   size_t most = 0;
   for (int nt = 1; nt <= (dm == 256 ? 1 : 2); ++nt) {
     const size_t ctas = static_cast<size_t>(kv_ctas(nt, dm));
-    most = std::max(most, ((ctas * 16 + 255) & ~size_t(255)) + ((ctas * (2 * kKvWarps + 2) * kv_part_floats(nt, dm) * 4 + 255) & ~size_t(255)));
+    most = std::max(most, ((ctas * 16 + 255) & ~size_t(255)) + ((ctas * (kKvWarps + 2) * kv_part_floats(nt, dm) * 4 + 255) & ~size_t(255)));
   }
   return most;
 }
@@ -626,9 +753,9 @@ cudaError_t kv_attention_launch(const AttnArgs& a, const kdnn_b200_kv_cache* c, 
            static_cast<int4*>(ws)};
   auto go = [&](auto scalar) {
     using ST = decltype(scalar);
-    if (dm == 64) return nt == 1 ? launch_kv<ST, 64, 1, 6>(p, ctas, st) : launch_kv<ST, 64, 2, 8>(p, ctas, st);
-    if (dm == 128) return nt == 1 ? launch_kv<ST, 128, 1, 3>(p, ctas, st) : launch_kv<ST, 128, 2, 4>(p, ctas, st);
-    return launch_kv<ST, 256, 1, 2>(p, ctas, st);
+    if (dm == 64) return nt == 1 ? launch_kv_dim<ST, 64, 1, 6>(p, ctas, st) : launch_kv_dim<ST, 64, 2, 8>(p, ctas, st);
+    if (dm == 128) return nt == 1 ? launch_kv_dim<ST, 128, 1, 3>(p, ctas, st) : launch_kv_dim<ST, 128, 2, 4>(p, ctas, st);
+    return launch_kv_dim<ST, 256, 1, 2>(p, ctas, st);
   };
   return a.scalar == KDNN_F32 ? go(float{}) : go(__nv_bfloat16{});
 }
