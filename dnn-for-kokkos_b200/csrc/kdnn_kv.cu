@@ -17,7 +17,6 @@ namespace kdnn {
 // Everything is a prefix sum over the sequences followed by independent entries, so each CTA of a small cluster
 // forms the sums for itself in shared memory and writes its share of the entries; the cluster barrier lies between the
 // last read of lens / state and their new values, which may go to the same arrays.
-constexpr int kPlanThreads = 1024;
 constexpr int kPlanCluster = 8;
 
 struct PlanArgs {
@@ -43,26 +42,26 @@ __device__ __forceinline__ unsigned cluster_size() {
 }
 
 // Exclusive sum over the block's threads of one 64-bit value each; `total` comes back to everybody.
+template <int THREADS>
 __device__ __forceinline__ long long block_exclusive(long long v, long long* warps, long long& total) {
+  constexpr int W = THREADS / 32;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  long long inc = v;
+  auto scan = [&](long long x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += u;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
+    }
+    return x;
+  };
+  const long long inc = scan(v);
   __syncthreads();   // the sums of the call before have been read
   if (lane == 31) warps[w] = inc;
   __syncthreads();
-  long long base = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kPlanThreads / 32; ++i) {
-    const long long s = warps[i];
-    if (i < w) base += s;
-    total += s;
-  }
-  return base + inc - v;
+  const long long all = scan(lane < W ? warps[lane] : 0);
+  total = __shfl_sync(0xffffffffu, all, W - 1);
+  const long long base = __shfl_sync(0xffffffffu, all, w == 0 ? 0 : w - 1);
+  return (w == 0 ? 0 : base) + inc - v;
 }
 
 // Largest b with at[b] <= x, for at[0] = 0 <= x < at[n]
@@ -75,10 +74,11 @@ __device__ __forceinline__ int upper_of(const int* at, int n, int x) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_plan_kernel(PlanArgs a) {
   pdl_chain_entry();
   extern __shared__ int sm[];
-  __shared__ long long s_warps[kPlanThreads / 32];
+  __shared__ long long s_warps[THREADS / 32];
   const int B = a.B, shift = a.shift, page = 1 << shift;
   int* rs   = sm;              // [B + 1] first row of a sequence
   int* tk   = rs + B + 1;      // [B + 1] pages taken before it
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   int* wr   = gv + B + 1;      // [B + 1] page writes before it
   int* len  = wr + B + 1;      // [B] tokens it holds (of an ended one: what it gives back)
   int* stor = len + B;         // [B] fresh tokens that get a slot; -1: ended
-  const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(B, static_cast<int>(threadIdx.x) * per), b1 = min(B, b0 + per);
+  const int per = (B + THREADS - 1) / THREADS, b0 = min(B, static_cast<int>(threadIdx.x) * per), b1 = min(B, b0 + per);
   int head = a.state[0];
   const int avail = max(0, min(a.pages, a.state[1]));
   if (head < 0 || head >= a.pages) head = ((head % a.pages) + a.pages) % a.pages;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     len[b]  = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.cols) * page)));
     n += max(f, 0);
   }
-  long long at = block_exclusive(n, s_warps, all);
+  long long at = block_exclusive<THREADS>(n, s_warps, all);
   for (int b = b0; b < b1; ++b) {
     rs[b] = static_cast<int>(min(at, static_cast<long long>(a.rows)));
     at += max(stor[b], 0);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     need += wants(b);
     back += stor[b] < 0 ? held(b) : 0;
   }
-  long long take = block_exclusive(need, s_warps, total), give = block_exclusive(back, s_warps, total);
+  long long take = block_exclusive<THREADS>(need, s_warps, total), give = block_exclusive<THREADS>(back, s_warps, total);
   const int given = static_cast<int>(min(total, static_cast<long long>(a.pages)));
   long long put = 0, kept = 0;
   for (int b = b0; b < b1; ++b) {
@@ -138,14 +138,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     put += st > 0 ? ((len[b] + st - 1) >> shift) - (len[b] >> shift) + 1 : 0;
   }
   long long stored;
-  block_exclusive(kept, s_warps, stored);
-  long long w0 = block_exclusive(put, s_warps, total);
+  block_exclusive<THREADS>(kept, s_warps, stored);
+  long long w0 = block_exclusive<THREADS>(put, s_warps, total);
   const int touched = static_cast<int>(min(total, static_cast<long long>(a.most)));
   for (int b = b0; b < b1; ++b) {
     wr[b] = static_cast<int>(min(w0, static_cast<long long>(a.most)));
     w0 += stor[b] > 0 ? ((len[b] + stor[b] - 1) >> shift) - (len[b] >> shift) + 1 : 0;
   }
-  if (threadIdx.x == kPlanThreads - 1) {
+  if (threadIdx.x == THREADS - 1) {
     tk[B] = static_cast<int>(min(take, static_cast<long long>(avail)));
     gv[B] = given;
     wr[B] = touched;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     const int h = held(b);
     return j < h ? a.table[static_cast<size_t>(b) * a.ldt + j] : a.ring[ring_at(head, tk[b] + j - h)];
   };
-  const int step = static_cast<int>(cluster_size()) * kPlanThreads, me = static_cast<int>(cluster_rank()) * kPlanThreads + threadIdx.x;
+  const int step = static_cast<int>(cluster_size()) * THREADS, me = static_cast<int>(cluster_rank()) * THREADS + threadIdx.x;
   const int rows = rs[B];
   // four rows per search; a page is looked up where it changes
   const bool wide = (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0;
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   }
   if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
   if (cluster_rank() == 0) {
-    for (int b = threadIdx.x; b < B; b += kPlanThreads) {
+    for (int b = threadIdx.x; b < B; b += THREADS) {
       const bool ended = stor[b] < 0;
       a.row_start[b] = rs[b];
       a.first[b]     = ended ? 0 : len[b];
@@ -224,6 +224,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
   }
 }
 
+template <int THREADS>
+static cudaError_t launch_plan(const PlanArgs& a, unsigned ctas, cudaStream_t st) {
+  static SmemAttrOnce once;
+  const cudaError_t e = set_max_smem_once(once, kv_plan_kernel<THREADS>, (6 * 8192 + 4) * 4);
+  if (e != cudaSuccess) return e;
+  return launch_chained_cluster(kv_plan_kernel<THREADS>, dim3(ctas), dim3(THREADS), (6 * static_cast<size_t>(a.B) + 4) * 4, ctas, st, a);
+}
+
 cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int32_t* state, int32_t* table, size_t ldt, size_t cols,
                            int32_t* ring, size_t pages, size_t B, size_t page, size_t rows, int32_t* row_start, int32_t* first,
                            int32_t* lens_out, int32_t* state_out, int32_t* slots, int32_t* writes, size_t most, cudaStream_t st) {
@@ -232,13 +240,9 @@ cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int3
   PlanArgs a{fresh, lens, state, table, ring, row_start, first, lens_out, state_out, slots, reinterpret_cast<int4*>(writes), ldt,
              static_cast<int>(B), shift, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
              static_cast<int>(most)};
-  const int smem = static_cast<int>((6 * B + 4) * sizeof(int));
-  static SmemAttrOnce once;
-  cudaError_t e = set_max_smem_once(once, kv_plan_kernel, (6 * 8192 + 4) * 4);
-  if (e != cudaSuccess) return e;
-  // one CTA while its threads have a few rows each
-  const unsigned ctas = rows / 4 + most > 2 * kPlanThreads ? kPlanCluster : 1;
-  return launch_chained_cluster(kv_plan_kernel, dim3(ctas), dim3(kPlanThreads), smem, ctas, st, a);
+  // one CTA of 256 threads while each has a few entries, else a cluster of large ones (a decode step of 64 sequences 5.5 us with the
+  // one, 9 with the other; 137 000 rows of 200 sequences: 21 us on the cluster)
+  return rows / 4 + most + B <= 1024 ? launch_plan<256>(a, 1, st) : launch_plan<1024>(a, kPlanCluster, st);
 }
 
 // ---- new rows into the cache ---------------------------------------------------------------------------------
@@ -267,42 +271,64 @@ __device__ __forceinline__ int code_of(float x, float inv) {
   return q != q ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
-// One CTA per (page write, head, key or value).
-template <class XT>
-__global__ void __launch_bounds__(128) kv_append_kernel(AppendArgs a) {
+// T threads per job, a job being (page write, head, key or value): the rows are read once and kept in registers where they fit (8 T pieces
+// of 8 elements), the largest of them gives the page's scale, then they are rounded and written.
+// Bound by memory for prompts; for a decode step by the chain entry -> rows and old scale -> codes.
+template <class XT, int T>
+__global__ void __launch_bounds__(T < 128 ? 128 : T) kv_append_kernel(AppendArgs a, long long jobs) {
   pdl_chain_entry();
-  const int4 w = a.writes[blockIdx.x];
-  const int row0 = w.x, count = w.y, pg = w.z, off = w.w;
+  constexpr int JOBS = T < 128 ? 128 / T : 1;      // jobs of a CTA: a warp each, or the whole CTA for one
+  static_assert(T == 32 || T >= 128, "a job is a warp's or a CTA's");
+  const long long job = static_cast<long long>(blockIdx.x) * JOBS + threadIdx.x / T;
+  if (job >= jobs) return;
+  const unsigned place = static_cast<unsigned>(job >> 1), entry = place / static_cast<unsigned>(a.heads);
+  const int t = threadIdx.x % T, h = static_cast<int>(place - entry * a.heads);
+  const bool z = job & 1;
+  const int4 e = a.writes[entry];
+  const int row0 = e.x, count = e.y, pg = e.z, off = e.w;
   // an entry without rows, or one that does not name a place of the cache
   if (count <= 0 || row0 < 0 || row0 > a.rows - count || pg < 0 || pg >= a.pages || off < 0 || off > a.page - count) return;
-  const int h = blockIdx.y, z = blockIdx.z, D = a.dim;
-  const XT* x = static_cast<const XT*>(a.x[z]) + static_cast<size_t>(row0) * a.ld[z] + static_cast<size_t>(h) * a.hd[z];
-  const size_t ld = a.ld[z];
-  const size_t ph = static_cast<size_t>(pg) * a.heads + h;
-  int8_t* codes = a.codes[z] + ph * a.page * D;
+  const int D = a.dim;
+  const size_t ld = z ? a.ld[1] : a.ld[0], ph = static_cast<size_t>(pg) * a.heads + h;
+  const XT* x = static_cast<const XT*>(z ? a.x[1] : a.x[0]) + static_cast<size_t>(row0) * ld + static_cast<size_t>(h) * (z ? a.hd[1] : a.hd[0]);
+  int8_t* codes = (z ? a.codes[1] : a.codes[0]) + ph * a.page * D;
+  float* scale = (z ? a.scale[1] : a.scale[0]) + ph;
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ld * sizeof(XT))) & 15u) == 0;
   const int per_row = D / 8, work = count * per_row;
-  float amax = 0.0f;
-  for (int i = threadIdx.x; i < work; i += blockDim.x) {
-    float v[8];
-    load8<XT>(x + static_cast<size_t>(i / per_row) * ld, static_cast<size_t>(i % per_row) * 8, vec, v);
+  const float old = off > 0 ? *scale : 0.0f;
+  float v[8][8], amax = 0.0f;
+  auto read = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float m = fabsf(v[k]);
-      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values alone
+      const int i = i0 + t + k * T;
+      if (i < work) load8<XT>(x + static_cast<size_t>(i / per_row) * ld, static_cast<size_t>(i % per_row) * 8, vec, v[k]);
     }
+  };
+  for (int i0 = 0; i0 < work; i0 += 8 * T) {
+    read(i0);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i0 + t + k * T < work) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float m = fabsf(v[k][j]);
+          if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values alone
+        }
+      }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  __shared__ float s_max[4];
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-  const float old = off > 0 ? a.scale[z][ph] : 0.0f;
-  __syncthreads();
-  amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  if (T > 32) {
+    __shared__ float s_max[T / 32];
+    if ((t & 31) == 0) s_max[t >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < T / 32; ++k) amax = fmaxf(amax, s_max[k]);
+  }
   const float s = fmaxf(old, scale_for(amax)), inv = s > 0.0f ? 1.0f / s : 0.0f;
   if (off > 0 && old != s) {   // the page's scale grows: older codes follow
     const float ratio = __fmul_rn(old, inv);
-    for (int i = threadIdx.x; i < off * D / 16; i += blockDim.x) {
+    for (int i = t; i < off * D / 16; i += T) {
       uint4 w = reinterpret_cast<uint4*>(codes)[i];
       uint32_t* u = &w.x;
 #pragma unroll
@@ -316,16 +342,36 @@ __global__ void __launch_bounds__(128) kv_append_kernel(AppendArgs a) {
       reinterpret_cast<uint4*>(codes)[i] = w;
     }
   }
-  int8_t* mine = codes + static_cast<size_t>(off) * D;
-  for (int i = threadIdx.x; i < work; i += blockDim.x) {
-    float v[8];
-    load8<XT>(x + static_cast<size_t>(i / per_row) * ld, static_cast<size_t>(i % per_row) * 8, vec, v);
-    uint32_t r[2] = {0u, 0u};
+  uint2* mine = reinterpret_cast<uint2*>(codes + static_cast<size_t>(off) * D);
+  for (int i0 = 0; i0 < work; i0 += 8 * T) {
+    if (work > 8 * T) read(i0);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) r[k >> 2] |= (static_cast<uint32_t>(code_of(v[k], inv)) & 0xFFu) << (8 * (k & 3));
-    reinterpret_cast<uint2*>(mine)[i] = make_uint2(r[0], r[1]);
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + t + k * T;
+      if (i >= work) break;
+      uint32_t r[2] = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j >> 2] |= (static_cast<uint32_t>(code_of(v[k][j], inv)) & 0xFFu) << (8 * (j & 3));
+      mine[i] = make_uint2(r[0], r[1]);
+    }
   }
-  if (threadIdx.x == 0) a.scale[z][ph] = s;
+  if (t == 0) *scale = s;
+}
+
+template <class XT>
+static cudaError_t launch_append(const AppendArgs& a, size_t most, cudaStream_t st) {
+  const long long jobs = static_cast<long long>(most) * a.heads * 2;
+  // a warp per job where a page gets a few rows, else as many threads as hold a page of rows
+  const int T = a.rows < 8 * static_cast<long long>(most) ? 32 : a.page * a.dim <= 8192 ? 128 : a.page * a.dim <= 16384 ? 256 : 512;
+  const long long ctas = T == 32 ? (jobs + 3) / 4 : jobs;
+  if (ctas > 0x7fffffffLL || jobs > 0x1ffffffffLL) return cudaErrorInvalidConfiguration;
+  const dim3 grid(static_cast<unsigned>(ctas));
+  switch (T) {
+    case 32: return launch_chained(kv_append_kernel<XT, 32>, grid, dim3(128), 0, st, a, jobs);
+    case 128: return launch_chained(kv_append_kernel<XT, 128>, grid, dim3(128), 0, st, a, jobs);
+    case 256: return launch_chained(kv_append_kernel<XT, 256>, grid, dim3(256), 0, st, a, jobs);
+    default: return launch_chained(kv_append_kernel<XT, 512>, grid, dim3(512), 0, st, a, jobs);
+  }
 }
 
 cudaError_t kv_append_launch(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
@@ -333,9 +379,7 @@ cudaError_t kv_append_launch(const void* k, size_t ldk, size_t hdk, const void* 
   AppendArgs a{{k, v}, {ldk, ldv}, {hdk, hdv}, {c->k, c->v}, {c->k_scale, c->v_scale}, reinterpret_cast<const int4*>(writes),
                static_cast<int>(rows), static_cast<int>(c->pages), static_cast<int>(c->kv_heads), static_cast<int>(c->page),
                static_cast<int>(c->dim)};
-  const dim3 grid(static_cast<unsigned>(most), static_cast<unsigned>(c->kv_heads), 2);
-  return scalar == KDNN_F32 ? launch_chained(kv_append_kernel<float>, grid, dim3(128), 0, st, a)
-                            : launch_chained(kv_append_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+  return scalar == KDNN_F32 ? launch_append<float>(a, most, st) : launch_append<__nv_bfloat16>(a, most, st);
 }
 
 }  // namespace kdnn
