@@ -4,8 +4,8 @@
 //
 // prompt_tc_kernel (bf16, heads of up to 128, 16-byte aligned rows): 128 query rows of one kv head, a few tokens times the
 // heads of the group, are the M of a tcgen05 product, so a group shares every key and value that is fetched and a short
-// prompt fills its tile. A CTA owns two such tiles and walks the keys 128 at a time: TMA brings keys and values (two stages
-// each), S = Q K^T lands in TMEM, a warpgroup per tile turns it into weights (a thread owns a row: no shuffles) and
+// prompt fills its tile. A CTA owns two such tiles and walks the keys 128 at a time: TMA brings keys and values (five stages
+// in turn), S = Q K^T lands in TMEM, a warpgroup per tile turns it into weights (a thread owns a row: no shuffles) and
 // writes them back as bf16 over the scores, O += P V accumulates in TMEM. While one tile's scores go through the exponentials,
 // the tensor cores work for the other. The reference m moves, and O is rescaled, only when a score passes it by 2^8.
 // Weights are rounded to bf16 (2^-8 each, averaged over the keys); sums and references are fp32.
@@ -281,14 +281,15 @@ static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
 }
 
 // ---- tcgen05 tiles ----------------------------------------------------------------------------------------------------------
-constexpr int kPtThreads = 384, kPtWarpTma = 8, kPtWarpMma = 9, kPtKeys = 128, kPtStages = 2;
+constexpr int kPtThreads = 384, kPtWarpTma = 8, kPtWarpMma = 9, kPtKeys = 128, kPtStages = 5;
 constexpr uint32_t kPtHalf = 128 * 128;     // 128 rows of 64 channels, 128-byte swizzle
 
 template <int DM>
 struct PtLayout {
   static constexpr uint32_t kOperand = (DM / 64) * kPtHalf;     // 128 rows x DM channels
-  static constexpr uint32_t q = 0, k = q + 2 * kOperand, v = k + kPtStages * kOperand, bar = v + kPtStages * kOperand;
+  static constexpr uint32_t q = 0, kv = q + 2 * kOperand, bar = kv + kPtStages * kOperand;   // kv: keys and values in turn
   static constexpr uint32_t total = bar + 256 + 1024;           // + slack for the 1024-byte alignment of the base
+  static_assert(total <= 232448, "one CTA's shared memory");
 };
 // TMEM columns: scores of the two tiles (the weights take the first half of the same columns), then their sums
 constexpr uint32_t kPtS = 0, kPtO = 256;
@@ -393,17 +394,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
 
   const uint32_t bars = base + L::bar;
   auto q_full  = [&](int x) { return bars + 8u * x; };
-  auto k_full  = [&](int s) { return bars + 16u + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 32u + 8u * s; };
-  auto v_full  = [&](int s) { return bars + 48u + 8u * s; };
-  auto v_empty = [&](int s) { return bars + 64u + 8u * s; };
-  auto s_full  = [&](int x) { return bars + 80u + 8u * x; };
-  auto p_full  = [&](int x) { return bars + 96u + 8u * x; };
-  auto o_full  = [&](int x) { return bars + 112u + 8u * x; };
-  const uint32_t mma_end = bars + 128u;
-  uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 144);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 148);
-  RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 152);   // what the TMA warp armed last
+  auto full    = [&](int s) { return bars + 16u + 8u * s; };
+  auto empty   = [&](int s) { return bars + 56u + 8u * s; };
+  auto s_full  = [&](int x) { return bars + 96u + 8u * x; };
+  auto p_full  = [&](int x) { return bars + 112u + 8u * x; };
+  auto o_full  = [&](int x) { return bars + 128u + 8u * x; };
+  const uint32_t mma_end = bars + 144u;
+  uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 152);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 156);
+  RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 160);   // what the TMA warp armed last
 
   if (warp == kPtWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
@@ -412,13 +411,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full(i), 1);
-      mbar_init(k_full(i), 1);
-      mbar_init(k_empty(i), 1);
-      mbar_init(v_full(i), 1);
-      mbar_init(v_empty(i), 1);
       mbar_init(s_full(i), 1);
       mbar_init(p_full(i), 4);
       mbar_init(o_full(i), 1);
+    }
+    for (int i = 0; i < kPtStages; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), 1);
     }
     mbar_init(mma_end, 1);
     *abort_flag = 0;
@@ -574,29 +573,25 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
       };
       const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128u;
       load(base + L::q, &p.q, g * p.G, it.row0 + t0, q_bytes, q_full(0));
-      armed.arm(4, 0);
-      for (int j = 0; j < steps && ok; ++j) {
-        const int s = j & 1;
-        const uint32_t ph = (j >> 1) & 1;
-        if (!(ok = wait1(k_empty(s), ph ^ 1u))) break;
-        load(base + L::k + s * L::kOperand, &p.k, g, it.row0 + beg + j * kPtKeys, kPtHalf, k_full(s));
-        armed.arm(s, ph);
-        if (j == 0 && n1 > 0) {
+      armed.arm(kPtStages, 0);
+      for (int i = 0, st = 0, ph = 0; i < 2 * steps; ++i) {       // keys 0, values 0, keys 1, ...
+        if (!(ok = wait1(empty(st), ph ^ 1u))) break;
+        load(base + L::kv + st * L::kOperand, i & 1 ? &p.v : &p.k, g, it.row0 + beg + (i >> 1) * kPtKeys, kPtHalf, full(st));
+        armed.arm(st, ph);
+        if (i == 0 && n1 > 0) {
           load(base + L::q + L::kOperand, &p.q, g * p.G, it.row0 + t0 + p.tokens, q_bytes, q_full(1));
-          armed.arm(5, 0);
+          armed.arm(kPtStages + 1, 0);
         }
-        if (!(ok = wait1(v_empty(s), ph ^ 1u))) break;
-        load(base + L::v + s * L::kOperand, &p.v, g, it.row0 + beg + j * kPtKeys, kPtHalf, v_full(s));
-        armed.arm(2 + s, ph);
+        if (++st == kPtStages) { st = 0; ph ^= 1; }
       }
       *ring_end = armed;
     }
     __syncwarp();
   } else if (warp == kPtWarpMma) {
     // ------------------------------------------------------------------ products
-    auto scores = [&](int x, int j) {
+    auto scores = [&](int x, int st) {
       if (pt_elect()) {
-        const uint32_t qa = base + L::q + x * L::kOperand, ka = base + L::k + (j & 1) * L::kOperand;
+        const uint32_t qa = base + L::q + x * L::kOperand, ka = base + L::kv + st * L::kOperand;
 #pragma unroll
         for (int k = 0; k < DM / 16; ++k)
           pt_mma_ss(tmem + kPtS + x * 128, pt_desc_k(qa + (k >> 2) * kPtHalf + (k & 3) * 32), pt_desc_k(ka + (k >> 2) * kPtHalf + (k & 3) * 32),
@@ -605,12 +600,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
       }
       __syncwarp();
     };
-    auto sums = [&](int x, int j, bool last) {
+    auto sums = [&](int x, int st, bool more, bool last) {
       if (pt_elect()) {
-        const uint32_t va = base + L::v + (j & 1) * L::kOperand;
+        const uint32_t va = base + L::kv + st * L::kOperand;
 #pragma unroll
         for (int k = 0; k < kPtKeys / 16; ++k)
-          pt_mma_ts(tmem + kPtO + x * 128, tmem + kPtS + x * 128 + 8 * k, pt_desc_mn(va + k * 2048), pt_idesc(DM, true), j != 0 || k != 0);
+          pt_mma_ts(tmem + kPtO + x * 128, tmem + kPtS + x * 128 + 8 * k, pt_desc_mn(va + k * 2048), pt_idesc(DM, true), more || k != 0);
         if (last) tc_commit(o_full(x));
       }
       __syncwarp();
@@ -619,7 +614,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
       if (pt_elect()) tc_commit(bar);
       __syncwarp();
     };
-    ok = wait(k_full(0), 0) && wait(q_full(0), 0);
+    struct Stage { int at; uint32_t ph; } ks = {0, 0}, vs = {1, 0};
+    auto two_on = [&](Stage& s) {
+      s.at += 2;
+      if (s.at >= kPtStages) { s.at -= kPtStages; s.ph ^= 1u; }
+    };
+    ok = wait(full(0), 0) && wait(q_full(0), 0);
     if (ok) {
       tc_after();
       scores(0, 0);
@@ -627,27 +627,29 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         ok = wait(q_full(1), 0);
         if (ok) scores(1, 0);
       }
-      done(k_empty(0));
+      done(empty(0));
     }
+    two_on(ks);
     for (int j = 0; j < steps && ok; ++j) {
-      const uint32_t ph = (j >> 1) & 1;
-      if (!(ok = wait(v_full(j & 1), ph))) break;
+      if (!(ok = wait(full(vs.at), vs.ph))) break;
       bool keys = false;       // the next step's keys are there
       for (int x = 0; x < 2 && ok; ++x) {
         const int n = x ? n1 : n0;
         if (j >= n) continue;
         if (!(ok = wait(p_full(x), j & 1))) break;
         tc_after();
-        sums(x, j, j + 1 == n);
+        sums(x, vs.at, j > 0, j + 1 == n);
         if (j + 1 < n) {
-          if (!keys && !(ok = wait(k_full((j + 1) & 1), ((j + 1) >> 1) & 1))) break;
+          if (!keys && !(ok = wait(full(ks.at), ks.ph))) break;
           keys = true;
-          scores(x, j + 1);
+          scores(x, ks.at);
         }
       }
       if (!ok) break;
-      done(v_empty(j & 1));
-      if (keys) done(k_empty((j + 1) & 1));
+      done(empty(vs.at));
+      if (keys) done(empty(ks.at));
+      two_on(vs);
+      two_on(ks);
     }
   }
   if (!ok && lane == 0) atomicExch(p.status, KDNN_ERR_DEVICE_WAIT);
@@ -656,8 +658,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   if (*abort_flag) {
     // some role gave up: the copies and products still in flight end (bounded) before the CTA gives its memory back
     if (warp == kPtWarpTma && lane == 0)
-      ring_drain(*ring_end, 6, 1u << 14, [&](int s, uint32_t parity) {
-        return mbar_try_wait(s < 2 ? k_full(s) : s < 4 ? v_full(s - 2) : q_full(s - 4), parity); });
+      ring_drain(*ring_end, kPtStages + 2, 1u << 14, [&](int s, uint32_t parity) {
+        return mbar_try_wait(s < kPtStages ? full(s) : q_full(s - kPtStages), parity); });
     if (warp == kPtWarpMma && pt_elect()) {
       tc_commit(mma_end);
       mbar_wait_bounded(mma_end, 0u, 1u << 16);
