@@ -16,7 +16,7 @@
 //    fp16 exactly (1024 + code + 128 by a byte permutation, minus 1152). k order and channel order are permuted the same way on both sides of a product.
 //  * Weights: 2^(s + log2 b - m), one running reference for the values and one for the sum of weights, so that scales
 //    that lie far apart lose neither. References are whole numbers and move only when a score passes them by 8 (weights
-//    stay below 2^15 in fp16; every rescale is exact).
+//    stay below 2^15 in fp16, and one below 2^-24, 2^-31 of the row's largest at the most, may vanish; every rescale is exact).
 //  * fp32 activations: q and the weights enter as two fp16 parts each (22 bits), and every tile's product is added to the sums
 //    by fp32 additions (the tensor core cuts instead of rounding).
 #include "kdnn_common.cuh"

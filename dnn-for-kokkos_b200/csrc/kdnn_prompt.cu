@@ -281,18 +281,20 @@ static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
 }
 
 // ---- tcgen05 tiles ----------------------------------------------------------------------------------------------------------
-constexpr int kPtThreads = 384, kPtWarpTma = 8, kPtWarpMma = 9, kPtKeys = 128, kPtStages = 5;
+constexpr int kPtKeys = 128;
 constexpr uint32_t kPtHalf = 128 * 128;     // 128 rows of 64 channels, 128-byte swizzle
 
-template <int DM>
+// TILES: query tiles of a CTA. Two share every key and value and keep the tensor cores busy in turn; one is for calls that would leave SMs idle.
+template <int DM, int TILES>
 struct PtLayout {
+  static constexpr int kThreads = 128 * TILES + 128, kWarpTma = 4 * TILES, kWarpMma = kWarpTma + 1, kStages = 5;
+  static constexpr uint32_t kColumns = 256 * TILES;             // TMEM: scores of the tiles (the weights take the first half of the
+  static constexpr uint32_t kO = 128 * TILES;                   // same columns), then their sums
   static constexpr uint32_t kOperand = (DM / 64) * kPtHalf;     // 128 rows x DM channels
-  static constexpr uint32_t q = 0, kv = q + 2 * kOperand, bar = kv + kPtStages * kOperand;   // kv: keys and values in turn
+  static constexpr uint32_t q = 0, kv = q + TILES * kOperand, bar = kv + kStages * kOperand;   // kv: keys and values in turn
   static constexpr uint32_t total = bar + 256 + 1024;           // + slack for the 1024-byte alignment of the base
   static_assert(total <= 232448, "one CTA's shared memory");
 };
-// TMEM columns: scores of the two tiles (the weights take the first half of the same columns), then their sums
-constexpr uint32_t kPtS = 0, kPtO = 256;
 
 struct alignas(64) PromptParams {
   CUtensorMap q, k, v;
@@ -371,25 +373,27 @@ __device__ __forceinline__ uint32_t pt_bf2(float lo, float hi) {
   return r;
 }
 
-template <int DM>
-__global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptParams p) {
-  using L = PtLayout<DM>;
+template <int DM, int TILES>
+__global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const __grid_constant__ PromptParams p) {
+  using L = PtLayout<DM, TILES>;
   extern __shared__ __align__(1024) uint8_t pt_raw[];
   const uint32_t base = (smem_u32(pt_raw) + 1023u) & ~1023u;
   uint8_t* smem = pt_raw + (base - smem_u32(pt_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AttnArgs& a = p.a;
 
+  if (threadIdx.x == 0)
+    for (const CUtensorMap* m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x % a.kv_heads;
   PromptItem it;
-  if (!find_item<kPtThreads>(a, 2 * p.tokens, blockIdx.x / a.kv_heads, it)) return;
+  if (!find_item<L::kThreads>(a, TILES * p.tokens, blockIdx.x / a.kv_heads, it)) return;
   // tokens [t0, t0 + tokens) and [t0 + tokens, ...) of the sequence; keys from `beg` on, 128 at a time
-  const int t0 = it.part * 2 * p.tokens;
+  const int t0 = it.part * TILES * p.tokens;
   const int beg = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
-  const int end0 = min(it.n, t0 + p.tokens), end1 = min(it.n, t0 + 2 * p.tokens);
-  const int n0 = (end0 - beg + kPtKeys - 1) / kPtKeys, n1 = end1 > end0 ? (end1 - beg + kPtKeys - 1) / kPtKeys : 0;
+  const int end0 = min(it.n, t0 + p.tokens), end1 = min(it.n, t0 + TILES * p.tokens);
+  const int n0 = (end0 - beg + kPtKeys - 1) / kPtKeys, n1 = TILES == 2 && end1 > end0 ? (end1 - beg + kPtKeys - 1) / kPtKeys : 0;
   const int steps = max(n0, n1);
 
   const uint32_t bars = base + L::bar;
@@ -404,8 +408,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 156);
   RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 160);   // what the TMA warp armed last
 
-  if (warp == kPtWarpMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+  if (warp == L::kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
       mbar_init(p_full(i), 4);
       mbar_init(o_full(i), 1);
     }
-    for (int i = 0; i < kPtStages; ++i) {
+    for (int i = 0; i < L::kStages; ++i) {
       mbar_init(full(i), 1);
       mbar_init(empty(i), 1);
     }
@@ -428,8 +432,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   tc_before();
   __syncthreads();
   tc_after();
-  constexpr uint32_t tmem = 0;     // all 512 columns are ours: the allocation starts at column 0
-  if (*tmem_slot != tmem) *abort_flag = 1;   // (cannot happen; every wait below then gives up)
+  const uint32_t tmem = *tmem_slot;
 
   // Bounded wait of a whole warp; the vote makes the verdict uniform.
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -442,13 +445,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   };
   bool ok = true;
 
-  // Registers go where the scores are: 2 x 128 threads of 224 and 128 of 40 are 62464 of the 64512 that the launch holds.
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  // Registers go where the scores are: 2 x 128 threads of 224 and 128 of 40 are 62464 of the 64512 that the launch holds. (One tile alone
+  // starts with 255 a thread.)
+  if (warp < L::kWarpTma) {
+    if (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------------ scores -> weights (a thread owns a row)
     const int x = warp >> 2, row = (warp & 3) * 32 + lane, n = x ? n1 : n0;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + kPtS + x * 128, to = tmem + lanes + kPtO + x * 128;
+    const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + L::kO + x * 128;
     if (n > 0) {
       const int t = row / p.G, h = row - t * p.G, first = t0 + x * p.tokens;
       const int last = (x ? end1 : end0) - 1;
@@ -468,12 +472,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         tc_wait_ld();
         const int k0 = beg + j * kPtKeys;
         if (k0 + kPtKeys > in_hi || k0 < in_lo) {
+          // a warp's rows are a few neighbouring tokens: of four blocks of 32 keys, their limits lie in one or two
           const int rh = hi - k0, rl = lo - k0;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
+            if (__any_sync(0xffffffffu, rh < 32 * i + 32 || rl > 32 * i)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * i + e >= rh || 32 * i + e < rl) s[i][e] = -INFINITY;
+              for (int e = 0; e < 32; ++e)
+                if (32 * i + e >= rh || 32 * i + e < rl) s[i][e] = -INFINITY;
+            }
         }
         float top[4];
 #pragma unroll
@@ -552,10 +559,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         }
       }
     }
-  } else {
+  } else if (TILES == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   }
-  if (warp == kPtWarpTma) {
+  if (warp == L::kWarpTma) {
     // ------------------------------------------------------------------ queries, then keys and values
     if (lane == 0) {
       RingArmed armed;
@@ -573,28 +580,28 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
       };
       const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128u;
       load(base + L::q, &p.q, g * p.G, it.row0 + t0, q_bytes, q_full(0));
-      armed.arm(kPtStages, 0);
+      armed.arm(L::kStages, 0);
       for (int i = 0, st = 0, ph = 0; i < 2 * steps; ++i) {       // keys 0, values 0, keys 1, ...
         if (!(ok = wait1(empty(st), ph ^ 1u))) break;
         load(base + L::kv + st * L::kOperand, i & 1 ? &p.v : &p.k, g, it.row0 + beg + (i >> 1) * kPtKeys, kPtHalf, full(st));
         armed.arm(st, ph);
         if (i == 0 && n1 > 0) {
           load(base + L::q + L::kOperand, &p.q, g * p.G, it.row0 + t0 + p.tokens, q_bytes, q_full(1));
-          armed.arm(kPtStages + 1, 0);
+          armed.arm(L::kStages + 1, 0);
         }
-        if (++st == kPtStages) { st = 0; ph ^= 1; }
+        if (++st == L::kStages) { st = 0; ph ^= 1; }
       }
       *ring_end = armed;
     }
     __syncwarp();
-  } else if (warp == kPtWarpMma) {
+  } else if (warp == L::kWarpMma) {
     // ------------------------------------------------------------------ products
     auto scores = [&](int x, int st) {
       if (pt_elect()) {
         const uint32_t qa = base + L::q + x * L::kOperand, ka = base + L::kv + st * L::kOperand;
 #pragma unroll
         for (int k = 0; k < DM / 16; ++k)
-          pt_mma_ss(tmem + kPtS + x * 128, pt_desc_k(qa + (k >> 2) * kPtHalf + (k & 3) * 32), pt_desc_k(ka + (k >> 2) * kPtHalf + (k & 3) * 32),
+          pt_mma_ss(tmem + x * 128, pt_desc_k(qa + (k >> 2) * kPtHalf + (k & 3) * 32), pt_desc_k(ka + (k >> 2) * kPtHalf + (k & 3) * 32),
                     pt_idesc(kPtKeys, false), k != 0);
         tc_commit(s_full(x));
       }
@@ -605,7 +612,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         const uint32_t va = base + L::kv + st * L::kOperand;
 #pragma unroll
         for (int k = 0; k < kPtKeys / 16; ++k)
-          pt_mma_ts(tmem + kPtO + x * 128, tmem + kPtS + x * 128 + 8 * k, pt_desc_mn(va + k * 2048), pt_idesc(DM, true), more || k != 0);
+          pt_mma_ts(tmem + L::kO + x * 128, tmem + x * 128 + 8 * k, pt_desc_mn(va + k * 2048), pt_idesc(DM, true), more || k != 0);
         if (last) tc_commit(o_full(x));
       }
       __syncwarp();
@@ -617,7 +624,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     struct Stage { int at; uint32_t ph; } ks = {0, 0}, vs = {1, 0};
     auto two_on = [&](Stage& s) {
       s.at += 2;
-      if (s.at >= kPtStages) { s.at -= kPtStages; s.ph ^= 1u; }
+      if (s.at >= L::kStages) { s.at -= L::kStages; s.ph ^= 1u; }
     };
     ok = wait(full(0), 0) && wait(q_full(0), 0);
     if (ok) {
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     for (int j = 0; j < steps && ok; ++j) {
       if (!(ok = wait(full(vs.at), vs.ph))) break;
       bool keys = false;       // the next step's keys are there
-      for (int x = 0; x < 2 && ok; ++x) {
+      for (int x = 0; x < TILES && ok; ++x) {
         const int n = x ? n1 : n0;
         if (j >= n) continue;
         if (!(ok = wait(p_full(x), j & 1))) break;
@@ -657,17 +664,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
   __syncthreads();
   if (*abort_flag) {
     // some role gave up: the copies and products still in flight end (bounded) before the CTA gives its memory back
-    if (warp == kPtWarpTma && lane == 0)
-      ring_drain(*ring_end, kPtStages + 2, 1u << 14, [&](int s, uint32_t parity) {
-        return mbar_try_wait(s < kPtStages ? full(s) : q_full(s - kPtStages), parity); });
-    if (warp == kPtWarpMma && pt_elect()) {
+    if (warp == L::kWarpTma && lane == 0)
+      ring_drain(*ring_end, L::kStages + 2, 1u << 14, [&](int s, uint32_t parity) {
+        return mbar_try_wait(s < L::kStages ? full(s) : q_full(s - L::kStages), parity); });
+    if (warp == L::kWarpMma && pt_elect()) {
       tc_commit(mma_end);
       mbar_wait_bounded(mma_end, 0u, 1u << 16);
     }
     __syncthreads();
   }
-  if (warp == kPtWarpMma)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
+  if (warp == L::kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kColumns) : "memory");
 }
 
 static bool encode_heads(CUtensorMap* map, const void* x, size_t ld, size_t hd, int rows, int heads, int dim, int box_heads, int box_rows) {
@@ -681,14 +688,22 @@ static bool encode_heads(CUtensorMap* map, const void* x, size_t ld, size_t hd, 
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DM>
+template <int DM, int TILES>
 static cudaError_t launch_tc(const PromptParams& p, cudaStream_t st) {
+  using L = PtLayout<DM, TILES>;
   static SmemAttrOnce once;
-  const cudaError_t e = set_max_smem_once(once, prompt_tc_kernel<DM>, static_cast<int>(PtLayout<DM>::total));
+  const cudaError_t e = set_max_smem_once(once, prompt_tc_kernel<DM, TILES>, static_cast<int>(L::total));
   if (e != cudaSuccess) return e;
-  const long long parts = std::min<long long>(p.a.rows, p.a.rows / (2 * p.tokens) + p.a.seqs), ctas = parts * p.a.kv_heads;
+  const long long parts = std::min<long long>(p.a.rows, p.a.rows / (TILES * p.tokens) + p.a.seqs), ctas = parts * p.a.kv_heads;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  return launch_chained(prompt_tc_kernel<DM>, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads), PtLayout<DM>::total, st, p);
+  return launch_chained(prompt_tc_kernel<DM, TILES>, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::total, st, p);
+}
+// One tile per CTA while all of them find an SM of their own (a prompt of 77 tokens, 32 / 8 heads: 7.6 us against 9.6), else two (with one,
+// 8192 tokens took 605 us against 500).
+template <int DM>
+static cudaError_t launch_tiles_tc(const PromptParams& p, cudaStream_t st) {
+  const long long tiles = static_cast<long long>(std::min(p.a.rows, p.a.rows / p.tokens + p.a.seqs)) * p.a.kv_heads;
+  return tiles <= device_sm_count() ? launch_tc<DM, 1>(p, st) : launch_tc<DM, 2>(p, st);
 }
 
 cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
@@ -709,7 +724,7 @@ cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
     if (encode_heads(&p.q, a.q, a.ldq, a.hdq, a.rows, a.heads, a.dim, G, p.tokens) &&
         encode_heads(&p.k, a.k, a.ldk, a.hdk, a.rows, a.kv_heads, a.dim, 1, kPtKeys) &&
         encode_heads(&p.v, a.v, a.ldv, a.hdv, a.rows, a.kv_heads, a.dim, 1, kPtKeys))
-      return a.dim <= 64 ? launch_tc<64>(p, st) : launch_tc<128>(p, st);
+      return a.dim <= 64 ? launch_tiles_tc<64>(p, st) : launch_tiles_tc<128>(p, st);
   }
   return launch_tiles<__nv_bfloat16>(a, st);
 }

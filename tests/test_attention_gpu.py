@@ -7,7 +7,9 @@ Tolerances count roundings. For one output o = sum_j p_j v_j with A = sum_j p_j 
   by the rounding of a weight that enters a matrix product, and by (keys) roundings of fp32 sums, which meet A;
   the result by half a step of its type.
 bf16 operands are exact in a product; a weight is rounded to bf16 (2^-8) for packed bf16 prompts and to fp16 (2^-11) over the
-cache; fp32 operands and weights over the cache are two fp16 parts (2^-22)."""
+cache; fp32 operands and weights over the cache are two fp16 parts (2^-22). Over the cache a weight is also off by half of fp16's
+smallest step, 2^-25, where the largest weight of its row is at least 2^6 (it is 2^(7 + s - m), and m, a whole number, is at most one
+above the largest score): by 2^-31 of the sum, which meets the sum of |v_j|."""
 import math
 import random
 
@@ -279,7 +281,7 @@ def test_append_leaves_what_no_entry_names(kd):
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 def attend(q, k, v, keep, scale):
-    """One sequence in float64: q [n, H, D], k, v [T, KV, D], keep [n, T] -> (o, A, bound of |score|, keys)."""
+    """One sequence in float64: q [n, H, D], k, v [T, KV, D], keep [n, T] -> (o, A, bound of |score|, keys, sum of |v|)."""
     n, H, D = q.shape
     G = H // k.shape[1]
     q, k, v = q.double(), k.double().repeat_interleave(G, 1), v.double().repeat_interleave(G, 1)
@@ -292,12 +294,14 @@ def attend(q, k, v, keep, scale):
     big = big.masked_fill(~keep, 0.0).amax(-1) if keep.shape[1] else torch.zeros(H, n, dtype=torch.float64, device=q.device)
     # a masked value does not enter, whatever it is
     v = torch.where((p == 0).all(1).T[..., None], 0.0, v)
-    return torch.einsum("hnt,thd->nhd", p, v), torch.einsum("hnt,thd->nhd", p, v.abs()), big.T, keep.sum(-1)
+    # what weights that vanish may take away: the sum of |v| over the kept keys
+    rest = torch.einsum("nt,thd->nhd", keep.double(), v.abs())
+    return torch.einsum("hnt,thd->nhd", p, v), torch.einsum("hnt,thd->nhd", p, v.abs()), big.T, keep.sum(-1), rest
 
 
-def held_to(got, want, A, big, keys, dtype, operand, weight, D):
+def held_to(got, want, A, big, keys, dtype, operand, weight, D, floor=0.0):
     es = big * (2 * operand + D * F32 + 8 * F32)
-    bound = A * (2 * es + 2 * weight + (8 + keys[:, None].double().sqrt() * 4) * F32)[..., None] + want.abs() * OUT[dtype] * 1.01 + 1e-30
+    bound = A * (2 * es + 2 * weight + (8 + keys[:, None].double().sqrt() * 4) * F32)[..., None] + want.abs() * OUT[dtype] * 1.01 + floor + 1e-30
     off = (got.double() - want).abs()
     assert torch.isfinite(got).all()
     assert (off <= bound).all(), f"{(off / bound).max().item():.3g} of the bound"
@@ -337,9 +341,9 @@ def check_cache(plan, table, cache, q, out, lens, fresh, window, dtype, scale=No
         keep = (j <= pos) & good.repeat_interleave(page)[None, :T]
         if window:
             keep &= j > pos - window
-        o, A, big, keys = attend(q[rs[b]:rs[b + 1]], k, v, keep, dim ** -0.5 if scale is None else scale)
+        o, A, big, keys, rest = attend(q[rs[b]:rs[b + 1]], k, v, keep, dim ** -0.5 if scale is None else scale)
         operand, weight = (0.0, 2.0 ** -11) if dtype == torch.bfloat16 else (2.0 ** -22, 2.0 ** -22)
-        held_to(out[rs[b]:rs[b + 1]], o, A, big, keys, dtype, operand, weight, dim)
+        held_to(out[rs[b]:rs[b + 1]], o, A, big, keys, dtype, operand, weight, dim, floor=rest * 2.0 ** -31)
     assert (out[rs[-1]:] == 777.0).all()
 
 
@@ -453,7 +457,7 @@ def check_prompt(q, k, v, out, starts, window, dtype, scale=None):
                 keep &= j > i - window
             rows = slice(lo + r0, lo + min(n, r0 + step))
             keys = slice(lo, lo + j.shape[1])
-            o, A, big, count = attend(q[rows], k[keys], v[keys], keep, D ** -0.5 if scale is None else scale)
+            o, A, big, count, _ = attend(q[rows], k[keys], v[keys], keep, D ** -0.5 if scale is None else scale)
             weight = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
             held_to(out[rows], o, A, big, count, dtype, 0.0, weight, D)
 
@@ -503,10 +507,27 @@ def test_prompt_attention_rows_outside_and_fused_projection(kd, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("dim", [64, 128, 256])
-def test_prompt_attention_masked_places_hold_anything(kd, dtype, dim):
+@pytest.mark.parametrize("heads,kv,dim,lens,window", [
+    (32, 8, 128, [1300, 0, 77], 0), (32, 4, 64, [900, 333], 200), (16, 16, 128, [700, 129, 700], 0), (24, 8, 96, [800, 50], 0),
+    (64, 8, 128, [257, 256, 255, 1], 64), (20, 4, 40, [1500], 0),
+])
+def test_prompt_attention_of_many_rows(kd, dtype, heads, kv, dim, lens, window):
+    """Enough work for every SM: two query tiles per CTA."""
+    prompt_case(kd, dtype, heads, kv, dim, lens, window, seed=dim + heads, lead=2, pad=3)
+
+
+def test_prompt_attention_of_many_sequences(kd):
+    rng = random.Random(4)
+    lens = [rng.choice([0, 1, 2, 17, 40]) for _ in range(700)]
+    prompt_case(kd, torch.bfloat16, 8, 2, 64, lens, 0)
+    prompt_case(kd, torch.float32, 4, 1, 64, lens, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 8), (256, 8), (64, 64), (128, 64)])
+def test_prompt_attention_masked_places_hold_anything(kd, dtype, dim, heads):
     """Infinities and NaN in later rows, in other sequences and behind the last one do not reach the rows before them."""
-    q, k, v, out, starts = prompt_case(kd, dtype, 8, 2, dim, [100, 150, 40], 0, pad=30)
+    q, k, v, out, starts = prompt_case(kd, dtype, heads, heads // 4, dim, [100, 150, 40], 0, pad=30)
     want, k0, v0 = out.clone(), k.clone(), v.clone()
     bad = (float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min)
     for i in range(30):
@@ -516,12 +537,12 @@ def test_prompt_attention_masked_places_hold_anything(kd, dtype, dim):
     assert (out[starts[-1]:] == 777.0).all()
     got = out[60:100].float()
     assert torch.isnan(got[:, :4]).all()                              # a NaN key
-    assert torch.isnan(got[:, 4:, 5]).all() and (torch.isinf(got[1:, :4, 7]) | torch.isnan(got[1:, :4, 7])).all()
+    assert torch.isnan(got[:, 4:8, 5]).all() and (torch.isinf(got[1:, :4, 7]) | torch.isnan(got[1:, :4, 7])).all()
     # everything else is what it was without them: held to the clean values' result (a row beside such a place may be summed
     # in another order, so by the bound and not by its bits)
     reached = torch.zeros_like(out, dtype=torch.bool)
     reached[60:100, :4] = True
-    reached[60:100, 4:, 5] = True
+    reached[60:100, 4:8, 5] = True
     reached[249] = True
     check_prompt(q, k0, v0, torch.where(reached, want, out), starts, 0, dtype)
 
