@@ -99,6 +99,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int 
 }
 
 // ---- fp32 tiles -----------------------------------------------------------------------------------------------------------
+// Bound by FMA issue and by what feeds it from shared memory (eight 16-byte loads per 32 FMA pairs). The next tile of keys and values is
+// fetched into registers while this one is used, where they hold it (DM <= 128).
 constexpr int kTileM = 64, kTileN = 64;
 template <int DM>
 struct TileShape {
@@ -106,13 +108,11 @@ struct TileShape {
   static constexpr int kFloats = (kTileM + kTileN) * kPitch + kTileN * DM + kTileM * kPPitch;
 };
 
-__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) { return ffma2(a, b, c); }
-
 // Four channels of a row; channels behind D are 0.
 template <class ST>
-__device__ __forceinline__ float4 four_of(const ST* p, int d, int D, bool vec) {
+__device__ __forceinline__ float4 four_of(const ST* p, int d, int D) {
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (d < D) load4<ST>(p, static_cast<size_t>(d), vec, v);
+  if (d < D) load4<ST>(p, static_cast<size_t>(d), (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(ST) - 1)) == 0, v);
   return make_float4(v[0], v[1], v[2], v[3]);
 }
 
@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
   pdl_chain_entry();
   extern __shared__ __align__(16) float sf[];
   float *sq = sf, *sk = sq + kTileM * S::kPitch, *sv = sk + kTileN * S::kPitch, *sp = sv + kTileN * DM;
+  __shared__ unsigned long long s_bad;
   const int g = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads, D = a.dim;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   PromptItem it;
@@ -134,12 +135,13 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
   const int tok0 = it.part * tokens;
   const int fn = min(min(tokens, it.n - tok0) * G - f0, kTileM);
   if (fn <= 0) return;
+  if (threadIdx.x == 0) s_bad = 0ull;
 
   auto q_at = [&](int r) { return f0 + min(r, fn - 1); };
   for (int i = threadIdx.x; i < kTileM * (DM / 4); i += 256) {
     const int r = i / (DM / 4), d = (i % (DM / 4)) * 4, f = q_at(r), t = f / G;
     const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldq + static_cast<size_t>(g * G + f - t * G) * a.hdq;
-    *reinterpret_cast<float4*>(sq + r * S::kPitch + d) = four_of<ST>(q, d, D, (reinterpret_cast<uintptr_t>(q) & (4 * sizeof(ST) - 1)) == 0);
+    *reinterpret_cast<float4*>(sq + r * S::kPitch + d) = four_of<ST>(q, d, D);
   }
   int hi[4], lo[4];
   float m[4], l[4];
@@ -157,25 +159,40 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
   const int p_lo = tok0 + f0 / G, p_hi = tok0 + (f0 + fn - 1) / G;
   const int k_beg = a.window > 0 ? max(0, p_lo - a.window + 1) : 0, k_end = p_hi + 1;
   const float c = a.scale * 1.4426950408889634f;
+  // this thread's share of a tile: rows r0 + RP i, four channels at d0
+  constexpr int RP = 1024 / DM, EACH = kTileN / RP;
+  constexpr bool AHEAD = DM <= 128;
+  const int r0 = threadIdx.x / (DM / 4), d0 = (threadIdx.x % (DM / 4)) * 4;
+  const ST* kbase = static_cast<const ST*>(a.k) + static_cast<size_t>(it.row0) * a.ldk + static_cast<size_t>(g) * a.hdk;
+  const ST* vbase = static_cast<const ST*>(a.v) + static_cast<size_t>(it.row0) * a.ldv + static_cast<size_t>(g) * a.hdv;
+  float4 kn[AHEAD ? EACH : 1], vn[AHEAD ? EACH : 1];
+  auto get = [&](const ST* x, size_t ld, int row) {      // a key behind the last one is 0
+    return row < k_end ? four_of<ST>(x + static_cast<size_t>(row) * ld, d0, D) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+  auto ahead = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < (AHEAD ? EACH : 0); ++i) {
+      kn[i] = get(kbase, a.ldk, k0 + r0 + RP * i);
+      vn[i] = get(vbase, a.ldv, k0 + r0 + RP * i);
+    }
+  };
+  ahead(k_beg);
   for (int k0 = k_beg; k0 < k_end; k0 += kTileN) {
     __syncthreads();      // the tile before has been used
-    bool odd = false;     // a value that is not finite
-    for (int i = threadIdx.x; i < kTileN * (DM / 4); i += 256) {
-      const int r = i / (DM / 4), d = (i % (DM / 4)) * 4;
-      float4 kv = make_float4(0, 0, 0, 0), vv = kv;
-      if (k0 + r < k_end) {
-        const size_t row = static_cast<size_t>(it.row0) + k0 + r;
-        const ST* k = static_cast<const ST*>(a.k) + row * a.ldk + static_cast<size_t>(g) * a.hdk;
-        const ST* v = static_cast<const ST*>(a.v) + row * a.ldv + static_cast<size_t>(g) * a.hdv;
-        kv = four_of<ST>(k, d, D, (reinterpret_cast<uintptr_t>(k) & (4 * sizeof(ST) - 1)) == 0);
-        vv = four_of<ST>(v, d, D, (reinterpret_cast<uintptr_t>(v) & (4 * sizeof(ST) - 1)) == 0);
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        *reinterpret_cast<float4*>(sk + (r0 + RP * i) * S::kPitch + d0) = kn[AHEAD ? i : 0];
+        *reinterpret_cast<float4*>(sv + (r0 + RP * i) * DM + d0) = vn[AHEAD ? i : 0];
       }
-      *reinterpret_cast<float4*>(sk + r * S::kPitch + d) = kv;
-      *reinterpret_cast<float4*>(sv + r * DM + d) = vv;
-      odd |= !(fmaxf(fmaxf(fabsf(vv.x), fabsf(vv.y)), fmaxf(fabsf(vv.z), fabsf(vv.w))) < INFINITY) || vv.x != vv.x || vv.y != vv.y ||
-             vv.z != vv.z || vv.w != vv.w;
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < EACH; ++i) {
+        *reinterpret_cast<float4*>(sk + (r0 + RP * i) * S::kPitch + d0) = get(kbase, a.ldk, k0 + r0 + RP * i);
+        *reinterpret_cast<float4*>(sv + (r0 + RP * i) * DM + d0) = get(vbase, a.ldv, k0 + r0 + RP * i);
+      }
     }
-    odd = __syncthreads_or(odd);
+    __syncthreads();
+    if (k0 + kTileN < k_end) ahead(k0 + kTileN);
     float2 s2[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -192,8 +209,8 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s2[r][i] = fma_pair(make_float2(qv[r].x, qv[r].y), make_float2(kv[i].x, kv[i].y), s2[r][i]);
-          s2[r][i] = fma_pair(make_float2(qv[r].z, qv[r].w), make_float2(kv[i].z, kv[i].w), s2[r][i]);
+          s2[r][i] = ffma2(make_float2(qv[r].x, qv[r].y), make_float2(kv[i].x, kv[i].y), s2[r][i]);
+          s2[r][i] = ffma2(make_float2(qv[r].z, qv[r].w), make_float2(kv[i].z, kv[i].w), s2[r][i]);
         }
     }
 #pragma unroll
@@ -221,7 +238,8 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
         sp[(4 * ty + r) * S::kPPitch + tx + 16 * i] = p;
       }
     }
-    __syncthreads();
+    __syncwarp();         // a warp's rows are its own: nobody else reads them
+#pragma unroll 4
     for (int k = 0; k < kTileN; k += 4) {
       float pv[4][4];
 #pragma unroll
@@ -233,15 +251,14 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
           const float4 v = *reinterpret_cast<const float4*>(sv + (k + e) * DM + 64 * i + 4 * tx);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float4 u = v;
-            if (odd && pv[r][e] == 0.0f) u = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a masked value does not enter
             const float2 pp = make_float2(pv[r][e], pv[r][e]);
-            const float2 x = fma_pair(pp, make_float2(u.x, u.y), make_float2(o[r][i].x, o[r][i].y));
-            const float2 y = fma_pair(pp, make_float2(u.z, u.w), make_float2(o[r][i].z, o[r][i].w));
+            const float2 x = ffma2(pp, make_float2(v.x, v.y), make_float2(o[r][i].x, o[r][i].y));
+            const float2 y = ffma2(pp, make_float2(v.z, v.w), make_float2(o[r][i].z, o[r][i].w));
             o[r][i] = make_float4(x.x, x.y, y.x, y.y);
           }
         }
     }
+    __syncwarp();
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -254,11 +271,21 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
     for (int i = 0; i < DM / 64; ++i) {
       const int d = 64 * i + 4 * tx;
       if (d >= D) continue;
-      store_scalar(out + d, o[r][i].x / l[r]);
-      store_scalar(out + d + 1, o[r][i].y / l[r]);
-      store_scalar(out + d + 2, o[r][i].z / l[r]);
-      store_scalar(out + d + 3, o[r][i].w / l[r]);
+      const float y[4] = {o[r][i].x / l[r], o[r][i].y / l[r], o[r][i].z / l[r], o[r][i].w / l[r]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        store_scalar(out + d + e, y[e]);
+        if (!(fabsf(y[e]) < INFINITY)) atomicOr(&s_bad, 1ull << (4 * ty + r));
+      }
     }
+  }
+  // rows that did not come out finite: a warp each
+  __syncthreads();
+  const unsigned long long bad = s_bad;
+  for (int r = threadIdx.x >> 5; r < kTileM && bad != 0ull; r += 8) {
+    if (!((bad >> r) & 1ull)) continue;
+    const int f = f0 + r, t = f / G;
+    row_alone<ST>(a, it.row0, tok0 + t, g * G + f - t * G);
   }
 }
 
