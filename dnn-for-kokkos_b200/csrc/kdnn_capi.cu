@@ -656,6 +656,7 @@ int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void
     return fail(KDNN_ERR_INVALID, "prompt_attention: dimension mismatch");
   if (rows > static_cast<size_t>(INT_MAX) / heads || seqs > 8192) return fail(KDNN_ERR_INVALID, "prompt_attention: too many rows or sequences");
   if (!q || !k || !v || !row_start || !out) return fail(KDNN_ERR_INVALID, "prompt_attention: null argument");
+  if (out == q || out == k || out == v) return fail(KDNN_ERR_INVALID, "prompt_attention: out must not overlap q, k or v");
   kdnn::AttnArgs a{};
   a.q = q; a.ldq = ldq; a.hdq = hdq; a.k = k; a.ldk = ldk; a.hdk = hdk; a.v = v; a.ldv = ldv; a.hdv = hdv;
   a.out = out; a.ldo = ldo; a.hdo = hdo; a.scalar = scalar;

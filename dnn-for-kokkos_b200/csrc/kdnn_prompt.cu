@@ -9,8 +9,8 @@
 // writes them back as bf16 over the scores, O += P V accumulates in TMEM. While one tile's scores go through the exponentials,
 // the tensor cores work for the other. The reference m moves, and O is rescaled, only when a score passes it by 2^8.
 // Weights are rounded to bf16 (2^-8 each, averaged over the keys); sums and references are fp32.
-// A product reads masked values with weight 0, so infinities or NaN there would reach the sum: a row that does not come out finite is
-// computed again from its own keys alone.
+// A product reads masked values with weight 0, so infinities or NaN there would reach the sum: a row that does not come out finite, although
+// its scores are, is computed again from its own keys alone where one of the masked values beside it is not finite.
 //
 // prompt_tile_kernel (fp32, larger heads, any alignment): 64 query rows against 64 keys in shared memory, fp32 FMA pairs.
 #include "kdnn_tc.cuh"
@@ -51,6 +51,18 @@ __device__ __forceinline__ void row_alone(const AttnArgs& a, int row0, int i, in
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (e * 32 + lane < D) store_scalar(out + e * 32 + lane, o[e] / l);
+}
+
+// Whether a value of kv head g in the rows [from, to) of a sequence (they may run into the next ones) is not finite. One warp.
+template <class ST>
+__device__ __forceinline__ bool odd_values(const AttnArgs& a, int row0, int from, int to, int g) {
+  const int lane = threadIdx.x & 31;
+  bool odd = false;
+  for (int j = max(from, 0); j < min(to, a.rows - row0); ++j) {
+    const ST* v = static_cast<const ST*>(a.v) + static_cast<size_t>(row0 + j) * a.ldv + static_cast<size_t>(g) * a.hdv;
+    for (int d = lane; d < a.dim; d += 32) odd |= !(fabsf(to_f32(v[d])) < INFINITY);
+  }
+  return __any_sync(0xffffffffu, odd);
 }
 
 // ---- which sequence and which part of it a CTA works on ---------------------------------------------------------------
@@ -275,14 +287,17 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         store_scalar(out + d + e, y[e]);
-        if (!(fabsf(y[e]) < INFINITY)) atomicOr(&s_bad, 1ull << (4 * ty + r));
+        if (!(fabsf(y[e]) < INFINITY) && fabsf(l[r]) < INFINITY) atomicOr(&s_bad, 1ull << (4 * ty + r));
       }
     }
   }
-  // rows that did not come out finite: a warp each
+  // rows that did not come out finite though their scores are: a warp each, where a value that some of the tile's rows do not see is not
   __syncthreads();
   const unsigned long long bad = s_bad;
-  for (int r = threadIdx.x >> 5; r < kTileM && bad != 0ull; r += 8) {
+  if (bad == 0ull || (!odd_values<ST>(a, it.row0, p_lo + 1, k_end, g) &&
+                      !odd_values<ST>(a, it.row0, k_beg, a.window > 0 ? p_hi - a.window + 1 : 0, g)))
+    return;
+  for (int r = threadIdx.x >> 5; r < kTileM; r += 8) {
     if (!((bad >> r) & 1ull)) continue;
     const int f = f0 + r, t = f / G;
     row_alone<ST>(a, it.row0, tok0 + t, g * G + f - t * G);
@@ -327,7 +342,7 @@ struct alignas(64) PromptParams {
   CUtensorMap q, k, v;
   AttnArgs a;
   int G, tokens;     // heads of a group; tokens of a tile (tokens * G <= 128 rows)
-  float c;           // scale * log2(e), not negative
+  float c;           // scale * log2(e), positive
   int* status;
 };
 
@@ -578,8 +593,13 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
             if (live && 32 * i + e < a.dim) *reinterpret_cast<uint4*>(out + 32 * i + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        // rows that did not come out finite, one after the other
-        for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo != 0; todo &= todo - 1) {
+        // rows that did not come out finite though their scores are: the masked keys of the tiles they met are (pos, ...) and [beg, lo)
+        unsigned todo = __ballot_sync(0xffffffffu, bad && live && fabsf(l) < INFINITY);
+        if (todo != 0) {
+          const int low = __reduce_min_sync(0xffffffffu, pos), high = __reduce_max_sync(0xffffffffu, lo);
+          if (!odd_values<__nv_bfloat16>(a, it.row0, low + 1, beg + n * kPtKeys, g) && !odd_values<__nv_bfloat16>(a, it.row0, beg, high, g)) todo = 0;
+        }
+        for (; todo != 0; todo &= todo - 1) {
           const int src = __ffs(todo) - 1;
           __syncwarp();
           row_alone<__nv_bfloat16>(a, it.row0, __shfl_sync(0xffffffffu, pos, src), g * p.G + __shfl_sync(0xffffffffu, h, src));
@@ -739,8 +759,8 @@ cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
   const size_t pitches = a.ldq | a.hdq | a.ldk | a.hdk | a.ldv | a.hdv | a.ldo | a.hdo;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                           reinterpret_cast<uintptr_t>(a.out);
-  // TMA wants 16-byte pitches; a reference for the largest score needs a scale that is not negative
-  if (a.dim <= 128 && G <= 128 && pitches % 8 == 0 && bases % 16 == 0 && a.scale >= 0.0f && a.scale < 1e30f) {
+  // TMA wants 16-byte pitches; the kernel's maximum is one of products, so the scale has to be positive
+  if (a.dim <= 128 && G <= 128 && pitches % 8 == 0 && bases % 16 == 0 && a.scale > 1e-30f && a.scale < 1e30f) {
     PromptParams p;
     p.a = a;
     p.G = G;

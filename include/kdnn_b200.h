@@ -456,7 +456,8 @@ size_t kdnn_b200_kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t h
  * kv_heads): 0 <= j < lens[b], j <= pos, and j > pos - window where window > 0; pos = first[b] + r - row_start[b]. A row
  * with no such token gives 0. The new rows themselves are read from the cache: append before this call. Tokens on a page
  * that the table does not hold (a number outside [0, pages), or beyond table_cols) are left out.
- * q, out [rows][heads][dim] Scalar with row and head pitches; out may be q. heads is a multiple of kv_heads. */
+ * q, out [rows][heads][dim] Scalar with row and head pitches; out may be q. heads is a multiple of kv_heads. Calls that overlap need
+ * workspaces of their own. A weight below 2^-31 of its row's largest may count as 0. seqs <= 8192. */
 int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, size_t rows, size_t heads, const int32_t* row_start,
                            const int32_t* first, const int32_t* lens, size_t seqs, const int32_t* table, size_t ldt,
                            size_t table_cols, const kdnn_b200_kv_cache* cache, void* out, size_t ldo, size_t hdo, float scale,
@@ -466,7 +467,8 @@ int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, si
  * the last `window` of them). q, out [rows][heads][dim], k, v [rows][kv_heads][dim] Scalar with row and head pitches in
  * elements; dim a multiple of 8 up to 256. Values in masked places (later rows, other sequences) do not reach the result,
  * infinities and NaN included. Rows outside [row_start[0], row_start[seqs]) are left as they were. out must not overlap
- * k or v. */
+ * q, k or v. bf16 heads of up to 128 elements whose rows are 16-byte aligned run on tcgen05 tiles (weights rounded to bf16, sums fp32), the
+ * rest on fp32 tiles. seqs <= 8192. */
 int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void* k, size_t ldk, size_t hdk, const void* v,
                                size_t ldv, size_t hdv, int scalar, size_t rows, size_t heads, size_t kv_heads, size_t dim,
                                const int32_t* row_start, size_t seqs, void* out, size_t ldo, size_t hdo, float scale,

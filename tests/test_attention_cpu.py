@@ -76,13 +76,13 @@ def test_cache_attention_refusals(kd):
 
 def test_prompt_attention_refusals(kd):
     ok = dict(q=P, ldq=512, hdq=128, k=P, ldk=256, hdk=128, v=P, ldv=256, hdv=128, scalar=1, rows=4, heads=4, kv_heads=2, dim=128,
-              row_start=P, seqs=2, out=P, ldo=512, hdo=128, scale=0.1, window=0)
+              row_start=P, seqs=2, out=2 * P, ldo=512, hdo=128, scale=0.1, window=0)
 
     def call(**kw):
         return kd.lib.kdnn_b200_prompt_attention(*dict(ok, **kw).values(), None)
 
     for kw in (dict(scalar=-1), dict(dim=0), dict(dim=12), dict(dim=264), dict(kv_heads=0), dict(kv_heads=3), dict(ldq=500), dict(hdk=64),
-               dict(ldv=200), dict(hdo=120), dict(seqs=8193), dict(rows=2 ** 30),
+               dict(ldv=200), dict(hdo=120), dict(seqs=8193), dict(rows=2 ** 30), dict(out=P),
                *({n: None} for n in ("q", "k", "v", "row_start", "out"))):
         assert call(**kw) == kd.KDNN_ERR_INVALID, kw
         assert "prompt_attention" in kd.last_error()

@@ -616,3 +616,38 @@ def test_two_streams_at_once(kd):
     torch.cuda.synchronize()
     for w, c in zip(want, cases):
         assert torch.equal(c[4], w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prompt_attention_of_values_that_are_not_finite(kd, dtype):
+    """What is not finite and seen stays so, in every later row and no other channel."""
+    q, k, v, out, starts = prompt_case(kd, dtype, 32, 8, 128, [700, 60], 0)
+    want = out.clone()
+    v[3, 2, 9], v[130, 0, 0], k[400, 5, 1] = float("nan"), float("inf"), float("nan")
+    kd.prompt_attention(q, k, v, i32(starts), out)
+    assert torch.isnan(out[3:700, 8:12, 9]).all() and torch.isnan(out[400:700, 20:24]).all()
+    assert not torch.isfinite(out[130:700, 0:4, 0]).any()
+    reached = torch.zeros_like(out, dtype=torch.bool)
+    reached[3:700, 8:12, 9], reached[400:700, 20:24], reached[130:700, 0:4, 0] = True, True, True
+    k[400, 5, 1] = v[3, 2, 9] = v[130, 0, 0] = 0.0
+    close = (out.float() - want.float()).abs() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-5) * (want.float().abs() + 1)
+    assert (close | reached).all()
+
+
+def test_calls_on_a_stream_of_their_own(kd):
+    """The launch goes to the current stream: work queued there before it is seen, and nothing waits for the default stream."""
+    stream = torch.cuda.Stream()
+    q, k, v, want, starts = prompt_case(kd, torch.bfloat16, 8, 2, 64, [100, 30], 0)
+    rs = i32(starts)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        q2 = torch.zeros_like(q)
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(5):
+            big = big @ big * 1e-3
+        q2.copy_(q)
+        out = torch.empty_like(q)
+        kd.prompt_attention(q2, k, v, rs, out)
+        got = out.clone()
+    stream.synchronize()
+    assert torch.equal(got, want)
