@@ -647,8 +647,10 @@ def run_ours(args):
 
 def run_case(args):
     """One small workload on one GPU, a few hundred MB on the device and a handful of launches: the thing to
-    put under a profiler (`--case gemv_q4k | gemv_q6k | gemv_q80 | gemv_q4k_pair | moe_block | moe_block_tcgen05`).
-    gemv_*: 13 cold copies of the matrix, three passes over them. moe_block*: one 128-expert / top-8 / hidden
+    put under a profiler (`--case gemv_q4k | gemv_q6k | gemv_q80 | gemv_q4k_pair | moe_block | moe_block_tcgen05 |
+    attention_cache | attention_prompt`). attention_cache: one decode step of 64 sequences of up to 8192 cached tokens (32 / 4 heads of
+    128, pages of 64), plan, write and attention, three times. attention_prompt: 4096 packed rows of two sequences, 32 / 8 heads
+    of 128, three times. gemv_*: 13 cold copies of the matrix, three passes over them. moe_block*: one 128-expert / top-8 / hidden
     2048 / FFN 768 block on 256 tokens, three calls."""
     import torch
     import __graft_entry__ as ge
@@ -674,6 +676,9 @@ def run_case(args):
         print(json.dumps({"case": args.case, "launches": 3 * (len(ws) // 2 if args.case == "gemv_q4k_pair" else len(ws)), "matrix_bytes": int(host.nbytes),
                           "device_status": kd.device_status()}))
         return
+    if args.case.startswith("attention"):
+        run_attention_case(args.case, kd, dev)
+        return
     ms = ge._load_module("_kd_moe_bench", os.path.join(ge.PKG_DIR, "moe_stack.py"))
     kd.tile_kind(2 if args.case.endswith("tcgen05") else 3)
     cfg = ms.StackConfig(layers=1)
@@ -683,6 +688,49 @@ def run_case(args):
         stack.forward(h0)
     torch.cuda.synchronize()
     print(json.dumps({"case": args.case, "block_calls": 3, "device_status": kd.device_status()}))
+
+
+def run_attention_case(name, kd, dev):
+    import torch
+    g = torch.Generator(device=dev).manual_seed(SEED)
+
+    def rows_of(n, heads):
+        return torch.randn(n, heads, 128, device=dev, generator=g).to(torch.bfloat16)
+
+    if name == "attention_prompt":
+        q, k, v = rows_of(4096, 32), rows_of(4096, 8), rows_of(4096, 8)
+        starts = torch.tensor([0, 3000, 4096], dtype=torch.int32, device=dev)
+        out = torch.empty_like(q)
+        for _ in range(3):
+            kd.prompt_attention(q, k, v, starts, out)
+        torch.cuda.synchronize()
+        print(json.dumps({"case": name, "calls": 3, "device_status": kd.device_status()}))
+        return
+    seqs, page, heads, kv = 64, 64, 32, 4
+    lens = torch.randint(1024, 8192, (seqs,), device=dev, generator=g, dtype=torch.int32)
+    held = (lens + page - 1) // page
+    pages, cols = int(held.sum()) + 2 * seqs, int(held.max()) + 2
+    j = torch.arange(cols, device=dev, dtype=torch.int32)
+    table = torch.where(j < held[:, None], (torch.cumsum(held, 0, dtype=torch.int32) - held)[:, None] + j, -1).contiguous()
+    used = int(held.sum())
+    ring = torch.arange(pages, device=dev, dtype=torch.int32).roll(-used).contiguous()
+    state = torch.tensor([0, pages - used, 0, 0], dtype=torch.int32, device=dev)
+    cache = kd.KvCache.empty(pages, kv, page, 128, dev)
+    for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        codes.copy_(torch.randint(-127, 128, codes.shape, device=dev, generator=g, dtype=torch.int8))
+        scale.fill_(2.0 ** -7)
+    plan = kd.KvPlan.empty(seqs, seqs, page, dev)
+    plan.lens, plan.state = lens, state
+    fresh = torch.ones(seqs, dtype=torch.int32, device=dev)
+    q, kn, vn = rows_of(seqs, heads), rows_of(seqs, kv), rows_of(seqs, kv)
+    out = torch.empty_like(q)
+    ws = torch.empty(kd.kv_attention_workspace_bytes(seqs, seqs, heads, kv, 128), dtype=torch.uint8, device=dev)
+    for _ in range(3):
+        kd.kv_plan(fresh, lens, table, ring, state, plan)
+        kd.kv_append(kn, vn, plan, cache)
+        kd.kv_attention(q, plan, table, cache, out, ws)
+    torch.cuda.synchronize()
+    print(json.dumps({"case": name, "steps": 3, "cached_bytes": int(lens.sum()) * 2 * kv * 128, "device_status": kd.device_status()}))
 
 
 def main():
@@ -695,7 +743,8 @@ def main():
     ap.add_argument("--check-multi-rank", action="store_true",
                     help="only compare the expert-parallel MoE stack with a one-rank run and print the errors")
     ap.add_argument("--case", default=None,
-                    choices=["gemv_q4k", "gemv_q4k_pair", "gemv_q6k", "gemv_q80", "moe_block", "moe_block_tcgen05"],
+                    choices=["gemv_q4k", "gemv_q4k_pair", "gemv_q6k", "gemv_q80", "moe_block", "moe_block_tcgen05", "attention_cache",
+                             "attention_prompt"],
                     help="run one small workload only (for a profiler) instead of the benchmark")
     args = ap.parse_args()
     if args.case:

@@ -303,6 +303,74 @@ void moe_ffn(const ExecSpace& space, const XView& X, const Table& gate, const Ta
 }
 
 
+// Attention over packed rows (kdnn_b200.h, "attention"). Row views are [rows, heads, dim] with unit stride in the last dimension;
+// plan: any struct with the views row_start, first, lens, state, slots, writes (int32; writes [entries, 4]) and `page`; cache: one
+// with k, v (int8 [pages, kv_heads, page, dim]) and k_scale, v_scale (float [pages, kv_heads]). In the reference: src/KokkosDNN_Attention.hpp,
+// src/KokkosDNN_KVCache.hpp.
+template <class Cache>
+kdnn_b200_kv_cache kv_cache_of(const Cache& c) {
+  return kdnn_b200_kv_cache{reinterpret_cast<int8_t*>(c.k.data()), reinterpret_cast<int8_t*>(c.v.data()), c.k_scale.data(),
+                            c.v_scale.data(), c.k.extent(0), c.k.extent(1), c.k.extent(2), c.k.extent(3)};
+}
+
+template <class ExecSpace, class FView, class LView, class TView, class RView, class SView, class Plan>
+void kv_plan(const ExecSpace& space, const FView& fresh, const LView& lens, const TView& table, const RView& ring, const SView& state,
+             const Plan& plan) {
+  const std::size_t seqs = fresh.extent(0);
+  if (lens.extent(0) != seqs || table.extent(0) != seqs || plan.row_start.extent(0) != seqs + 1 || plan.first.extent(0) != seqs ||
+      plan.lens.extent(0) != seqs || state.extent(0) != 4 || plan.state.extent(0) != 4 || plan.writes.extent(1) != 4)
+    throw std::invalid_argument("kv_plan: dimension mismatch");
+  throw_on_error(kdnn_b200_kv_plan(fresh.data(), lens.data(), seqs, plan.page, plan.slots.extent(0), table.data(), table.stride(0),
+                                   table.extent(1), ring.data(), ring.extent(0), state.data(), plan.row_start.data(),
+                                   plan.first.data(), plan.lens.data(), plan.state.data(), plan.slots.data(), plan.writes.data(),
+                                   plan.writes.extent(0), StreamOf<ExecSpace>::get(space)),
+                 "kv_plan");
+}
+
+template <class ExecSpace, class XView, class Plan, class Cache>
+void kv_append(const ExecSpace& space, const XView& k, const XView& v, const Plan& plan, const Cache& cache) {
+  using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(k.data())>::type>::type;
+  const kdnn_b200_kv_cache c = kv_cache_of(cache);
+  if (k.extent(0) != plan.slots.extent(0) || v.extent(0) != k.extent(0) || k.extent(1) != c.kv_heads || v.extent(1) != c.kv_heads ||
+      k.extent(2) != c.dim || v.extent(2) != c.dim || c.page != static_cast<std::size_t>(plan.page))
+    throw std::invalid_argument("kv_append: dimension mismatch");
+  throw_on_error(kdnn_b200_kv_append(k.data(), k.stride(0), k.stride(1), v.data(), v.stride(0), v.stride(1), scalar_tag<Scalar>(),
+                                     k.extent(0), plan.writes.data(), plan.writes.extent(0), &c, StreamOf<ExecSpace>::get(space)),
+                 "kv_append");
+}
+
+template <class ExecSpace, class XView, class Plan, class TView, class Cache, class WsView>
+void kv_attention(const ExecSpace& space, const XView& q, const Plan& plan, const TView& table, const Cache& cache, const XView& out,
+                  float scale, std::size_t window, const WsView& workspace) {
+  using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(q.data())>::type>::type;
+  const kdnn_b200_kv_cache c = kv_cache_of(cache);
+  const std::size_t seqs = plan.first.extent(0);
+  if (out.extent(0) != q.extent(0) || out.extent(1) != q.extent(1) || q.extent(2) != c.dim || out.extent(2) != c.dim ||
+      plan.row_start.extent(0) != seqs + 1 || plan.lens.extent(0) != seqs || table.extent(0) != seqs ||
+      c.page != static_cast<std::size_t>(plan.page))
+    throw std::invalid_argument("kv_attention: dimension mismatch");
+  throw_on_error(kdnn_b200_kv_attention(q.data(), q.stride(0), q.stride(1), scalar_tag<Scalar>(), q.extent(0), q.extent(1),
+                                        plan.row_start.data(), plan.first.data(), plan.lens.data(), seqs, table.data(),
+                                        table.stride(0), table.extent(1), &c, out.data(), out.stride(0), out.stride(1), scale, window,
+                                        workspace.data(), workspace.extent(0), StreamOf<ExecSpace>::get(space)),
+                 "kv_attention");
+}
+
+template <class ExecSpace, class XView, class RView>
+void prompt_attention(const ExecSpace& space, const XView& q, const XView& k, const XView& v, const RView& row_start, const XView& out,
+                      float scale, std::size_t window) {
+  using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(q.data())>::type>::type;
+  if (k.extent(0) != q.extent(0) || v.extent(0) != q.extent(0) || out.extent(0) != q.extent(0) || out.extent(1) != q.extent(1) ||
+      v.extent(1) != k.extent(1) || k.extent(2) != q.extent(2) || v.extent(2) != q.extent(2) || out.extent(2) != q.extent(2) ||
+      row_start.extent(0) == 0)
+    throw std::invalid_argument("prompt_attention: dimension mismatch");
+  throw_on_error(kdnn_b200_prompt_attention(q.data(), q.stride(0), q.stride(1), k.data(), k.stride(0), k.stride(1), v.data(),
+                                            v.stride(0), v.stride(1), scalar_tag<Scalar>(), q.extent(0), q.extent(1), k.extent(1),
+                                            q.extent(2), row_start.data(), row_start.extent(0) - 1, out.data(), out.stride(0),
+                                            out.stride(1), scale, window, StreamOf<ExecSpace>::get(space)),
+                 "prompt_attention");
+}
+
 // The model's MoE block for a chunk of tokens in ONE call (router product, moe_route / moe_route_sigmoid, experts,
 // residual add, the next block's un-scaled RMS norm; models/lfm2_5/KokkosDNN_LFM25Model.hpp:770-816):
 //   h_out = h + MoE(x),  x_next = rmsnorm_noscale(h_out).
