@@ -28,7 +28,7 @@ struct PlanArgs {
 };
 
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -240,8 +240,8 @@ cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int3
   PlanArgs a{fresh, lens, state, table, ring, row_start, first, lens_out, state_out, slots, reinterpret_cast<int4*>(writes), ldt,
              static_cast<int>(B), shift, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
              static_cast<int>(most)};
-  // one CTA of 256 threads while each has a few entries, else a cluster of large ones (a decode step of 64 sequences 5.5 us with the
-  // one, 9 with the other; 137 000 rows of 200 sequences: 21 us on the cluster)
+  // one CTA of 256 threads while each has a few entries (a decode step of 64 sequences: 6.7 us, 12.6 with 1024 threads), else a cluster of large
+  // ones (134 000 rows of 200 sequences: 16 us)
   return rows / 4 + most + B <= 1024 ? launch_plan<256>(a, 1, st) : launch_plan<1024>(a, kPlanCluster, st);
 }
 

@@ -381,6 +381,13 @@ def test_cache_attention_many_sequences(kd):
     cache_case(kd, torch.bfloat16, 8, 4, 64, 16, [rng.choice([0, 1, 1, 2]) for _ in lens], lens, 0)
 
 
+def test_cache_attention_thousands_of_sequences(kd):
+    """More than a CTA keeps the lengths of."""
+    rng = random.Random(9)
+    lens = [rng.randrange(0, 40) for _ in range(3000)]
+    cache_case(kd, torch.bfloat16, 2, 1, 64, 16, [rng.choice([0, 1, 1]) for _ in lens], lens, 0)
+
+
 def test_cache_attention_peaked_and_far_scales(kd):
     """Scores that leave one token, pages whose scales lie far apart, a page of zeros."""
     for dtype in (torch.bfloat16, torch.float32):
