@@ -274,18 +274,30 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
   __shared__ int4 s_seg[2 * kKvWarps];              // pieces of this CTA's warps: {b, unit, 1, in the queue's place}; z 0: none
   line_of<NT>(a, G, p.pshift, at, known);
   auto work_of = [&](int b) { return seq_work<NT>(a, G, b < kKnown ? known[b] : seq_lengths(a, p.pshift, b)); };
-  const long long total = at[a.seqs];
-  // every warp takes a run while there are kLeast tiles for it; with fewer, the first CTAs' warps do. (Several runs per warp, the later
+  // Runs: every warp takes one while there are kLeast tiles for it; with fewer, the first CTAs' warps do. (Several runs per warp, the later
   // ones by CTAs that follow on the SMs that finish early, cost more than the SMs' different bandwidths: 122 us against 98 for
   // three contexts of 131071.)
-  const int workers = static_cast<int>(max(1LL, min(static_cast<long long>(kKvWarps) * gridDim.x, (total + kLeast - 1) / kLeast)));
-  const long long share = total < 0x7fffffffLL ? static_cast<int>(total) / workers : total / workers;
-  const int longer = static_cast<int>(total - share * workers);      // the first ones take one tile more
-  auto start_of = [&](int i) { return i >= workers ? total : share * i + min(i, longer); };
-  const int my0 = blockIdx.x * kKvWarps;
-  const long long cta0 = start_of(my0), cta1 = start_of(my0 + kKvWarps);
-  long long pos = start_of(my0 + w);
-  const long long end = start_of(my0 + w + 1), begin = pos;
+  struct Runs {
+    long long total, share;
+    int workers, longer;      // the first `longer` ones take one tile more
+    __device__ __forceinline__ Runs(long long all) : total(all) {
+      workers = static_cast<int>(max(1LL, min(static_cast<long long>(kKvWarps) * gridDim.x, (all + kLeast - 1) / kLeast)));
+      share   = all < 0x7fffffffLL ? static_cast<int>(all) / workers : all / workers;
+      longer  = static_cast<int>(all - share * workers);
+    }
+    __device__ __forceinline__ long long start(int i) const { return i >= workers ? total : share * i + min(i, longer); }
+    __device__ __forceinline__ int of(long long x) const {      // the run that tile x lies in
+      const long long cut = (share + 1) * longer;
+      return static_cast<int>(x < cut ? x / (share + 1) : longer + (x - cut) / share);
+    }
+  };
+  long long pos, end;
+  {
+    const Runs runs(at[a.seqs]);
+    pos = runs.start(blockIdx.x * kKvWarps + w);
+    end = runs.start(blockIdx.x * kKvWarps + w + 1);
+  }
+  bool first_piece = true;      // of the run
   if (lane < 2) s_seg[2 * w + lane] = make_int4(0, 0, 0, 0);
 
   const uint32_t my_ring = ring + static_cast<uint32_t>(w) * STAGES * Sh::kStageBytes;
@@ -318,7 +330,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
     const int unit = in_b < 0x7fffffffLL ? static_cast<int>(in_b) / s.line : static_cast<int>(in_b / s.line);
     const int place = static_cast<int>(in_b - static_cast<long long>(unit) * s.line);
     const int run = static_cast<int>(min(static_cast<long long>(s.line - place), end - pos));
-    const bool first_of_run = pos == begin;
+    const bool first_of_run = first_piece;
+    first_piece = false;
     pos += run;
     in_b += run;
     const int tile = max(place - kSwitch, 0), take = place + run - kSwitch - tile;
@@ -405,7 +418,6 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
     // ---- query rows as fp16 fragments
     uint32_t qf[PARTS][NT][KS][2];
     float rsc[NT][2], bias[NT][2];      // factor of a row's scores; 128 sum(q) in their units: products are with code + 128
-    int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[DM / 4];
@@ -449,9 +461,6 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
       for (int h = 0; h < 2; ++h) {
         rsc[nt][h]  = __shfl_sync(0xffffffffu, r, (2 * c + h) * 4) * 16777216.0f;
         bias[nt][h] = __shfl_sync(0xffffffffu, sum, (2 * c + h) * 4) * -0x1p-17f;
-        const int fr = f0 + min(nt * 8 + 2 * c + h, fn - 1), ps = s.first + fr / G;
-        hi[nt][h] = min(s.len, ps + 1);
-        lo[nt][h] = a.window > 0 ? ps - a.window + 1 : 0;
         mz[nt][h] = ml[nt][h] = kLowest;
         l[nt][h] = 0.0f;
       }
@@ -529,9 +538,11 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = t0 + (e & 2);
-            if (tok >= hi[nt][e & 1] || tok < lo[nt][e & 1] || gone) sc[nt][e] = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            const int ps = s.first + (f0 + min(nt * 8 + 2 * c + h, fn - 1)) / G;
+            const int hi = gone ? 0 : min(s.len, ps + 1), lo = a.window > 0 ? ps - a.window + 1 : 0;
+            if (t0 >= hi || t0 < lo) sc[nt][h] = -INFINITY;
+            if (t0 + 2 >= hi || t0 + 2 < lo) sc[nt][2 + h] = -INFINITY;
           }
       }
 #pragma unroll
@@ -665,6 +676,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
 
   // ---- pieces of one unit that this CTA's warps hold are joined, an m tile per warp
   __syncthreads();
+  const Runs runs(at[a.seqs]);
+  const long long cta0 = runs.start(blockIdx.x * kKvWarps), cta1 = runs.start((blockIdx.x + 1) * kKvWarps);
   const float* mine = p.parts + static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) * Pt::kFloats;
   const float* queues = reinterpret_cast<const float*>(sm + (ring - smem_u32(sm)));
   int4 goes_on = make_int4(0, 0, 0, 0);
@@ -684,9 +697,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
         return s_seg[at].w ? queues + (at >> 1) * (STAGES * Sh::kStageBytes / 4) : mine + (at >> 1) * Pt::kFloats; },
                             u0 >= cta0 && u1 <= cta1 ? nullptr : to);
     if (u0 >= cta0 && u1 > cta1) {      // how many CTAs further its last tile is
-      const long long x = u1 - 1, cut = (share + 1) * longer;
-      const int in = static_cast<int>(x < cut ? x / (share + 1) : longer + (x - cut) / share);
-      goes_on = make_int4(in / kKvWarps - static_cast<int>(blockIdx.x), ub, uu, 0);
+      goes_on = make_int4(runs.of(u1 - 1) / kKvWarps - static_cast<int>(blockIdx.x), ub, uu, 0);
     }
     __syncwarp();
   }
