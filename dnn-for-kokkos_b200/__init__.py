@@ -776,21 +776,21 @@ def moe_block_routing(workspace: torch.Tensor, tokens_local: int, world: int, to
 _I32 = torch.int32
 
 
-def _here(what: str, *tensors: torch.Tensor) -> None:
-    """Every tensor on the current CUDA device, where the launch goes."""
-    dev = tensors[0].get_device()
+def _stream_of(what: str, *tensors: torch.Tensor) -> int:
+    """The current stream, where the launch goes; every tensor has to live on its device."""
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else -2
     for t in tensors:
-        if t.get_device() != dev or dev < 0:
+        if t.get_device() != dev:
             raise ValueError(f"{what}: tensors must live on the current CUDA device")
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors must live on the current CUDA device")
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _packed(what: str, name: str, t: torch.Tensor, rows: int, heads: int, dim: int):
+def _packed(what: str, name: str, t: torch.Tensor, shape):
     """(row pitch, head pitch) of a [rows, heads, dim] tensor whose heads are contiguous rows."""
-    if t.shape != (rows, heads, dim):
-        raise ValueError(f"{what}: {name} must be [rows, heads, dim] = {(rows, heads, dim)}, got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} must be [rows, heads, dim] = {tuple(shape)}, got {tuple(t.shape)}")
     ld, hd, one = t.stride()
+    rows, heads, dim = shape
     if one != 1 and dim > 1:
         raise ValueError(f"{what}: {name} must have unit stride in its last dimension")
     if heads == 1:
@@ -897,26 +897,27 @@ def kv_plan(fresh: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, ring: 
         if t.dtype != _I32 or not t.is_contiguous():
             raise ValueError("kv_plan: fresh, lens, ring and state must be contiguous int32")
     ldt = _table("kv_plan", table, seqs)
-    _here("kv_plan", fresh, lens, table, ring, state, plan.first)
+    stream = _stream_of("kv_plan", fresh, lens, table, ring, state, plan.first)
     rc = lib.kdnn_b200_kv_plan(fresh.data_ptr(), lens.data_ptr(), seqs, plan.page, plan.rows, table.data_ptr(), ldt, table.shape[1],
                                ring.data_ptr(), ring.shape[0], state.data_ptr(), plan.row_start.data_ptr(), plan.first.data_ptr(),
                                plan.lens.data_ptr(), plan.state.data_ptr(), plan.slots.data_ptr(), plan.writes.data_ptr(),
-                               plan.writes.shape[0], _stream())
+                               plan.writes.shape[0], stream)
     _check(rc, "kv_plan")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, plan: KvPlan, cache: KvCache) -> None:
     """The step's keys and values [rows, kv_heads, dim] into the places that ``plan`` gives them (see kdnn_b200_kv_append)."""
     rows, heads, dim = plan.rows, cache.kv_heads, cache.dim
-    ldk, hdk = _packed("kv_append", "k", k, rows, heads, dim)
-    ldv, hdv = _packed("kv_append", "v", v, rows, heads, dim)
+    shape = (rows, heads, dim)
+    ldk, hdk = _packed("kv_append", "k", k, shape)
+    ldv, hdv = _packed("kv_append", "v", v, shape)
     if k.dtype != v.dtype:
         raise ValueError("kv_append: k and v must share one Scalar")
     if cache.page != plan.page:
         raise ValueError("kv_append: cache and plan have pages of different size")
-    _here("kv_append", k, v, plan.first, cache.k)
+    stream = _stream_of("kv_append", k, v, plan.first, cache.k)
     _check(lib.kdnn_b200_kv_append(k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(k), rows, plan.writes.data_ptr(),
-                                   plan.writes.shape[0], C.byref(cache.c_struct()), _stream()), "kv_append")
+                                   plan.writes.shape[0], C.byref(cache.c_struct()), stream), "kv_append")
 
 
 def kv_attention_workspace_bytes(rows: int, seqs: int, heads: int, kv_heads: int, dim: int) -> int:
@@ -930,18 +931,19 @@ def kv_attention(q: torch.Tensor, plan: KvPlan, table: torch.Tensor, cache: KvCa
     if q.dim() != 3:
         raise ValueError("kv_attention: q must be [rows, heads, dim]")
     rows, heads, dim, seqs = plan.rows, q.shape[1], cache.dim, plan.seqs
-    ldq, hdq = _packed("kv_attention", "q", q, rows, heads, dim)
-    ldo, hdo = _packed("kv_attention", "out", out, rows, heads, dim)
+    shape = (rows, heads, dim)
+    ldq, hdq = _packed("kv_attention", "q", q, shape)
+    ldo, hdo = _packed("kv_attention", "out", out, shape)
     if out.dtype != q.dtype:
         raise ValueError("kv_attention: q and out must share one Scalar")
     ldt = _table("kv_attention", table, seqs)
     if cache.page != plan.page or window < 0:
         raise ValueError("kv_attention: cache and plan have pages of different size, or the window is negative")
-    _here("kv_attention", q, out, table, workspace, plan.first, cache.k)
+    stream = _stream_of("kv_attention", q, out, table, workspace, plan.first, cache.k)
     _check(lib.kdnn_b200_kv_attention(q.data_ptr(), ldq, hdq, _scalar(q), rows, heads, plan.row_start.data_ptr(), plan.first.data_ptr(),
                                       plan.lens.data_ptr(), seqs, table.data_ptr(), ldt, table.shape[1], C.byref(cache.c_struct()),
                                       out.data_ptr(), ldo, hdo, dim ** -0.5 if scale is None else float(scale), window,
-                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()), "kv_attention")
+                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream), "kv_attention")
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_start: torch.Tensor, out: torch.Tensor,
@@ -953,18 +955,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_star
         raise ValueError(f"{what}: q and k must be [rows, heads, dim]")
     rows, heads, dim = q.shape
     kv_heads, dtype = k.shape[1], q.dtype
-    ldq, hdq = _packed(what, "q", q, rows, heads, dim)
-    ldk, hdk = _packed(what, "k", k, rows, kv_heads, dim)
-    ldv, hdv = _packed(what, "v", v, rows, kv_heads, dim)
-    ldo, hdo = _packed(what, "out", out, rows, heads, dim)
+    of_q, of_kv = q.shape, (rows, kv_heads, dim)
+    ldq, hdq = _packed(what, "q", q, of_q)
+    ldk, hdk = _packed(what, "k", k, of_kv)
+    ldv, hdv = _packed(what, "v", v, of_kv)
+    ldo, hdo = _packed(what, "out", out, of_q)
     if k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
         raise ValueError(f"{what}: q, k, v and out must share one Scalar")
     if row_start.dim() != 1 or row_start.shape[0] < 1 or row_start.dtype != _I32 or not row_start.is_contiguous() or window < 0:
         raise ValueError(f"{what}: row_start must be contiguous int32 [seqs + 1] and the window not negative")
-    _here(what, q, k, v, out, row_start)
+    stream = _stream_of(what, q, k, v, out, row_start)
     _check(lib.kdnn_b200_prompt_attention(q.data_ptr(), ldq, hdq, k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv, _scalar(q), rows,
                                           heads, kv_heads, dim, row_start.data_ptr(), row_start.shape[0] - 1, out.data_ptr(), ldo, hdo,
-                                          dim ** -0.5 if scale is None else float(scale), window, _stream()), what)
+                                          dim ** -0.5 if scale is None else float(scale), window, stream), what)
 
 
 def read_probe(buf: torch.Tensor, sink: torch.Tensor) -> None:
