@@ -111,14 +111,18 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int 
 }
 
 // ---- fp32 tiles -----------------------------------------------------------------------------------------------------------
-// Bound by FMA issue and by what feeds it from shared memory (eight 16-byte loads per 32 FMA pairs). The next tile of keys and values is
-// fetched into registers while this one is used, where they hold it (DM <= 128).
+// Bound by FMA issue and by what feeds it from shared memory (eight 16-byte loads per 32 FMA pairs). fp32 keys and values of the next tile
+// come by cp.async while this one is used, where two tiles fit (DM <= 128).
 constexpr int kTileM = 64, kTileN = 64;
-template <int DM>
+template <class ST, int DM>
 struct TileShape {
-  static constexpr int kPitch = DM + 4, kPPitch = kTileN + 4;
-  static constexpr int kFloats = (kTileM + kTileN) * kPitch + kTileN * DM + kTileM * kPPitch;
+  static constexpr bool kAhead = sizeof(ST) == 4 && DM <= 128;
+  static constexpr int kPitch = DM + 4, kPPitch = kTileN + 4, kKv = kTileN * (kPitch + DM);   // a tile of keys, then of values
+  static constexpr int kFloats = kTileM * kPitch + (kAhead ? 2 : 1) * kKv + kTileM * kPPitch;
 };
+__device__ __forceinline__ void tile_fetch(float* dst, const void* src, bool there) {   // 16 bytes, zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 
 // Four channels of a row; channels behind D are 0.
 template <class ST>
@@ -131,10 +135,10 @@ __device__ __forceinline__ float4 four_of(const ST* p, int d, int D) {
 // Thread (ty, tx) of 16 x 16 holds rows 4 ty .. + 3 against keys tx + 16 i, and channels 4 tx + 64 i of the result.
 template <class ST, int DM>
 __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(AttnArgs a) {
-  using S = TileShape<DM>;
+  using S = TileShape<ST, DM>;
   pdl_chain_entry();
   extern __shared__ __align__(16) float sf[];
-  float *sq = sf, *sk = sq + kTileM * S::kPitch, *sv = sk + kTileN * S::kPitch, *sp = sv + kTileN * DM;
+  float *sq = sf, *kv = sq + kTileM * S::kPitch, *sp = kv + (S::kAhead ? 2 : 1) * S::kKv;
   __shared__ unsigned long long s_bad;
   const int g = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads, D = a.dim;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -173,38 +177,53 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
   const float c = a.scale * 1.4426950408889634f;
   // this thread's share of a tile: rows r0 + RP i, four channels at d0
   constexpr int RP = 1024 / DM, EACH = kTileN / RP;
-  constexpr bool AHEAD = DM <= 128;
   const int r0 = threadIdx.x / (DM / 4), d0 = (threadIdx.x % (DM / 4)) * 4;
   const ST* kbase = static_cast<const ST*>(a.k) + static_cast<size_t>(it.row0) * a.ldk + static_cast<size_t>(g) * a.hdk;
   const ST* vbase = static_cast<const ST*>(a.v) + static_cast<size_t>(it.row0) * a.ldv + static_cast<size_t>(g) * a.hdv;
-  float4 kn[AHEAD ? EACH : 1], vn[AHEAD ? EACH : 1];
-  auto get = [&](const ST* x, size_t ld, int row) {      // a key behind the last one is 0
-    return row < k_end ? four_of<ST>(x + static_cast<size_t>(row) * ld, d0, D) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
-  auto ahead = [&](int k0) {
-#pragma unroll
-    for (int i = 0; i < (AHEAD ? EACH : 0); ++i) {
-      kn[i] = get(kbase, a.ldk, k0 + r0 + RP * i);
-      vn[i] = get(vbase, a.ldv, k0 + r0 + RP * i);
-    }
-  };
-  ahead(k_beg);
-  for (int k0 = k_beg; k0 < k_end; k0 += kTileN) {
-    __syncthreads();      // the tile before has been used
-    if (AHEAD) {
+  // rows on 16 bytes: fetched asynchronously; else loaded one by one
+  const bool async = S::kAhead && ((reinterpret_cast<uintptr_t>(kbase) | reinterpret_cast<uintptr_t>(vbase)) & 15u) == 0 && ((a.ldk | a.ldv) & 3u) == 0;
+  auto request = [&](int k0, int buf) {      // a key behind the last one is 0
+    float *tk = kv + buf * S::kKv + r0 * S::kPitch + d0, *tv = kv + buf * S::kKv + kTileN * S::kPitch + r0 * DM + d0;
+    if (async) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        *reinterpret_cast<float4*>(sk + (r0 + RP * i) * S::kPitch + d0) = kn[AHEAD ? i : 0];
-        *reinterpret_cast<float4*>(sv + (r0 + RP * i) * DM + d0) = vn[AHEAD ? i : 0];
+        const int row = k0 + r0 + RP * i;
+        const bool there = row < k_end && d0 < D;
+        const size_t at = there ? row : 0;
+        tile_fetch(tk + RP * i * S::kPitch, kbase + at * a.ldk + (there ? d0 : 0), there);
+        tile_fetch(tv + RP * i * DM, vbase + at * a.ldv + (there ? d0 : 0), there);
       }
     } else {
 #pragma unroll 4
       for (int i = 0; i < EACH; ++i) {
-        *reinterpret_cast<float4*>(sk + (r0 + RP * i) * S::kPitch + d0) = get(kbase, a.ldk, k0 + r0 + RP * i);
-        *reinterpret_cast<float4*>(sv + (r0 + RP * i) * DM + d0) = get(vbase, a.ldv, k0 + r0 + RP * i);
+        const int row = k0 + r0 + RP * i;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+        if (row < k_end) {
+          x = four_of<ST>(kbase + static_cast<size_t>(row) * a.ldk, d0, D);
+          y = four_of<ST>(vbase + static_cast<size_t>(row) * a.ldv, d0, D);
+        }
+        *reinterpret_cast<float4*>(tk + RP * i * S::kPitch) = x;
+        *reinterpret_cast<float4*>(tv + RP * i * DM) = y;
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (S::kAhead) request(k_beg, 0);
+  for (int k0 = k_beg, buf = 0; k0 < k_end; k0 += kTileN) {
+    __syncthreads();      // the tile before has been used
+    if (S::kAhead) {
+      if (k0 + kTileN < k_end) {
+        request(k0 + kTileN, buf ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+    } else {
+      request(k0, 0);
+    }
     __syncthreads();
-    if (k0 + kTileN < k_end) ahead(k0 + kTileN);
+    const float *sk = kv + buf * S::kKv, *sv = sk + kTileN * S::kPitch;
+    if (S::kAhead) buf ^= 1;
     float2 s2[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -306,7 +325,7 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
 
 template <class ST, int DM>
 static cudaError_t launch_tile(const AttnArgs& a, cudaStream_t st) {
-  const int smem = TileShape<DM>::kFloats * 4, G = a.heads / a.kv_heads;
+  const int smem = TileShape<ST, DM>::kFloats * 4, G = a.heads / a.kv_heads;
   static SmemAttrOnce once;
   const cudaError_t e = set_max_smem_once(once, prompt_tile_kernel<ST, DM>, smem);
   if (e != cudaSuccess) return e;
