@@ -443,20 +443,6 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AttnArgs& a = p.a;
 
-  if (threadIdx.x == 0)
-    for (const CUtensorMap* m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
-  pdl_launch_dependents();
-  pdl_wait();
-  const int g = blockIdx.x % a.kv_heads;
-  PromptItem it;
-  if (!find_item<L::kThreads>(a, TILES * p.tokens, blockIdx.x / a.kv_heads, it)) return;
-  // tokens [t0, t0 + tokens) and [t0 + tokens, ...) of the sequence; keys from `beg` on, 128 at a time
-  const int t0 = it.part * TILES * p.tokens;
-  const int beg = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
-  const int end0 = min(it.n, t0 + p.tokens), end1 = min(it.n, t0 + TILES * p.tokens);
-  const int n0 = (end0 - beg + kPtKeys - 1) / kPtKeys, n1 = TILES == 2 && end1 > end0 ? (end1 - beg + kPtKeys - 1) / kPtKeys : 0;
-  const int steps = max(n0, n1);
-
   const uint32_t bars = base + L::bar;
   auto q_full  = [&](int x) { return bars + 8u * x; };
   auto full    = [&](int s) { return bars + 16u + 8u * s; };
@@ -468,12 +454,8 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 152);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 156);
   RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 160);   // what the TMA warp armed last
-
-  if (warp == L::kWarpMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   if (threadIdx.x == 0) {
+    for (const CUtensorMap* m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full(i), 1);
       mbar_init(s_full(i), 1);
@@ -489,6 +471,45 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     *ring_end = RingArmed();
     fence_barrier_init();
     fence_proxy_async();
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = blockIdx.x % a.kv_heads;
+  PromptItem it;
+  if (!find_item<L::kThreads>(a, TILES * p.tokens, blockIdx.x / a.kv_heads, it)) return;   // (its barriers publish the ones above)
+  // tokens [t0, t0 + tokens) and [t0 + tokens, ...) of the sequence; keys from `beg` on, 128 at a time
+  const int t0 = it.part * TILES * p.tokens;
+  const int beg = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
+  const int end0 = min(it.n, t0 + p.tokens), end1 = min(it.n, t0 + TILES * p.tokens);
+  const int n0 = (end0 - beg + kPtKeys - 1) / kPtKeys, n1 = TILES == 2 && end1 > end0 ? (end1 - beg + kPtKeys - 1) / kPtKeys : 0;
+  const int steps = max(n0, n1);
+
+  // The TMA warp's copies: queries, then keys 0, values 0, keys 1, ... The first ones need no room made and start at once.
+  RingArmed armed;
+  auto load = [&](uint32_t dst, const CUtensorMap* map, int head, int row, uint32_t bytes, uint32_t bar) {
+    mbar_expect_tx(bar, bytes * (DM / 64));
+    for (int d = 0; d < DM; d += 64) pt_load(dst + (d / 64) * kPtHalf, map, d, head, row, bar);
+  };
+  auto load_queries = [&](int x) {
+    load(base + L::q + x * L::kOperand, &p.q, g * p.G, it.row0 + t0 + x * p.tokens, static_cast<uint32_t>(p.tokens * p.G) * 128u, q_full(x));
+    armed.arm(L::kStages + x, 0);
+  };
+  auto load_keys = [&](int i, int st, uint32_t ph) {
+    load(base + L::kv + st * L::kOperand, i & 1 ? &p.v : &p.k, g, it.row0 + beg + (i >> 1) * kPtKeys, kPtHalf, full(st));
+    armed.arm(st, ph);
+  };
+  if (warp == L::kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (warp == L::kWarpTma) {
+    if (lane == 0) {
+      load_queries(0);
+      for (int i = 0; i < min(L::kStages, 2 * steps); ++i) {
+        load_keys(i, i, 0);
+        if (i == 0 && n1 > 0) load_queries(1);
+      }
+    }
+    __syncwarp();
   }
   tc_before();
   __syncthreads();
@@ -629,9 +650,8 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   }
   if (warp == L::kWarpTma) {
-    // ------------------------------------------------------------------ queries, then keys and values
+    // ------------------------------------------------------------------ keys and values behind the first ones
     if (lane == 0) {
-      RingArmed armed;
       auto wait1 = [&](uint32_t bar, uint32_t parity) -> bool {
         for (uint32_t i = 0; i < (1u << 21); ++i) {
           if (mbar_try_wait(bar, parity)) return true;
@@ -640,22 +660,11 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
         *abort_flag = 1;
         return false;
       };
-      auto load = [&](uint32_t dst, const CUtensorMap* map, int head, int row, uint32_t bytes, uint32_t bar) {
-        mbar_expect_tx(bar, bytes * (DM / 64));
-        for (int d = 0; d < DM; d += 64) pt_load(dst + (d / 64) * kPtHalf, map, d, head, row, bar);
-      };
-      const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128u;
-      load(base + L::q, &p.q, g * p.G, it.row0 + t0, q_bytes, q_full(0));
-      armed.arm(L::kStages, 0);
-      for (int i = 0, st = 0, ph = 0; i < 2 * steps; ++i) {       // keys 0, values 0, keys 1, ...
+      uint32_t ph = 1;
+      for (int i = L::kStages, st = 0; i < 2 * steps; ++i) {
         if (!(ok = wait1(empty(st), ph ^ 1u))) break;
-        load(base + L::kv + st * L::kOperand, i & 1 ? &p.v : &p.k, g, it.row0 + beg + (i >> 1) * kPtKeys, kPtHalf, full(st));
-        armed.arm(st, ph);
-        if (i == 0 && n1 > 0) {
-          load(base + L::q + L::kOperand, &p.q, g * p.G, it.row0 + t0 + p.tokens, q_bytes, q_full(1));
-          armed.arm(L::kStages + 1, 0);
-        }
-        if (++st == L::kStages) { st = 0; ph ^= 1; }
+        load_keys(i, st, ph);
+        if (++st == L::kStages) { st = 0; ph ^= 1u; }
       }
       *ring_end = armed;
     }
