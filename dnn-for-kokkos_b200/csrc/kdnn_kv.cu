@@ -7,6 +7,8 @@
 // older codes by a shift, and the attention kernel applies scales without error.
 #include "kdnn_common.cuh"
 
+#include <algorithm>
+
 namespace kdnn {
 
 // ---- page plan ------------------------------------------------------------------------------------------
@@ -14,10 +16,10 @@ namespace kdnn {
 //   row_start = min(cumsum max(n, 0), rows), m = its difference; have = ceil(L / page);
 //   need = min(ceil((L + m) / page), cols) - have; pages are handed out in sequence order while there are any:
 //   got = clamp(available - sum of the needs before, 0, need); stored = min(m, (have + got) page - L).
-// Everything is a prefix sum over the sequences followed by independent entries, so each CTA of a small cluster
-// forms the sums for itself in shared memory and writes its share of the entries; the cluster barrier lies between the
-// last read of lens / state and their new values, which may go to the same arrays.
-constexpr int kPlanCluster = 8;
+// Everything is a prefix sum over the sequences followed by independent entries, so each CTA forms the sums for itself in
+// shared memory and writes its share of the entries. Where lens / state are updated in place, a large plan's CTAs are one cluster, whose
+// barrier lies between the last read of them and their new values; else there are as many CTAs as there is work for.
+constexpr int kPlanCluster = 8, kPlanCtas = 64;
 
 struct PlanArgs {
   const int32_t *fresh, *lens, *state;
@@ -25,22 +27,12 @@ struct PlanArgs {
   int4* writes;
   size_t ldt;
   int B, shift, rows, cols, pages, most;   // pages of 1 << shift tokens
+  bool in_place;                           // lens_out / state_out overlap lens / state
 };
 
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
 }
-__device__ __forceinline__ unsigned cluster_rank() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ unsigned cluster_size() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-
 // Exclusive sum over the block's threads of one 64-bit value each; `total` comes back to everybody.
 template <int THREADS>
 __device__ __forceinline__ long long block_exclusive(long long v, long long* warps, long long& total) {
@@ -159,7 +151,7 @@ __global__ void __launch_bounds__(THREADS) kv_plan_kernel(PlanArgs a) {
     const int h = held(b);
     return j < h ? a.table[static_cast<size_t>(b) * a.ldt + j] : a.ring[ring_at(head, tk[b] + j - h)];
   };
-  const int step = static_cast<int>(cluster_size()) * THREADS, me = static_cast<int>(cluster_rank()) * THREADS + threadIdx.x;
+  const int step = static_cast<int>(gridDim.x) * THREADS, me = static_cast<int>(blockIdx.x) * THREADS + threadIdx.x;
   const int rows = rs[B];
   // four rows per search; a page is looked up where it changes
   const bool wide = (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0;
@@ -206,8 +198,8 @@ __global__ void __launch_bounds__(THREADS) kv_plan_kernel(PlanArgs a) {
     const int b = upper_of(gv, B, p);
     a.ring[ring_at(tail, p)] = a.table[static_cast<size_t>(b) * a.ldt + p - gv[b]];
   }
-  if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
-  if (cluster_rank() == 0) {
+  if (a.in_place && gridDim.x > 1) cluster_sync_all(); else __syncthreads();
+  if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < B; b += THREADS) {
       const bool ended = stor[b] < 0;
       a.row_start[b] = rs[b];
@@ -229,7 +221,13 @@ static cudaError_t launch_plan(const PlanArgs& a, unsigned ctas, cudaStream_t st
   static SmemAttrOnce once;
   const cudaError_t e = set_max_smem_once(once, kv_plan_kernel<THREADS>, (6 * 8192 + 4) * 4);
   if (e != cudaSuccess) return e;
-  return launch_chained_cluster(kv_plan_kernel<THREADS>, dim3(ctas), dim3(THREADS), (6 * static_cast<size_t>(a.B) + 4) * 4, ctas, st, a);
+  const size_t smem = (6 * static_cast<size_t>(a.B) + 4) * 4;
+  if (a.in_place && ctas > 1) return launch_chained_cluster(kv_plan_kernel<THREADS>, dim3(ctas), dim3(THREADS), smem, ctas, st, a);
+  return launch_chained(kv_plan_kernel<THREADS>, dim3(ctas), dim3(THREADS), smem, st, a);
+}
+static bool overlap(const int32_t* x, const int32_t* y, size_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return a < b + n * 4 && b < a + n * 4;
 }
 
 cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int32_t* state, int32_t* table, size_t ldt, size_t cols,
@@ -239,10 +237,12 @@ cudaError_t kv_plan_launch(const int32_t* fresh, const int32_t* lens, const int3
   while ((size_t(1) << shift) < page) ++shift;
   PlanArgs a{fresh, lens, state, table, ring, row_start, first, lens_out, state_out, slots, reinterpret_cast<int4*>(writes), ldt,
              static_cast<int>(B), shift, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(pages),
-             static_cast<int>(most)};
-  // one CTA of 256 threads while each has a few entries (a decode step of 64 sequences: 6.7 us, 12.6 with 1024 threads), else a cluster of large
-  // ones (134 000 rows of 200 sequences: 16 us)
-  return rows / 4 + most + B <= 1024 ? launch_plan<256>(a, 1, st) : launch_plan<1024>(a, kPlanCluster, st);
+             static_cast<int>(most), overlap(lens, lens_out, B) || overlap(state, state_out, 4)};
+  // one CTA of 256 threads while each has a few entries (a decode step of 64 sequences: 6.7 us, 12.6 with 1024 threads), else large ones
+  // (134 000 rows of 200 sequences: 9.3 us, on a cluster of eight 16)
+  const size_t work = rows / 4 + most;
+  if (work + B <= 1024) return launch_plan<256>(a, 1, st);
+  return launch_plan<1024>(a, a.in_place ? kPlanCluster : static_cast<unsigned>(std::min<size_t>(kPlanCtas, work / 1024 + 1)), st);
 }
 
 // ---- new rows into the cache ---------------------------------------------------------------------------------

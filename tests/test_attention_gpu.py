@@ -113,6 +113,15 @@ def test_plan(kd, B, page, ctx, fresh):
     check_plan(kd, new, lens, table, ring, state, page, rows + 13, in_place=B % 2 == 0, ldt=len(table[0]) + 3)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("B,page,ctx,fresh", [(200, 64, 300, 700), (8192, 32, 40, 9)])
+def test_plan_of_many_rows(kd, B, page, ctx, fresh, in_place):
+    rng = random.Random(B)
+    lens, table, ring, state = make_pool(rng, B, page, ctx, extra=B * (fresh // page + 1))
+    new = [rng.choice([fresh, 0, -1, rng.randrange(0, fresh + 1)]) for _ in range(B)]
+    check_plan(kd, new, lens, table, ring, state, page, sum(max(n, 0) for n in new), in_place=in_place)
+
+
 def test_plan_when_something_runs_out(kd):
     rng = random.Random(5)
     for extra, cols, cut in ((0, None, 0), (3, None, 0), (100, 4, 0), (100, None, 50), (5, 6, 11)):
