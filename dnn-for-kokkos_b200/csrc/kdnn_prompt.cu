@@ -2,17 +2,17 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2(e),  m a running reference.
 //
-// prompt_tc_kernel (bf16, heads of up to 128, 16-byte aligned rows): 128 query rows of one kv head, a few tokens times the
+// prompt_tc_kernel (bf16, 16-byte aligned rows): 128 query rows of one kv head, a few tokens times the
 // heads of the group, are the M of a tcgen05 product, so a group shares every key and value that is fetched and a short
-// prompt fills its tile. A CTA owns two such tiles and walks the keys 128 at a time: TMA brings keys and values (five stages
-// in turn), S = Q K^T lands in TMEM, a warpgroup per tile turns it into weights (a thread owns a row: no shuffles) and
+// prompt fills its tile. A CTA owns two such tiles (one, where heads are over 128) and walks the keys 128 at a time: TMA brings keys and values (five stages
+// in turn, two for heads over 128), S = Q K^T lands in TMEM, a warpgroup per tile turns it into weights (a thread owns a row: no shuffles) and
 // writes them back as bf16 over the scores, O += P V accumulates in TMEM. While one tile's scores go through the exponentials,
 // the tensor cores work for the other. The reference m moves, and O is rescaled, only when a score passes it by 2^8.
 // Weights are rounded to bf16 (2^-8 each, averaged over the keys); sums and references are fp32.
 // A product reads masked values with weight 0, so infinities or NaN there would reach the sum: a row that does not come out finite, although
 // its scores are, is computed again from its own keys alone where one of the masked values beside it is not finite.
 //
-// prompt_tile_kernel (fp32, larger heads, any alignment): 64 query rows against 64 keys in shared memory, fp32 FMA pairs.
+// prompt_tile_kernel (fp32, any alignment, any scale): 64 query rows against 64 keys in shared memory, fp32 FMA pairs.
 #include "kdnn_tc.cuh"
 
 #include "kdnn_ring.cuh"
@@ -348,13 +348,13 @@ constexpr uint32_t kPtHalf = 128 * 128;     // 128 rows of 64 channels, 128-byte
 // TILES: query tiles of a CTA. Two share every key and value and keep the tensor cores busy in turn; one is for calls that would leave SMs idle.
 template <int DM, int TILES>
 struct PtLayout {
-  static constexpr int kThreads = 128 * TILES + 128, kWarpTma = 4 * TILES, kWarpMma = kWarpTma + 1, kStages = 5;
-  static constexpr uint32_t kColumns = 256 * TILES;             // TMEM: scores of the tiles (the weights take the first half of the
+  static constexpr int kThreads = 128 * TILES + 128, kWarpTma = 4 * TILES, kWarpMma = kWarpTma + 1, kStages = DM == 256 ? 2 : 5;
+  static constexpr uint32_t kColumns = DM == 256 ? 512 : 256 * TILES;   // TMEM: scores of the tiles (the weights take the first half of the
   static constexpr uint32_t kO = 128 * TILES;                   // same columns), then their sums
   static constexpr uint32_t kOperand = (DM / 64) * kPtHalf;     // 128 rows x DM channels
   static constexpr uint32_t q = 0, kv = q + TILES * kOperand, bar = kv + kStages * kOperand;   // kv: keys and values in turn
   static constexpr uint32_t total = bar + 256 + 1024;           // + slack for the 1024-byte alignment of the base
-  static_assert(total <= 232448, "one CTA's shared memory");
+  static_assert(total <= 232448 && 128 * TILES + TILES * DM <= kColumns, "one CTA's shared memory and TMEM");
 };
 
 struct alignas(64) PromptParams {
@@ -773,8 +773,9 @@ static cudaError_t launch_tc(const PromptParams& p, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   return launch_chained(prompt_tc_kernel<DM, TILES>, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::total, st, p);
 }
-// One tile per CTA while all of them find an SM of their own (a prompt of 77 tokens, 32 / 8 heads: 7.6 us against 9.6), else two (with one,
-// 8192 tokens took 605 us against 500).
+// One tile per CTA while all of them find an SM of their own (a prompt of 77 tokens, 32 / 8 heads: 7.6 us against 9.6 when it was chosen, 6.7
+// now), else two (with one, 8192 tokens took 605 us against 500). Heads over 128 leave room for one: queries and two operands
+// of 64 KB (4096 tokens, 8 / 4 heads of 256: 79 us, 870 TFLOP/s).
 template <int DM>
 static cudaError_t launch_tiles_tc(const PromptParams& p, cudaStream_t st) {
   const long long tiles = static_cast<long long>(std::min(p.a.rows, p.a.rows / p.tokens + p.a.seqs)) * p.a.kv_heads;
@@ -788,7 +789,7 @@ cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                           reinterpret_cast<uintptr_t>(a.out);
   // TMA wants 16-byte pitches; the kernel's maximum is one of products, so the scale has to be positive
-  if (a.dim <= 128 && G <= 128 && pitches % 8 == 0 && bases % 16 == 0 && a.scale > 1e-30f && a.scale < 1e30f) {
+  if (G <= 128 && pitches % 8 == 0 && bases % 16 == 0 && a.scale > 1e-30f && a.scale < 1e30f) {
     PromptParams p;
     p.a = a;
     p.G = G;
@@ -799,7 +800,7 @@ cudaError_t prompt_attention_launch(const AttnArgs& a, cudaStream_t st) {
     if (encode_heads(&p.q, a.q, a.ldq, a.hdq, a.rows, a.heads, a.dim, G, p.tokens) &&
         encode_heads(&p.k, a.k, a.ldk, a.hdk, a.rows, a.kv_heads, a.dim, 1, kPtKeys) &&
         encode_heads(&p.v, a.v, a.ldv, a.hdv, a.rows, a.kv_heads, a.dim, 1, kPtKeys))
-      return a.dim <= 64 ? launch_tiles_tc<64>(p, st) : launch_tiles_tc<128>(p, st);
+      return a.dim <= 64 ? launch_tiles_tc<64>(p, st) : a.dim <= 128 ? launch_tiles_tc<128>(p, st) : launch_tc<256, 1>(p, st);
   }
   return launch_tiles<__nv_bfloat16>(a, st);
 }

@@ -532,6 +532,14 @@ def test_prompt_attention_of_many_rows(kd, dtype, heads, kv, dim, lens, window):
     prompt_case(kd, dtype, heads, kv, dim, lens, window, seed=dim + heads, lead=2, pad=3)
 
 
+@pytest.mark.parametrize("heads,kv,dim,lens,window", [
+    (16, 2, 256, [1300, 0, 77], 0), (8, 8, 256, [700, 129], 200), (6, 2, 200, [515], 0), (4, 1, 136, [300, 1, 2], 64),
+    (20, 4, 192, [257, 256, 255], 0), (3, 3, 256, [1], 0), (128, 1, 256, [140], 33),
+])
+def test_prompt_attention_of_wide_heads(kd, heads, kv, dim, lens, window):
+    prompt_case(kd, torch.bfloat16, heads, kv, dim, lens, window, seed=dim + heads, lead=1, pad=5)
+
+
 def test_prompt_attention_of_many_sequences(kd):
     rng = random.Random(4)
     lens = [rng.choice([0, 1, 2, 17, 40]) for _ in range(700)]
