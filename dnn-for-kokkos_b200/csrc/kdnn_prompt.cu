@@ -12,7 +12,7 @@
 // A product reads masked values with weight 0, so infinities or NaN there would reach the sum: a row that does not come out finite, although
 // its scores are, is computed again from its own keys alone where one of the masked values beside it is not finite.
 //
-// prompt_tile_kernel (fp32, any alignment, any scale): 64 query rows against 64 keys in shared memory, fp32 FMA pairs.
+// prompt_tile_kernel (fp32, any alignment, any scale): 64 query rows against 32 keys in shared memory, tf32 products of two parts each.
 #include "kdnn_tc.cuh"
 
 #include "kdnn_ring.cuh"
@@ -111,17 +111,41 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int 
 }
 
 // ---- fp32 tiles -----------------------------------------------------------------------------------------------------------
-// Bound by FMA issue and by what feeds it from shared memory (eight 16-byte loads per 32 FMA pairs). fp32 keys and values of the next tile
-// come by cp.async while this one is used, where two tiles fit (DM <= 128).
-constexpr int kTileM = 64, kTileN = 64;
-template <class ST, int DM>
+// S = Q K^T and O = P V on mma.sync m16n8k8 with tf32 operands in two parts, x = hi + lo: hi is x rounded to eleven bits, lo the rest
+// cut to eleven, and hi hi + hi lo + lo hi leaves out 2^-21 of a product at most (bf16 values are one part). The products' own sums drop
+// bits without rounding, so no more than four products with hi hi meet in one before it goes to an fp32 register by an ordinary sum.
+// A part needs finite values below 2^127: a tile that holds others is computed by single FMAs, which leave masked keys out.
+// The order of channels within 16 (of a product over them) and of keys within 8 is such that fragments are 16-byte loads and
+// the scores' accumulators are the weights' operand.
+constexpr int kTileM = 64, kTileN = 32, kTileWarps = kTileM / 16;
+template <int DM, int GROUPS>
 struct TileShape {
-  static constexpr bool kAhead = sizeof(ST) == 4 && DM <= 128;
-  static constexpr int kPitch = DM + 4, kPPitch = kTileN + 4, kKv = kTileN * (kPitch + DM);   // a tile of keys, then of values
-  static constexpr int kFloats = kTileM * kPitch + (kAhead ? 2 : 1) * kKv + kTileM * kPPitch;
+  static constexpr int kKeys = kTileN * GROUPS, kThreads = kTileWarps * 32 * GROUPS;
+  static constexpr int kKPitch = DM + 16, kVPitch = DM + 4, kKv = kKeys * (kKPitch + kVPitch);   // no two lanes of a load in a bank
+  static constexpr int kFloats = kTileM * kKPitch + 2 * kKv;
+  static_assert(GROUPS == 1 || kTileWarps * 32 * (DM / 2 + 4) <= kKv, "a group's sums fit where its keys were");
 };
 __device__ __forceinline__ void tile_fetch(float* dst, const void* src, bool there) {   // 16 bytes, zeros where there is nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void mma1688(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TWO>
+__device__ __forceinline__ void in_parts(float x, uint32_t& hi, uint32_t& lo) {
+  if (TWO) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
+  } else {
+    hi = __float_as_uint(x);
+    lo = 0u;
+  }
+}
+__device__ __forceinline__ bool beyond_parts(float4 x) {
+  auto size = [](float v) { return __float_as_int(v) & 0x7FFFFFFF; };
+  return max(max(size(x.x), size(x.y)), max(size(x.z), size(x.w))) >= 0x7F000000;
 }
 
 // Four channels of a row; channels behind D are 0.
@@ -132,66 +156,77 @@ __device__ __forceinline__ float4 four_of(const ST* p, int d, int D) {
   return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// Thread (ty, tx) of 16 x 16 holds rows 4 ty .. + 3 against keys tx + 16 i, and channels 4 tx + 64 i of the result.
-template <class ST, int DM>
-__global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(AttnArgs a) {
-  using S = TileShape<ST, DM>;
+// GROUPS groups of warps hold the same rows and take kTileN keys each of what is fetched at a time.
+// Warp w of a group holds the rows 16 w + g and + 8 (lane = 4 g + c): keys 8 j + 2 c, + 1 of the scores, channels 32 i + 8 c .. + 7 of the result.
+template <class ST, int DM, int GROUPS>
+__global__ void __launch_bounds__(kTileWarps * 32 * GROUPS, GROUPS == 2 ? 128 / DM : DM == 64 ? 3 : DM == 128 ? 2 : 1) prompt_tile_kernel(AttnArgs a) {
+  using S = TileShape<DM, GROUPS>;
+  constexpr int THREADS = S::kThreads;
+  constexpr bool TWO = sizeof(ST) == 4;
   pdl_chain_entry();
   extern __shared__ __align__(16) float sf[];
-  float *sq = sf, *kv = sq + kTileM * S::kPitch, *sp = kv + (S::kAhead ? 2 : 1) * S::kKv;
-  __shared__ unsigned long long s_bad;
+  float *sq = sf, *kv = sq + kTileM * S::kKPitch;
   const int g = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads, D = a.dim;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % kTileWarps, group = threadIdx.x / (kTileWarps * 32), lg = lane >> 2, lc = lane & 3;
   PromptItem it;
   // a part of a sequence: the tokens whose query rows (token, head of the group) fill a tile, or one token of a larger group
   const int tokens = max(kTileM / G, 1), splits = (tokens * G + kTileM - 1) / kTileM;
   const int idx = blockIdx.x / a.kv_heads;
-  if (!find_item<256>(a, tokens, idx / splits, it)) return;
+  if (!find_item<THREADS>(a, tokens, idx / splits, it)) return;
   const int f0 = (idx % splits) * kTileM;             // first flattened row inside the part
   const int tok0 = it.part * tokens;
   const int fn = min(min(tokens, it.n - tok0) * G - f0, kTileM);
   if (fn <= 0) return;
-  if (threadIdx.x == 0) s_bad = 0ull;
 
   auto q_at = [&](int r) { return f0 + min(r, fn - 1); };
-  for (int i = threadIdx.x; i < kTileM * (DM / 4); i += 256) {
+  bool odd_q = false;
+  for (int i = threadIdx.x; i < kTileM * (DM / 4); i += THREADS) {
     const int r = i / (DM / 4), d = (i % (DM / 4)) * 4, f = q_at(r), t = f / G;
     const ST* q = static_cast<const ST*>(a.q) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldq + static_cast<size_t>(g * G + f - t * G) * a.hdq;
-    *reinterpret_cast<float4*>(sq + r * S::kPitch + d) = four_of<ST>(q, d, D);
+    const float4 x = four_of<ST>(q, d, D);
+    odd_q |= beyond_parts(x);
+    *reinterpret_cast<float4*>(sq + r * S::kKPitch + d) = x;
   }
-  int hi[4], lo[4];
-  float m[4], l[4];
-  float4 o[4][DM / 64];
+  int hi[2], lo[2];
+  float m[2], l[2];
+  float o[DM / 8][4];          // [4 i + e]: channels 32 i + 8 c + e and + 4 of row g, then of row g + 8
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int pos = tok0 + q_at(4 * ty + r) / G;
+  for (int r = 0; r < 2; ++r) {
+    const int pos = tok0 + q_at(16 * w + lg + 8 * r) / G;
     hi[r] = pos + 1;
     lo[r] = a.window > 0 ? pos - a.window + 1 : 0;
     m[r] = -INFINITY;
     l[r] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DM / 64; ++i) o[r][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
+#pragma unroll
+  for (int i = 0; i < DM / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
   const int p_lo = tok0 + f0 / G, p_hi = tok0 + (f0 + fn - 1) / G;
   const int k_beg = a.window > 0 ? max(0, p_lo - a.window + 1) : 0, k_end = p_hi + 1;
+  // keys that some row of this warp sees, and those that all of them see
+  const int w_lo = tok0 + q_at(16 * w) / G, w_hi = tok0 + q_at(16 * w + 15) / G;
+  const int see_beg = a.window > 0 ? w_lo - a.window + 1 : 0, all_beg = a.window > 0 ? w_hi - a.window + 1 : 0;
   const float c = a.scale * 1.4426950408889634f;
   // this thread's share of a tile: rows r0 + RP i, four channels at d0
-  constexpr int RP = 1024 / DM, EACH = kTileN / RP;
+  constexpr int RP = THREADS * 4 / DM, EACH = S::kKeys / RP;
   const int r0 = threadIdx.x / (DM / 4), d0 = (threadIdx.x % (DM / 4)) * 4;
   const ST* kbase = static_cast<const ST*>(a.k) + static_cast<size_t>(it.row0) * a.ldk + static_cast<size_t>(g) * a.hdk;
   const ST* vbase = static_cast<const ST*>(a.v) + static_cast<size_t>(it.row0) * a.ldv + static_cast<size_t>(g) * a.hdv;
-  // rows on 16 bytes: fetched asynchronously; else loaded one by one
-  const bool async = S::kAhead && ((reinterpret_cast<uintptr_t>(kbase) | reinterpret_cast<uintptr_t>(vbase)) & 15u) == 0 && ((a.ldk | a.ldv) & 3u) == 0;
+  // fp32 rows on 16 bytes: fetched asynchronously; others loaded one by one
+  const bool async = TWO && ((reinterpret_cast<uintptr_t>(kbase) | reinterpret_cast<uintptr_t>(vbase)) & 15u) == 0 && ((a.ldk | a.ldv) & 3u) == 0;
+  auto share = [&](int buf) { return kv + buf * S::kKv + r0 * S::kKPitch + d0; };
+  auto share_v = [&](int buf) { return kv + buf * S::kKv + S::kKeys * S::kKPitch + r0 * S::kVPitch + d0; };
   auto request = [&](int k0, int buf) {      // a key behind the last one is 0
-    float *tk = kv + buf * S::kKv + r0 * S::kPitch + d0, *tv = kv + buf * S::kKv + kTileN * S::kPitch + r0 * DM + d0;
+    float *tk = share(buf), *tv = share_v(buf);
     if (async) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int row = k0 + r0 + RP * i;
         const bool there = row < k_end && d0 < D;
         const size_t at = there ? row : 0;
-        tile_fetch(tk + RP * i * S::kPitch, kbase + at * a.ldk + (there ? d0 : 0), there);
-        tile_fetch(tv + RP * i * DM, vbase + at * a.ldv + (there ? d0 : 0), there);
+        tile_fetch(tk + RP * i * S::kKPitch, kbase + at * a.ldk + (there ? d0 : 0), there);
+        tile_fetch(tv + RP * i * S::kVPitch, vbase + at * a.ldv + (there ? d0 : 0), there);
       }
     } else {
 #pragma unroll 4
@@ -202,143 +237,261 @@ __global__ void __launch_bounds__(256, DM == 64 ? 2 : 1) prompt_tile_kernel(Attn
           x = four_of<ST>(kbase + static_cast<size_t>(row) * a.ldk, d0, D);
           y = four_of<ST>(vbase + static_cast<size_t>(row) * a.ldv, d0, D);
         }
-        *reinterpret_cast<float4*>(tk + RP * i * S::kPitch) = x;
-        *reinterpret_cast<float4*>(tv + RP * i * DM) = y;
+        *reinterpret_cast<float4*>(tk + RP * i * S::kKPitch) = x;
+        *reinterpret_cast<float4*>(tv + RP * i * S::kVPitch) = y;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (S::kAhead) request(k_beg, 0);
-  for (int k0 = k_beg, buf = 0; k0 < k_end; k0 += kTileN) {
+  request(k_beg, 0);
+  for (int at = k_beg, buf = 0; at < k_end; at += S::kKeys, buf ^= 1) {
     __syncthreads();      // the tile before has been used
-    if (S::kAhead) {
-      if (k0 + kTileN < k_end) {
-        request(k0 + kTileN, buf ^ 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      } else {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      }
+    if (at + S::kKeys < k_end) {
+      request(at + S::kKeys, buf ^ 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
-      request(k0, 0);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    __syncthreads();
-    const float *sk = kv + buf * S::kKv, *sv = sk + kTileN * S::kPitch;
-    if (S::kAhead) buf ^= 1;
-    float2 s2[4][4];
+    bool odd = odd_q;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s2[r][i] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (int d = 0; d < DM; d += 4) {
-      float4 qv[4], kv[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) qv[r] = *reinterpret_cast<const float4*>(sq + (4 * ty + r) * S::kPitch + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(sk + (tx + 16 * i) * S::kPitch + d);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s2[r][i] = ffma2(make_float2(qv[r].x, qv[r].y), make_float2(kv[i].x, kv[i].y), s2[r][i]);
-          s2[r][i] = ffma2(make_float2(qv[r].z, qv[r].w), make_float2(kv[i].z, kv[i].w), s2[r][i]);
-        }
+    for (int i = 0; i < EACH; ++i) {
+      odd |= beyond_parts(*reinterpret_cast<const float4*>(share(buf) + RP * i * S::kKPitch));
+      odd |= beyond_parts(*reinterpret_cast<const float4*>(share_v(buf) + RP * i * S::kVPitch));
     }
+    odd = __syncthreads_or(odd);
+    const int k0 = at + group * kTileN;      // this group's keys
+    if (k0 > w_hi || k0 + kTileN <= see_beg) continue;
+    const float *sk = kv + buf * S::kKv + group * kTileN * S::kKPitch;
+    const float* sv = kv + buf * S::kKv + S::kKeys * S::kKPitch + group * kTileN * S::kVPitch;
+    const float *qr = sq + (16 * w + lg) * S::kKPitch, *kr = sk + lg * S::kKPitch;
+    // ---- scores
+    float s[kTileN / 8][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float s[4], top = -INFINITY;
+    for (int j = 0; j < kTileN / 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = k0 + tx + 16 * i;
-        s[i] = key < hi[r] && key >= lo[r] ? (s2[r][i].x + s2[r][i].y) * c : -INFINITY;
-        top = fmaxf(top, s[i]);
-      }
+      for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+    if (!odd) {
+      float low[kTileN / 8][4];       // what the lower parts bring
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float nm = fmaxf(m[r], top), ref = nm == -INFINITY ? 0.0f : nm, f = exp2f(m[r] - ref);
-      m[r] = nm;
-      l[r] *= f;
+      for (int j = 0; j < kTileN / 8; ++j)
 #pragma unroll
-      for (int i = 0; i < DM / 64; ++i) {
-        o[r][i].x *= f; o[r][i].y *= f; o[r][i].z *= f; o[r][i].w *= f;
-      }
+        for (int e = 0; e < 4; ++e) low[j][e] = 0.0f;
+#pragma unroll 2
+      for (int d = 0; d < DM; d += 32) {
+        float top[kTileN / 8][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = exp2f(s[i] - ref);
-        l[r] += p;
-        sp[(4 * ty + r) * S::kPPitch + tx + 16 * i] = p;
-      }
-    }
-    __syncwarp();         // a warp's rows are its own: nobody else reads them
-#pragma unroll 4
-    for (int k = 0; k < kTileN; k += 4) {
-      float pv[4][4];
+        for (int j = 0; j < kTileN / 8; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(pv[r]) = *reinterpret_cast<const float4*>(sp + (4 * ty + r) * S::kPPitch + k);
+          for (int e = 0; e < 4; ++e) top[j][e] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+        for (int h = 0; h < 32; h += 16) {
+          const float4 x0 = *reinterpret_cast<const float4*>(qr + d + h + 4 * lc), x1 = *reinterpret_cast<const float4*>(qr + 8 * S::kKPitch + d + h + 4 * lc);
+          uint32_t ah[2][4], al[2][4];
+          in_parts<TWO>(x0.x, ah[0][0], al[0][0]); in_parts<TWO>(x1.x, ah[0][1], al[0][1]);
+          in_parts<TWO>(x0.y, ah[0][2], al[0][2]); in_parts<TWO>(x1.y, ah[0][3], al[0][3]);
+          in_parts<TWO>(x0.z, ah[1][0], al[1][0]); in_parts<TWO>(x1.z, ah[1][1], al[1][1]);
+          in_parts<TWO>(x0.w, ah[1][2], al[1][2]); in_parts<TWO>(x1.w, ah[1][3], al[1][3]);
 #pragma unroll
-        for (int i = 0; i < DM / 64; ++i) {
-          const float4 v = *reinterpret_cast<const float4*>(sv + (k + e) * DM + 64 * i + 4 * tx);
+          for (int j = 0; j < kTileN / 8; ++j) {
+            const float4 y = *reinterpret_cast<const float4*>(kr + 8 * j * S::kKPitch + d + h + 4 * lc);
+            uint32_t bh[4], bl[4];
+            in_parts<TWO>(y.x, bh[0], bl[0]); in_parts<TWO>(y.y, bh[1], bl[1]);
+            in_parts<TWO>(y.z, bh[2], bl[2]); in_parts<TWO>(y.w, bh[3], bl[3]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float2 pp = make_float2(pv[r][e], pv[r][e]);
-            const float2 x = ffma2(pp, make_float2(v.x, v.y), make_float2(o[r][i].x, o[r][i].y));
-            const float2 y = ffma2(pp, make_float2(v.z, v.w), make_float2(o[r][i].z, o[r][i].w));
-            o[r][i] = make_float4(x.x, x.y, y.x, y.y);
+            for (int u = 0; u < 2; ++u) {
+              mma1688(top[j], ah[u], bh[2 * u], bh[2 * u + 1]);
+              if (TWO) {
+                mma1688(low[j], ah[u], bl[2 * u], bl[2 * u + 1]);
+                mma1688(low[j], al[u], bh[2 * u], bh[2 * u + 1]);
+              }
+            }
           }
         }
-    }
-    __syncwarp();
-  }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+        for (int j = 0; j < kTileN / 8; ++j)
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
-    if (4 * ty + r >= fn) continue;
-    const int f = f0 + 4 * ty + r, t = f / G;
-    ST* out = static_cast<ST*>(a.out) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldo + static_cast<size_t>(g * G + f - t * G) * a.hdo;
+          for (int e = 0; e < 4; ++e) s[j][e] += top[j][e];
+      }
+      if (TWO) {
 #pragma unroll
-    for (int i = 0; i < DM / 64; ++i) {
-      const int d = 64 * i + 4 * tx;
-      if (d >= D) continue;
-      const float y[4] = {o[r][i].x / l[r], o[r][i].y / l[r], o[r][i].z / l[r], o[r][i].w / l[r]};
+        for (int j = 0; j < kTileN / 8; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        store_scalar(out + d + e, y[e]);
-        if (!(fabsf(y[e]) < INFINITY) && fabsf(l[r]) < INFINITY) atomicOr(&s_bad, 1ull << (4 * ty + r));
+          for (int e = 0; e < 4; ++e) s[j][e] += low[j][e];
+      }
+    } else {
+      for (int d = 0; d < DM; ++d) {
+        const float x0 = qr[d], x1 = qr[8 * S::kKPitch + d];
+#pragma unroll
+        for (int j = 0; j < kTileN / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float y = sk[(8 * j + 2 * lc + e) * S::kKPitch + d];
+            s[j][e] += x0 * y;
+            s[j][2 + e] += x1 * y;
+          }
       }
     }
+    // ---- weights
+    const bool edge = k0 + kTileN > w_lo + 1 || k0 < all_beg;
+    float top[2] = {-INFINITY, -INFINITY}, f[2], ref[2];
+#pragma unroll
+    for (int j = 0; j < kTileN / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = e >> 1, key = k0 + 8 * j + 2 * lc + (e & 1);
+        s[j][e] *= c;
+        if (edge && (key >= hi[r] || key < lo[r])) s[j][e] = -INFINITY;
+        top[r] = fmaxf(top[r], s[j][e]);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      const float nm = fmaxf(m[r], top[r]);
+      ref[r] = nm == -INFINITY ? 0.0f : nm;
+      f[r] = exp2f(m[r] - ref[r]);
+      m[r] = nm;
+      l[r] *= f[r];
+    }
+#pragma unroll
+    for (int j = 0; j < kTileN / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = exp2f(s[j][e] - ref[e >> 1]);
+        l[e >> 1] += s[j][e];
+      }
+#pragma unroll
+    for (int i = 0; i < DM / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] *= f[e >> 1];
+    // ---- O += P V
+    if (!odd) {
+      uint32_t ph[kTileN / 8][4], pl[kTileN / 8][4];      // rows g, g + 8 at key 2 c, then at key 2 c + 1
+#pragma unroll
+      for (int j = 0; j < kTileN / 8; ++j) {
+        in_parts<true>(s[j][0], ph[j][0], pl[j][0]); in_parts<true>(s[j][2], ph[j][1], pl[j][1]);
+        in_parts<true>(s[j][1], ph[j][2], pl[j][2]); in_parts<true>(s[j][3], ph[j][3], pl[j][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < DM / 32; ++i) {
+        float top[4][4], low[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[n][e] = low[n][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kTileN / 8; ++j) {
+          const float* vr = sv + (8 * j + 2 * lc) * S::kVPitch + 32 * i + 4 * lg;
+          const float4 x = *reinterpret_cast<const float4*>(vr), y = *reinterpret_cast<const float4*>(vr + S::kVPitch);
+          const float v0[4] = {x.x, x.y, x.z, x.w}, v1[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t h0, h1, l0, l1;
+            in_parts<TWO>(v0[n], h0, l0);
+            in_parts<TWO>(v1[n], h1, l1);
+            mma1688(top[n], ph[j], h0, h1);
+            mma1688(low[n], pl[j], h0, h1);
+            if (TWO) mma1688(low[n], ph[j], l0, l1);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[4 * i + n][e] += top[n][e] + low[n][e];
+      }
+    } else {
+      for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+        for (int j = 0; j < kTileN / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = 8 * j + 2 * cc + e, key = k0 + row;
+            const float p0 = __shfl_sync(0xffffffffu, s[j][e], (lane & 28) + cc), p1 = __shfl_sync(0xffffffffu, s[j][2 + e], (lane & 28) + cc);
+            const bool in0 = key < hi[0] && key >= lo[0], in1 = key < hi[1] && key >= lo[1];
+#pragma unroll
+            for (int i = 0; i < DM / 32; ++i)
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float v = sv[row * S::kVPitch + 32 * i + 8 * lc + 4 * h + n];
+                  if (in0) o[4 * i + n][h] += p0 * v;
+                  if (in1) o[4 * i + n][2 + h] += p1 * v;
+                }
+          }
+    }
   }
-  // rows that did not come out finite though their scores are: a warp each, where a value that some of the tile's rows do not see is not
-  __syncthreads();
-  const unsigned long long bad = s_bad;
-  if (bad == 0ull || (!odd_values<ST>(a, it.row0, p_lo + 1, k_end, g) &&
-                      !odd_values<ST>(a, it.row0, k_beg, a.window > 0 ? p_hi - a.window + 1 : 0, g)))
-    return;
-  for (int r = threadIdx.x >> 5; r < kTileM; r += 8) {
-    if (!((bad >> r) & 1ull)) continue;
-    const int f = f0 + r, t = f / G;
-    row_alone<ST>(a, it.row0, tok0 + t, g * G + f - t * G);
+  if (GROUPS == 2) {      // the second group's sums join the first one's
+    float* other = kv + w * 32 * (DM / 2 + 4) + lane;
+    __syncthreads();
+    if (group == 1) {
+#pragma unroll
+      for (int i = 0; i < DM / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) other[32 * (4 * i + e)] = o[i][e];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        other[32 * (DM / 2 + r)] = m[r];
+        other[32 * (DM / 2 + 2 + r)] = l[r];
+      }
+    }
+    __syncthreads();
+    if (group == 1) return;
+    float f0[2], f1[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float m1 = other[32 * (DM / 2 + r)], nm = fmaxf(m[r], m1), ref = nm == -INFINITY ? 0.0f : nm;
+      f0[r] = exp2f(m[r] - ref);
+      f1[r] = exp2f(m1 - ref);
+      l[r] = l[r] * f0[r] + other[32 * (DM / 2 + 2 + r)] * f1[r];
+    }
+#pragma unroll
+    for (int i = 0; i < DM / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * f0[e >> 1] + other[32 * (4 * i + e)] * f1[e >> 1];
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const int fr = 16 * w + lg + 8 * r;
+    if (fr >= fn) continue;
+    const int fl = f0 + fr, t = fl / G;
+    ST* out = static_cast<ST*>(a.out) + static_cast<size_t>(it.row0 + tok0 + t) * a.ldo + static_cast<size_t>(g * G + fl - t * G) * a.hdo;
+#pragma unroll
+    for (int i = 0; i < DM / 32; ++i) {
+      const int d = 32 * i + 8 * lc;
+      if (d >= D) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) store_scalar(out + d + 4 * h + n, o[4 * i + n][2 * r + h] / l[r]);
+    }
   }
 }
 
-template <class ST, int DM>
-static cudaError_t launch_tile(const AttnArgs& a, cudaStream_t st) {
-  const int smem = TileShape<ST, DM>::kFloats * 4, G = a.heads / a.kv_heads;
+template <class ST, int DM, int GROUPS>
+static cudaError_t launch_tile(const AttnArgs& a, unsigned ctas, cudaStream_t st) {
+  using S = TileShape<DM, GROUPS>;
   static SmemAttrOnce once;
-  const cudaError_t e = set_max_smem_once(once, prompt_tile_kernel<ST, DM>, smem);
+  const cudaError_t e = set_max_smem_once(once, prompt_tile_kernel<ST, DM, GROUPS>, S::kFloats * 4);
   if (e != cudaSuccess) return e;
-  const long long tokens = std::max(kTileM / G, 1), splits = (tokens * G + kTileM - 1) / kTileM;
-  const long long parts = std::min<long long>(a.rows, a.rows / tokens + a.seqs);
-  const long long ctas = parts * splits * a.kv_heads;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  return launch_chained(prompt_tile_kernel<ST, DM>, dim3(static_cast<unsigned>(ctas)), dim3(256), smem, st, a);
+  return launch_chained(prompt_tile_kernel<ST, DM, GROUPS>, dim3(ctas), dim3(S::kThreads), S::kFloats * 4, st, a);
 }
+// Two groups of warps where three CTAs per SM hold the call and its longest rows decide (1500 tokens, 16 / 8 heads of 64, window 512:
+// 72 us, 81 with one group), else one (4096 tokens, 16 / 4 heads of 128: 1323 us, 1569 with two).
 template <class ST>
 static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
-  if (a.dim <= 64) return launch_tile<ST, 64>(a, st);
-  return a.dim <= 128 ? launch_tile<ST, 128>(a, st) : launch_tile<ST, 256>(a, st);
+  const int G = a.heads / a.kv_heads;
+  const long long tokens = std::max(kTileM / G, 1), splits = (tokens * G + kTileM - 1) / kTileM;
+  const long long all = std::min<long long>(a.rows, a.rows / tokens + a.seqs) * splits * a.kv_heads;
+  if (all > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  const unsigned ctas = static_cast<unsigned>(all);
+  if constexpr (sizeof(ST) == 4) {
+    if (a.dim <= 128 && all <= 3LL * device_sm_count()) return a.dim <= 64 ? launch_tile<ST, 64, 2>(a, ctas, st) : launch_tile<ST, 128, 2>(a, ctas, st);
+  }
+  if (a.dim <= 64) return launch_tile<ST, 64, 1>(a, ctas, st);
+  return a.dim <= 128 ? launch_tile<ST, 128, 1>(a, ctas, st) : launch_tile<ST, 256, 1>(a, ctas, st);
 }
 
 // ---- tcgen05 tiles ----------------------------------------------------------------------------------------------------------

@@ -7,7 +7,8 @@ Tolerances count roundings. For one output o = sum_j p_j v_j with A = sum_j p_j 
   by the rounding of a weight that enters a matrix product, and by (keys) roundings of fp32 sums, which meet A;
   the result by half a step of its type.
 bf16 operands are exact in a product; a weight is rounded to bf16 (2^-8) for packed bf16 prompts and to fp16 (2^-11) over the
-cache; fp32 operands and weights over the cache are two fp16 parts (2^-22). Over the cache a weight is also off by half of fp16's
+cache; fp32 operands and weights over the cache are two fp16 parts (2^-22). fp32 prompts take two tf32 parts of each operand, which leaves
+out 2^-22 + 2 * 2^-23 = 8 * 2^-24 of a product: the eight roundings that a score and a result have beside those of their sums. Over the cache a weight is also off by half of fp16's
 smallest step, 2^-25, where the largest weight of its row is at least 2^6 (it is 2^(7 + s - m), and m, a whole number, is at most one
 above the largest score): by 2^-31 of the sum, which meets the sum of |v_j|."""
 import math
@@ -656,6 +657,26 @@ def test_prompt_attention_of_values_that_are_not_finite(kd, dtype):
     k[400, 5, 1] = v[3, 2, 9] = v[130, 0, 0] = 0.0
     close = (out.float() - want.float()).abs() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-5) * (want.float().abs() + 1)
     assert (close | reached).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,dim", [(150, 64), (90, 128), (70, 256), (2100, 64)])
+def test_prompt_attention_at_the_ends_of_the_type(kd, dtype, n, dim):
+    """A key whose scores are -inf has no weight; a value near the largest number is met as it is."""
+    q, k, v = rows_of(n, 16, dim, dtype, 1), rows_of(n, 8, dim, dtype, 2), rows_of(n, 8, dim, dtype, 3)
+    q[:, :, 2] = -q[:, :, 2].abs() - 0.125
+    out, far = torch.empty_like(q), torch.empty_like(q)
+    v[5, 1, 3], v[9, 2, 7] = torch.finfo(dtype).max, torch.finfo(dtype).tiny
+    kd.prompt_attention(q, k, v, i32([0, n]), out)
+    check_prompt(q, k, v, out, [0, n], 0, dtype)
+    v[5, 1, 3] = 1.0
+    k[7, 0, 2] = 1e30                     # q . k is below -1e28
+    kd.prompt_attention(q, k, v, i32([0, n]), far)
+    k[7, 0, 2] = float("inf")
+    kd.prompt_attention(q, k, v, i32([0, n]), out)
+    assert torch.isnan(out[7:8, 0:2]).sum() == 0 and torch.isfinite(out).all()
+    close = (out.float() - far.float()).abs() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-5) * (far.float().abs() + 1)
+    assert close.all()
 
 
 def test_calls_on_a_stream_of_their_own(kd):
