@@ -467,7 +467,8 @@ int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, si
  * the last `window` of them). q, out [rows][heads][dim], k, v [rows][kv_heads][dim] Scalar with row and head pitches in
  * elements; dim a multiple of 8 up to 256. Values in masked places (later rows, other sequences) do not reach the result,
  * infinities and NaN included. Rows outside [row_start[0], row_start[seqs]) are left as they were. out must not overlap
- * q, k or v. bf16 rows that are 16-byte aligned run on tcgen05 tiles (weights rounded to bf16, sums fp32), the rest on fp32 tiles. seqs <= 8192. */
+ * q, k or v. bf16 rows that are 16-byte aligned (groups of up to 128 heads, scale > 0) run on tcgen05 tiles, weights rounded to bf16, sums
+ * fp32; the rest on mma.sync tiles with two tf32 parts of each number (about 2^-21 of a product is left out). seqs <= 8192. */
 int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void* k, size_t ldk, size_t hdk, const void* v,
                                size_t ldv, size_t hdv, int scalar, size_t rows, size_t heads, size_t kv_heads, size_t dim,
                                const int32_t* row_start, size_t seqs, void* out, size_t ldo, size_t hdo, float scale,
