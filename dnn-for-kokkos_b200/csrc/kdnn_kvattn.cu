@@ -7,6 +7,8 @@
 //    The tiles of all units form one line; each warp takes an equal run of it, so a long context is split over as many
 //    warps as a batch of short ones. Runs that end inside a unit leave partial sums, joined in a fixed order: within a
 //    CTA through shared memory, between CTAs by kv_join_kernel.
+//  * Calls of few units and short contexts, where launches and dependent loads are all, give each unit a cluster of eight CTAs, whose
+//    pieces meet in distributed shared memory: one launch, no workspace (one sequence of 1900 tokens: 9.4 us, 14.3 with the join).
 //  * Each warp has its own queue of tiles in shared memory, filled by cp.async: bytes in flight without registers, no barrier
 //    between warps, no bank conflicts, and the cache keeps plain rows. What a fetch instruction covers matters: eight neighbouring lanes
 //    a whole 128-byte line is the fast form (lanes of a quarter warp on four rows took 1.3 times as long for the same bytes).
@@ -124,6 +126,10 @@ __device__ __forceinline__ int4 seq_lengths(const AttnArgs& a, int pshift, int b
                    min(max(a.lens[b], 0), a.cols << pshift));      // nothing lies behind the table's pages
 }
 template <int NT>
+__device__ __forceinline__ int row_tiles_of(int n, int G) {
+  return static_cast<int>((static_cast<long long>(n) * G + 8 * NT - 1) / (8 * NT));
+}
+template <int NT>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int G, int4 v) {
   SeqWork s;
   s.row0 = v.x; s.n = v.y; s.first = v.z; s.len = v.w;
@@ -131,7 +137,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int G, int4 v) {
   s.lo = a.window > 0 ? max(s.first - a.window + 1, 0) >> 4 : 0;
   s.tiles = s.n > 0 ? max(((end + 15) >> 4) - s.lo, 1) : 0;
   s.line = s.tiles + kSwitch;
-  s.row_tiles = static_cast<int>((static_cast<long long>(s.n) * G + 8 * NT - 1) / (8 * NT));
+  s.row_tiles = row_tiles_of<NT>(s.n, G);
   return s;
 }
 
@@ -254,8 +260,44 @@ __device__ __forceinline__ void join_tile(const AttnArgs& a, const SeqWork& s, i
   }
 }
 
-// FULL: dim == DM (piece addresses are immediate offsets).
-template <class ST, int DM, int NT, int STAGES, bool FULL>
+// Short calls: a cluster of kCluster CTAs for one unit, whose pieces meet in distributed shared memory, without a second kernel.
+constexpr int kCluster = 8, kShort = 16384;
+// The unit of cluster `index`, by every warp for itself; false: there is none.
+template <int NT>
+__device__ __forceinline__ bool unit_of_cluster(const AttnArgs& a, int G, int pshift, int index, int& b, int& unit, SeqWork& s) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+    const int mine = b0 + lane;
+    const int4 v = mine < a.seqs ? seq_lengths(a, pshift, mine) : make_int4(0, 0, 0, 0);
+    const int units = v.y > 0 ? row_tiles_of<NT>(v.y, G) * a.kv_heads : 0;
+    int inc = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, index >= inc - units && index < inc);
+    if (here != 0) {
+      const int src = __ffs(here) - 1;
+      b = b0 + src;
+      unit = index - __shfl_sync(0xffffffffu, inc - units, src);
+      s = seq_work<NT>(a, G, make_int4(__shfl_sync(0xffffffffu, v.x, src), __shfl_sync(0xffffffffu, v.y, src),
+                                       __shfl_sync(0xffffffffu, v.z, src), __shfl_sync(0xffffffffu, v.w, src)));
+      return true;
+    }
+    index -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory"); }
+__device__ __forceinline__ const float* of_rank(const float* p, int rank) {      // the same place in another CTA of the cluster
+  uint64_t r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(p), "r"(rank));
+  return reinterpret_cast<const float*>(r);
+}
+
+// FULL: dim == DM (piece addresses are immediate offsets). CLUSTER: a unit per cluster, else equal runs of the line per warp.
+template <class ST, int DM, int NT, int STAGES, bool FULL, bool CLUSTER>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) kv_attention_kernel(KvArgs p) {
   using Sh = KvShape<DM>;
   using Pt = KvPart<DM, NT>;
@@ -269,10 +311,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
   const int G = a.heads / a.kv_heads, D = FULL ? DM : a.dim, page = 1 << p.pshift;
   long long* at = reinterpret_cast<long long*>(sm);
   int4* known = reinterpret_cast<int4*>(sm + ((static_cast<uint32_t>(a.seqs + 1) * 8 + 15) & ~15u));
-  const uint32_t ring = smem_u32(sm) + kv_lists_bytes(a.seqs);
+  const uint32_t ring = smem_u32(sm) + (CLUSTER ? 0u : kv_lists_bytes(a.seqs));
   __shared__ int s_order[kKvWarps][2 * kKvWarps];
   __shared__ int4 s_seg[2 * kKvWarps];              // pieces of this CTA's warps: {b, unit, 1, in the queue's place}; z 0: none
-  line_of<NT>(a, G, p.pshift, at, known);
+  if (!CLUSTER) line_of<NT>(a, G, p.pshift, at, known);
   auto work_of = [&](int b) { return seq_work<NT>(a, G, b < kKnown ? known[b] : seq_lengths(a, p.pshift, b)); };
   // Runs: every warp takes one while there are kLeast tiles for it; with fewer, the first CTAs' warps do. (Several runs per warp, the later
   // ones by CTAs that follow on the SMs that finish early, cost more than the SMs' different bandwidths: 122 us against 98 for
@@ -291,8 +333,19 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
       return static_cast<int>(x < cut ? x / (share + 1) : longer + (x - cut) / share);
     }
   };
-  long long pos, end;
-  {
+  int b = 0;
+  SeqWork s{};
+  long long in_b = 0;          // tiles of sequence b before pos
+  long long pos = 0, end = 0;
+  int cluster_unit = 0, workers = 0;
+  const int rank = static_cast<int>(blockIdx.x) % kCluster;
+  if (CLUSTER) {
+    if (!unit_of_cluster<NT>(a, G, p.pshift, static_cast<int>(blockIdx.x) / kCluster, b, cluster_unit, s)) return;   // (all of the cluster)
+    workers = min(kCluster * kKvWarps, (s.tiles + kLeast - 1) / kLeast);
+    const int i = rank * kKvWarps + w, share = s.tiles / workers, longer = s.tiles - share * workers;
+    end  = i < workers ? share + (i < longer ? 1 : 0) : 0;
+    in_b = static_cast<long long>(cluster_unit) * s.line + kSwitch + share * i + min(i, longer);
+  } else {
     const Runs runs(at[a.seqs]);
     pos = runs.start(blockIdx.x * kKvWarps + w);
     end = runs.start(blockIdx.x * kKvWarps + w + 1);
@@ -309,10 +362,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
   float acc[NT][KS][4];
   float mz[NT][2], ml[NT][2], l[NT][2];
 
-  int b = 0;
-  SeqWork s{};
-  long long in_b = 0;          // tiles of sequence b before pos
-  if (pos < end) {
+  if (!CLUSTER && pos < end) {
     int lo = 0, hi = a.seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -323,7 +373,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
     in_b = pos - at[b];
   }
   while (pos < end) {
-    while (in_b >= static_cast<long long>(s.line) * s.row_tiles * a.kv_heads) {
+    while (!CLUSTER && in_b >= static_cast<long long>(s.line) * s.row_tiles * a.kv_heads) {
       in_b = 0;
       s = work_of(++b);
     }
@@ -674,6 +724,21 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
     }
   }
 
+  if (CLUSTER) {      // the CTA's pieces, in its warps' order, then the cluster's, in its CTAs' order; an m tile per warp
+    if (workers == 1) return;
+    const float* queues = reinterpret_cast<const float*>(sm + (ring - smem_u32(sm)));
+    float* piece = reinterpret_cast<float*>(sm + kKvWarps * STAGES * Sh::kStageBytes);
+    const int held = min(workers - rank * kKvWarps, kKvWarps), ctas = (workers + kKvWarps - 1) / kKvWarps;
+    __syncthreads();
+    if (held > 0)
+      for (int x = w; x < Pt::kTiles; x += kKvWarps)
+        join_tile<ST, DM, NT, true>(a, s, cluster_unit, x / KS, x % KS, held, [&](int k) { return queues + k * (STAGES * Sh::kStageBytes / 4); }, piece);
+    cluster_meet();
+    for (int x = rank + kCluster * w; x < Pt::kTiles; x += kCluster * kKvWarps)
+      join_tile<ST, DM, NT, true>(a, s, cluster_unit, x / KS, x % KS, ctas, [&](int k) { return of_rank(piece, k); }, nullptr);
+    cluster_meet();      // nobody's memory goes before it has been read
+    return;
+  }
   // ---- pieces of one unit that this CTA's warps hold are joined, an m tile per warp
   __syncthreads();
   const Runs runs(at[a.seqs]);
@@ -723,11 +788,19 @@ static cudaError_t launch_kv(const KvArgs& p, int ctas, cudaStream_t st) {
   const size_t ring = static_cast<size_t>(kKvWarps) * STAGES * KvShape<DM>::kStageBytes;
   const size_t smem = kv_lists_bytes(p.a.seqs) + ring;
   static SmemAttrOnce once;
-  cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, NT, STAGES, FULL>, static_cast<int>(ring + kv_lists_bytes(8192)));
+  cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, NT, STAGES, FULL, false>, static_cast<int>(ring + kv_lists_bytes(8192)));
   if (e == cudaSuccess)
-    e = launch_chained(kv_attention_kernel<ST, DM, NT, STAGES, FULL>, dim3(ctas), dim3(kKvWarps * 32), smem, st, p);
+    e = launch_chained(kv_attention_kernel<ST, DM, NT, STAGES, FULL, false>, dim3(ctas), dim3(kKvWarps * 32), smem, st, p);
   if (e == cudaSuccess) e = launch_chained(kv_join_kernel<ST, DM, NT>, dim3(ctas), dim3(NT * DM * 2), 0, st, p);
   return e;
+}
+template <class ST, int DM, int STAGES>
+static cudaError_t launch_kv_cluster(const KvArgs& p, int units, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(kKvWarps) * STAGES * KvShape<DM>::kStageBytes + KvPart<DM, 1>::kFloats * 4;
+  static SmemAttrOnce once;
+  const cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, 1, STAGES, true, true>, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  return launch_chained_cluster(kv_attention_kernel<ST, DM, 1, STAGES, true, true>, dim3(units * kCluster), dim3(kKvWarps * 32), smem, kCluster, st, p);
 }
 template <class ST, int DM, int NT, int STAGES>
 static cudaError_t launch_kv_dim(const KvArgs& p, int ctas, cudaStream_t st) {
@@ -762,8 +835,17 @@ cudaError_t kv_attention_launch(const AttnArgs& a, const kdnn_b200_kv_cache* c, 
   KvArgs p{a, c->k, c->v, c->k_scale, c->v_scale, static_cast<int>(c->pages), shift,
            reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ((static_cast<size_t>(ctas) * 16 + 255) & ~size_t(255))),
            static_cast<int4*>(ws)};
+  // A cluster per unit while all of them are resident at once (clusters of eight fill 7/4 of a CTA per SM: 32 units took 7.5 us where
+  // 10.7 are usual, 36 took 12.7 against 10.9) and the table has room for kShort tokens of a sequence at most. 8 kv heads of 128, one
+  // sequence, us with clusters and without: 60 tokens 6.7 and 10.2, 1900 tokens 9.5 and 14.3, 16384 tokens 20.7 and 30.1, 32768
+  // tokens 35.0 and 33.5 (64 CTAs of the 148 SMs then have too little bandwidth).
+  const long long groups = a.heads / a.kv_heads, units = std::min<long long>(a.rows, a.rows * groups / 8 + a.seqs) * a.kv_heads;
+  const bool clusters = nt == 1 && a.seqs <= 64 && (a.dim == 64 || a.dim == 128) && units * kCluster * 4 <= 7LL * device_sm_count() &&
+                        (static_cast<long long>(a.cols) << shift) <= kShort;
   auto go = [&](auto scalar) {
     using ST = decltype(scalar);
+    if (clusters && dm == 64) return launch_kv_cluster<ST, 64, 6>(p, static_cast<int>(units), st);
+    if (clusters) return launch_kv_cluster<ST, 128, 3>(p, static_cast<int>(units), st);
     if (dm == 64) return nt == 1 ? launch_kv_dim<ST, 64, 1, 6>(p, ctas, st) : launch_kv_dim<ST, 64, 2, 8>(p, ctas, st);
     if (dm == 128) return nt == 1 ? launch_kv_dim<ST, 128, 1, 3>(p, ctas, st) : launch_kv_dim<ST, 128, 2, 4>(p, ctas, st);
     return launch_kv_dim<ST, 256, 1, 2>(p, ctas, st);

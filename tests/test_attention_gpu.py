@@ -430,6 +430,24 @@ def test_cache_attention_pages_that_are_not_there(kd):
         check_cache(plan, padded, cache, q, out, [100], [1], 0, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,dim,page,fresh,lens,window", [
+    (32, 8, 128, 64, [1], [1900], 0), (8, 1, 128, 64, [1], [0], 0), (16, 2, 64, 16, [1, 0, 1, 1], [33, 50, 2000, 31], 0),
+    (8, 8, 128, 128, [1, 1, 1, 1], [1, 700, 15, 16], 100), (8, 2, 64, 32, [2, 2, 1, 3], [5, 90, 1000, 0], 0), (4, 4, 64, 64, [7], [900], 33),
+    (32, 8, 128, 64, [1, 1, 1, 1], [8000, 3, 1023, 1024], 0), (16, 2, 128, 64, [1], [16000], 0),
+])
+def test_cache_attention_of_short_and_wide_tables(kd, dtype, heads, kv, dim, page, fresh, lens, window):
+    """Few sequences: a table with room for short contexts alone, and the same one with room for long ones."""
+    plan, table, cache, q, out, ws = cache_case(kd, dtype, heads, kv, dim, page, fresh, lens, window, seed=7, pad=2)
+    wide = torch.cat([table, torch.full((len(fresh), 17000 // page), -1, dtype=torch.int32, device="cuda")], 1)
+    again = torch.full_like(out, 777.0)
+    kd.kv_attention(q, plan, wide, cache, again, ws, window=window)
+    check_cache(plan, wide, cache, q, again, lens, fresh, window, dtype)
+    third = torch.full_like(out, 777.0)
+    kd.kv_attention(q, plan, table, cache, third, ws, window=window)
+    assert torch.equal(out, third) and (out[sum(fresh):] == 777.0).all() and (again[sum(fresh):] == 777.0).all()
+
+
 def test_cache_attention_stale_places_do_not_reach_the_result(kd):
     plan, table, cache, q, out, ws = cache_case(kd, torch.bfloat16, 8, 2, 128, 64, [1, 1], [70, 5], 0)
     want = out.clone()
