@@ -769,30 +769,41 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && DM <= 128 ? 2 : 1) k
   if (threadIdx.x == 0) p.joins[blockIdx.x] = goes_on;
 }
 
-// Units that several CTAs share, joined by the one they begin in: an m tile per warp.
-template <class ST, int DM, int NT>
-__global__ void __launch_bounds__(NT * DM * 2) kv_join_kernel(KvArgs p) {
+// Units that several CTAs share, joined by the one they begin in: an m tile per SPLIT warps, which take a stretch of the pieces each and meet
+// in shared memory where there are many.
+template <class ST, int DM, int NT, int SPLIT>
+__global__ void __launch_bounds__(NT * DM * 2 * SPLIT) kv_join_kernel(KvArgs p) {
   using Pt = KvPart<DM, NT>;
   pdl_chain_entry();
   const int4 job = __ldcg(p.joins + blockIdx.x);
   if (job.x <= 0) return;
   const SeqWork u = seq_work<NT>(p.a, p.a.heads / p.a.kv_heads, seq_lengths(p.a, p.pshift, job.y));
   const float* first = p.parts + (static_cast<size_t>(blockIdx.x) * (kKvWarps + 2) + kKvWarps) * Pt::kFloats;
-  const int w = threadIdx.x >> 5;
-  join_tile<ST, DM, NT, false>(p.a, u, job.z, w / (DM / 16), w % (DM / 16), job.x + 1, [&](int k) {
-    return first + (static_cast<size_t>(k) * (kKvWarps + 2) + (k == 0 ? 1 : 0)) * Pt::kFloats; }, nullptr);
+  const int w = threadIdx.x >> 5, x = w % Pt::kTiles, pieces = job.x + 1;
+  auto piece = [&](int k) { return first + (static_cast<size_t>(k) * (kKvWarps + 2) + (k == 0 ? 1 : 0)) * Pt::kFloats; };
+  if (SPLIT == 1 || pieces <= 8 * SPLIT) {
+    if (SPLIT == 1 || w < Pt::kTiles) join_tile<ST, DM, NT, false>(p.a, u, job.z, x / (DM / 16), x % (DM / 16), pieces, piece, nullptr);
+    return;
+  }
+  __shared__ __align__(16) float s_part[SPLIT][SPLIT > 1 ? Pt::kFloats : 4];
+  const int part = w / Pt::kTiles, k0 = pieces * part / SPLIT, k1 = pieces * (part + 1) / SPLIT;
+  join_tile<ST, DM, NT, false>(p.a, u, job.z, x / (DM / 16), x % (DM / 16), k1 - k0, [&](int k) { return piece(k0 + k); }, s_part[part]);
+  __syncthreads();
+  if (part == 0) join_tile<ST, DM, NT, true>(p.a, u, job.z, x / (DM / 16), x % (DM / 16), SPLIT, [&](int k) { return s_part[k]; }, nullptr);
 }
 
 template <class ST, int DM, int NT, int STAGES, bool FULL>
-static cudaError_t launch_kv(const KvArgs& p, int ctas, cudaStream_t st) {
+static cudaError_t launch_kv(const KvArgs& p, int ctas, bool few, cudaStream_t st) {
   const size_t ring = static_cast<size_t>(kKvWarps) * STAGES * KvShape<DM>::kStageBytes;
   const size_t smem = kv_lists_bytes(p.a.seqs) + ring;
   static SmemAttrOnce once;
   cudaError_t e = set_max_smem_once(once, kv_attention_kernel<ST, DM, NT, STAGES, FULL, false>, static_cast<int>(ring + kv_lists_bytes(8192)));
   if (e == cudaSuccess)
     e = launch_chained(kv_attention_kernel<ST, DM, NT, STAGES, FULL, false>, dim3(ctas), dim3(kKvWarps * 32), smem, st, p);
-  if (e == cudaSuccess) e = launch_chained(kv_join_kernel<ST, DM, NT>, dim3(ctas), dim3(NT * DM * 2), 0, st, p);
-  return e;
+  if (e != cudaSuccess) return e;
+  if constexpr (NT == 1 && DM <= 128)
+    if (few) return launch_chained(kv_join_kernel<ST, DM, NT, 4>, dim3(ctas), dim3(NT * DM * 8), 0, st, p);
+  return launch_chained(kv_join_kernel<ST, DM, NT, 1>, dim3(ctas), dim3(NT * DM * 2), 0, st, p);
 }
 template <class ST, int DM, int STAGES>
 static cudaError_t launch_kv_cluster(const KvArgs& p, int units, cudaStream_t st) {
@@ -803,8 +814,8 @@ static cudaError_t launch_kv_cluster(const KvArgs& p, int units, cudaStream_t st
   return launch_chained_cluster(kv_attention_kernel<ST, DM, 1, STAGES, true, true>, dim3(units * kCluster), dim3(kKvWarps * 32), smem, kCluster, st, p);
 }
 template <class ST, int DM, int NT, int STAGES>
-static cudaError_t launch_kv_dim(const KvArgs& p, int ctas, cudaStream_t st) {
-  return p.a.dim == DM ? launch_kv<ST, DM, NT, STAGES, true>(p, ctas, st) : launch_kv<ST, DM, NT, STAGES, false>(p, ctas, st);
+static cudaError_t launch_kv_dim(const KvArgs& p, int ctas, bool few, cudaStream_t st) {
+  return p.a.dim == DM ? launch_kv<ST, DM, NT, STAGES, true>(p, ctas, few, st) : launch_kv<ST, DM, NT, STAGES, false>(p, ctas, few, st);
 }
 
 int device_sm_count();
@@ -842,13 +853,16 @@ cudaError_t kv_attention_launch(const AttnArgs& a, const kdnn_b200_kv_cache* c, 
   const long long groups = a.heads / a.kv_heads, units = std::min<long long>(a.rows, a.rows * groups / 8 + a.seqs) * a.kv_heads;
   const bool clusters = nt == 1 && a.seqs <= 64 && (a.dim == 64 || a.dim == 128) && units * kCluster * 4 <= 7LL * device_sm_count() &&
                         (static_cast<long long>(a.cols) << shift) <= kShort;
+  // Units of 32 pieces and more: four warps join an m tile (one kv head, 65536 tokens: 40 us, 95 with one; 8 kv heads 43 and 50; with many
+  // units the larger CTAs cost up to 2 us: 64 sequences of 8192 tokens 72.8 and 70.3).
+  const bool few = units * 32 <= ctas;
   auto go = [&](auto scalar) {
     using ST = decltype(scalar);
     if (clusters && dm == 64) return launch_kv_cluster<ST, 64, 6>(p, static_cast<int>(units), st);
     if (clusters) return launch_kv_cluster<ST, 128, 3>(p, static_cast<int>(units), st);
-    if (dm == 64) return nt == 1 ? launch_kv_dim<ST, 64, 1, 6>(p, ctas, st) : launch_kv_dim<ST, 64, 2, 8>(p, ctas, st);
-    if (dm == 128) return nt == 1 ? launch_kv_dim<ST, 128, 1, 3>(p, ctas, st) : launch_kv_dim<ST, 128, 2, 4>(p, ctas, st);
-    return launch_kv_dim<ST, 256, 1, 2>(p, ctas, st);
+    if (dm == 64) return nt == 1 ? launch_kv_dim<ST, 64, 1, 6>(p, ctas, few, st) : launch_kv_dim<ST, 64, 2, 8>(p, ctas, few, st);
+    if (dm == 128) return nt == 1 ? launch_kv_dim<ST, 128, 1, 3>(p, ctas, few, st) : launch_kv_dim<ST, 128, 2, 4>(p, ctas, few, st);
+    return launch_kv_dim<ST, 256, 1, 2>(p, ctas, few, st);
   };
   return a.scalar == KDNN_F32 ? go(float{}) : go(__nv_bfloat16{});
 }

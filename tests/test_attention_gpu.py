@@ -448,6 +448,16 @@ def test_cache_attention_of_short_and_wide_tables(kd, dtype, heads, kv, dim, pag
     assert torch.equal(out, third) and (out[sum(fresh):] == 777.0).all() and (again[sum(fresh):] == 777.0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,dim,window", [(8, 1, 128, 0), (4, 1, 64, 0), (16, 2, 96, 0), (8, 1, 256, 0), (6, 6, 128, 30000)])
+def test_cache_attention_of_one_long_sequence(kd, dtype, heads, kv, dim, window):
+    """A unit of many CTAs' pieces."""
+    plan, table, cache, q, out, ws = cache_case(kd, dtype, heads, kv, dim, 64, [1], [40001], window, seed=3)
+    again = torch.full_like(out, 777.0)
+    kd.kv_attention(q, plan, table, cache, again, ws, window=window)
+    assert torch.equal(out, again)
+
+
 def test_cache_attention_stale_places_do_not_reach_the_result(kd):
     plan, table, cache, q, out, ws = cache_case(kd, torch.bfloat16, 8, 2, 128, 64, [1, 1], [70, 5], 0)
     want = out.clone()
