@@ -114,7 +114,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int 
 // S = Q K^T and O = P V on mma.sync m16n8k8 with tf32 operands in two parts, x = hi + lo: hi is x rounded to eleven bits, lo the rest
 // cut to eleven, and hi hi + hi lo + lo hi leaves out 2^-21 of a product at most (bf16 values are one part). The products' own sums drop
 // bits without rounding, so no more than four products with hi hi meet in one before it goes to an fp32 register by an ordinary sum.
-// A part needs finite values below 2^127: a tile that holds others is computed by single FMAs, which leave masked keys out.
+// Values from 2^64 on, infinities and NaN among them, are not taken apart (what the lower parts bring could then overflow against the
+// rest): a tile that holds one is computed by single FMAs, which leave masked keys out.
 // The order of channels within 16 (of a product over them) and of keys within 8 is such that fragments are 16-byte loads and
 // the scores' accumulators are the weights' operand.
 constexpr int kTileM = 64, kTileN = 32, kTileWarps = kTileM / 16;
@@ -145,7 +146,7 @@ __device__ __forceinline__ void in_parts(float x, uint32_t& hi, uint32_t& lo) {
 }
 __device__ __forceinline__ bool beyond_parts(float4 x) {
   auto size = [](float v) { return __float_as_int(v) & 0x7FFFFFFF; };
-  return max(max(size(x.x), size(x.y)), max(size(x.z), size(x.w))) >= 0x7F000000;
+  return max(max(size(x.x), size(x.y)), max(size(x.z), size(x.w))) >= 0x5F800000;
 }
 
 // Four channels of a row; channels behind D are 0.

@@ -702,9 +702,18 @@ def test_prompt_attention_at_the_ends_of_the_type(kd, dtype, n, dim):
     kd.prompt_attention(q, k, v, i32([0, n]), far)
     k[7, 0, 2] = float("inf")
     kd.prompt_attention(q, k, v, i32([0, n]), out)
-    assert torch.isnan(out[7:8, 0:2]).sum() == 0 and torch.isfinite(out).all()
-    close = (out.float() - far.float()).abs() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-5) * (far.float().abs() + 1)
-    assert close.all()
+    assert torch.isfinite(out).all()
+    limit = 2.0 ** -6 if dtype == torch.bfloat16 else 1e-5
+    assert ((out.float() - far.float()).abs() <= limit * (far.float().abs() + 1)).all()
+    # finite operands whose product is beyond the type, and one whose parts' products would be
+    q[:, :, 2] = -1e8
+    k[:, :, 2] = 0.0
+    k[7, 0, 2] = 1e20
+    kd.prompt_attention(q, k, v, i32([0, n]), far)
+    k[7, 0, 2] = 1e38
+    kd.prompt_attention(q, k, v, i32([0, n]), out)
+    assert torch.isfinite(out).all()
+    assert ((out.float() - far.float()).abs() <= limit * (far.float().abs() + 1)).all()
 
 
 def test_calls_on_a_stream_of_their_own(kd):
