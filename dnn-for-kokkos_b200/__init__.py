@@ -815,9 +815,16 @@ class KvPlan:
         self._check()
 
     def __setattr__(self, name, value):
+        if not hasattr(self, "seqs"):      # (the constructor fills the fields and checks them together)
+            object.__setattr__(self, name, value)
+            return
+        before = getattr(self, name, None)
         object.__setattr__(self, name, value)
-        if hasattr(self, "seqs"):      # complete: a tensor put in later is checked as the first ones were
-            self._check()
+        try:
+            self._check()      # a tensor put in later is checked as the first ones were, and one that fails does not stay
+        except Exception:
+            object.__setattr__(self, name, before)
+            raise
 
     def _check(self):
         tensors = (self.row_start, self.first, self.lens, self.state, self.slots, self.writes)
@@ -827,6 +834,8 @@ class KvPlan:
                 raise ValueError("KvPlan: tensors must be contiguous int32 on one device")
         if self.slots.dim() != 1 or self.first.dim() != 1:
             raise ValueError("KvPlan: first is [seqs] and slots [rows]")
+        if self.page not in (16, 32, 64, 128):
+            raise ValueError("KvPlan: pages hold 16, 32, 64 or 128 tokens")
         seqs, rows = self.first.shape[0], self.slots.shape[0]
         if self.row_start.shape != (seqs + 1,) or self.lens.shape != (seqs,) or self.state.shape != (4,) or \
                 self.writes.dim() != 2 or self.writes.shape[1] != 4 or self.writes.shape[0] < kv_writes(rows, seqs, self.page):

@@ -120,3 +120,17 @@ def test_python_checks(kd):
                  (q, k, k, rs, q)):
         with pytest.raises(ValueError):
             kd.prompt_attention(*args)
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("lens", lambda: torch.zeros(1, dtype=torch.int32)), ("lens", lambda: torch.zeros(2)), ("first", lambda: torch.zeros(3, dtype=torch.int32)),
+    ("state", lambda: torch.zeros(8, dtype=torch.int32)[::2]), ("slots", lambda: torch.zeros(400, dtype=torch.int32)),
+    ("writes", lambda: torch.zeros(3, 4, dtype=torch.int32)), ("row_start", lambda: None), ("page", lambda: 0), ("page", lambda: "16"),
+])
+def test_a_plan_keeps_its_tensors_when_a_new_one_is_refused(kd, name, bad):
+    plan = kd.KvPlan.empty(2, 5, 16, device="cpu")
+    before, seqs, rows = getattr(plan, name), plan.seqs, plan.rows
+    with pytest.raises((ValueError, AttributeError, TypeError, C.ArgumentError)):
+        setattr(plan, name, bad())
+    assert getattr(plan, name) is before and (plan.seqs, plan.rows) == (seqs, rows)
+    plan._check()
