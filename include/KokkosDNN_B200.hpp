@@ -303,12 +303,45 @@ void moe_ffn(const ExecSpace& space, const XView& X, const Table& gate, const Ta
 }
 
 
-// Attention over packed rows (kdnn_b200.h, "attention"). Row views are [rows, heads, dim] with unit stride in the last dimension;
+// Attention over packed rows (kdnn_b200.h, "attention"). Row views are [rows, heads, dim] with unit stride in the last dimension, a table
+// is [seqs, columns] with unit stride in its last; all others are dense. Views of another shape or stride throw std::invalid_argument.
 // plan: any struct with the views row_start, first, lens, state, slots, writes (int32; writes [entries, 4]) and `page`; cache: one
 // with k, v (int8 [pages, kv_heads, page, dim]) and k_scale, v_scale (float [pages, kv_heads]). In the reference: src/KokkosDNN_Attention.hpp,
 // src/KokkosDNN_KVCache.hpp.
+namespace attention {
+// Whether the last of a view's R dimensions is contiguous, and whether all are (strides of dimensions of one entry do not count).
+template <int R, class V>
+bool unit_stride(const V& v) { return v.extent(R - 1) <= 1 || v.stride(R - 1) == 1; }
+template <int R, class V>
+bool dense(const V& v) {
+  std::size_t at = 1;
+  for (int i = R - 1; i >= 0; --i) {
+    if (v.extent(i) == 0) return true;
+    if (v.extent(i) > 1 && static_cast<std::size_t>(v.stride(i)) != at) return false;
+    at *= v.extent(i);
+  }
+  return true;
+}
+inline void require(bool ok, const char* what, const char* why) {
+  if (!ok) throw std::invalid_argument(std::string(what) + ": " + why);
+}
+template <class Plan>
+void check_plan(const Plan& plan, std::size_t seqs, std::size_t rows, const char* what) {
+  require(plan.row_start.extent(0) == seqs + 1 && plan.first.extent(0) == seqs && plan.lens.extent(0) == seqs && plan.state.extent(0) == 4 &&
+              plan.slots.extent(0) == rows && plan.writes.extent(1) == 4, what, "dimension mismatch");
+  require(dense<1>(plan.row_start) && dense<1>(plan.first) && dense<1>(plan.lens) && dense<1>(plan.state) && dense<1>(plan.slots) &&
+              dense<2>(plan.writes), what, "the plan's views must be dense and LayoutRight");
+}
+}  // namespace attention
+
 template <class Cache>
 kdnn_b200_kv_cache kv_cache_of(const Cache& c) {
+  static_assert(sizeof(*c.k.data()) == 1 && sizeof(*c.v.data()) == 1, "codes are int8");
+  for (int i = 0; i < 4; ++i) attention::require(c.v.extent(i) == c.k.extent(i), "kv_cache", "k and v differ in shape");
+  for (int i = 0; i < 2; ++i)
+    attention::require(c.k_scale.extent(i) == c.k.extent(i) && c.v_scale.extent(i) == c.k.extent(i), "kv_cache", "scales must be [pages, kv_heads]");
+  attention::require(attention::dense<4>(c.k) && attention::dense<4>(c.v) && attention::dense<2>(c.k_scale) && attention::dense<2>(c.v_scale),
+                     "kv_cache", "views must be dense and LayoutRight");
   return kdnn_b200_kv_cache{reinterpret_cast<int8_t*>(c.k.data()), reinterpret_cast<int8_t*>(c.v.data()), c.k_scale.data(),
                             c.v_scale.data(), c.k.extent(0), c.k.extent(1), c.k.extent(2), c.k.extent(3)};
 }
@@ -317,9 +350,10 @@ template <class ExecSpace, class FView, class LView, class TView, class RView, c
 void kv_plan(const ExecSpace& space, const FView& fresh, const LView& lens, const TView& table, const RView& ring, const SView& state,
              const Plan& plan) {
   const std::size_t seqs = fresh.extent(0);
-  if (lens.extent(0) != seqs || table.extent(0) != seqs || plan.row_start.extent(0) != seqs + 1 || plan.first.extent(0) != seqs ||
-      plan.lens.extent(0) != seqs || state.extent(0) != 4 || plan.state.extent(0) != 4 || plan.writes.extent(1) != 4)
-    throw std::invalid_argument("kv_plan: dimension mismatch");
+  attention::require(lens.extent(0) == seqs && table.extent(0) == seqs && state.extent(0) == 4, "kv_plan", "dimension mismatch");
+  attention::check_plan(plan, seqs, plan.slots.extent(0), "kv_plan");
+  attention::require(attention::dense<1>(fresh) && attention::dense<1>(lens) && attention::dense<1>(ring) && attention::dense<1>(state) &&
+                         attention::unit_stride<2>(table), "kv_plan", "views must be dense, rows of the table contiguous");
   throw_on_error(kdnn_b200_kv_plan(fresh.data(), lens.data(), seqs, plan.page, plan.slots.extent(0), table.data(), table.stride(0),
                                    table.extent(1), ring.data(), ring.extent(0), state.data(), plan.row_start.data(),
                                    plan.first.data(), plan.lens.data(), plan.state.data(), plan.slots.data(), plan.writes.data(),
@@ -331,9 +365,10 @@ template <class ExecSpace, class XView, class Plan, class Cache>
 void kv_append(const ExecSpace& space, const XView& k, const XView& v, const Plan& plan, const Cache& cache) {
   using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(k.data())>::type>::type;
   const kdnn_b200_kv_cache c = kv_cache_of(cache);
-  if (k.extent(0) != plan.slots.extent(0) || v.extent(0) != k.extent(0) || k.extent(1) != c.kv_heads || v.extent(1) != c.kv_heads ||
-      k.extent(2) != c.dim || v.extent(2) != c.dim || c.page != static_cast<std::size_t>(plan.page))
-    throw std::invalid_argument("kv_append: dimension mismatch");
+  attention::check_plan(plan, plan.first.extent(0), k.extent(0), "kv_append");
+  attention::require(v.extent(0) == k.extent(0) && k.extent(1) == c.kv_heads && v.extent(1) == c.kv_heads && k.extent(2) == c.dim &&
+                         v.extent(2) == c.dim && c.page == static_cast<std::size_t>(plan.page), "kv_append", "dimension mismatch");
+  attention::require(attention::unit_stride<3>(k) && attention::unit_stride<3>(v), "kv_append", "k and v must have unit stride in their last dimension");
   throw_on_error(kdnn_b200_kv_append(k.data(), k.stride(0), k.stride(1), v.data(), v.stride(0), v.stride(1), scalar_tag<Scalar>(),
                                      k.extent(0), plan.writes.data(), plan.writes.extent(0), &c, StreamOf<ExecSpace>::get(space)),
                  "kv_append");
@@ -345,10 +380,11 @@ void kv_attention(const ExecSpace& space, const XView& q, const Plan& plan, cons
   using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(q.data())>::type>::type;
   const kdnn_b200_kv_cache c = kv_cache_of(cache);
   const std::size_t seqs = plan.first.extent(0);
-  if (out.extent(0) != q.extent(0) || out.extent(1) != q.extent(1) || q.extent(2) != c.dim || out.extent(2) != c.dim ||
-      plan.row_start.extent(0) != seqs + 1 || plan.lens.extent(0) != seqs || table.extent(0) != seqs ||
-      c.page != static_cast<std::size_t>(plan.page))
-    throw std::invalid_argument("kv_attention: dimension mismatch");
+  attention::check_plan(plan, seqs, q.extent(0), "kv_attention");
+  attention::require(out.extent(0) == q.extent(0) && out.extent(1) == q.extent(1) && q.extent(2) == c.dim && out.extent(2) == c.dim &&
+                         table.extent(0) == seqs && c.page == static_cast<std::size_t>(plan.page), "kv_attention", "dimension mismatch");
+  attention::require(attention::unit_stride<3>(q) && attention::unit_stride<3>(out) && attention::unit_stride<2>(table) &&
+                         attention::dense<1>(workspace), "kv_attention", "rows of q, out and the table must be contiguous, the workspace dense");
   throw_on_error(kdnn_b200_kv_attention(q.data(), q.stride(0), q.stride(1), scalar_tag<Scalar>(), q.extent(0), q.extent(1),
                                         plan.row_start.data(), plan.first.data(), plan.lens.data(), seqs, table.data(),
                                         table.stride(0), table.extent(1), &c, out.data(), out.stride(0), out.stride(1), scale, window,
@@ -360,10 +396,11 @@ template <class ExecSpace, class XView, class RView>
 void prompt_attention(const ExecSpace& space, const XView& q, const XView& k, const XView& v, const RView& row_start, const XView& out,
                       float scale, std::size_t window) {
   using Scalar = typename std::remove_cv<typename std::remove_pointer<decltype(q.data())>::type>::type;
-  if (k.extent(0) != q.extent(0) || v.extent(0) != q.extent(0) || out.extent(0) != q.extent(0) || out.extent(1) != q.extent(1) ||
-      v.extent(1) != k.extent(1) || k.extent(2) != q.extent(2) || v.extent(2) != q.extent(2) || out.extent(2) != q.extent(2) ||
-      row_start.extent(0) == 0)
-    throw std::invalid_argument("prompt_attention: dimension mismatch");
+  attention::require(k.extent(0) == q.extent(0) && v.extent(0) == q.extent(0) && out.extent(0) == q.extent(0) && out.extent(1) == q.extent(1) &&
+                         v.extent(1) == k.extent(1) && k.extent(2) == q.extent(2) && v.extent(2) == q.extent(2) && out.extent(2) == q.extent(2) &&
+                         row_start.extent(0) != 0, "prompt_attention", "dimension mismatch");
+  attention::require(attention::unit_stride<3>(q) && attention::unit_stride<3>(k) && attention::unit_stride<3>(v) && attention::unit_stride<3>(out) &&
+                         attention::dense<1>(row_start), "prompt_attention", "rows must have unit stride in their last dimension, row_start be dense");
   throw_on_error(kdnn_b200_prompt_attention(q.data(), q.stride(0), q.stride(1), k.data(), k.stride(0), k.stride(1), v.data(),
                                             v.stride(0), v.stride(1), scalar_tag<Scalar>(), q.extent(0), q.extent(1), k.extent(1),
                                             q.extent(2), row_start.data(), row_start.extent(0) - 1, out.data(), out.stride(0),
