@@ -608,14 +608,6 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 152);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 156);
   RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 160);   // what the TMA warp armed last
-  // The kernel behind this one may come onto the SMs when every CTA has said so, which it does when it has its tensor memory and not before: a CTA of that
-  // kernel that took the columns first would keep them until this grid is done, and this one would wait for them without end.
-  if (warp == L::kWarpMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    tc_before();
-    pdl_launch_dependents();
-  }
   if (threadIdx.x == 0) {
     for (const CUtensorMap* m : {&p.q, &p.k, &p.v}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     for (int i = 0; i < 2; ++i) {
@@ -636,16 +628,8 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   }
   pdl_wait();
   const int g = blockIdx.x % a.kv_heads;
-  auto give_back = [&]() {
-    if (warp == L::kWarpMma)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(L::kColumns) : "memory");
-  };
   PromptItem it;
-  if (!find_item<L::kThreads>(a, TILES * p.tokens, blockIdx.x / a.kv_heads, it)) {   // (its barriers publish the ones above)
-    tc_after();
-    give_back();
-    return;
-  }
+  if (!find_item<L::kThreads>(a, TILES * p.tokens, blockIdx.x / a.kv_heads, it)) return;   // (its barriers publish the ones above)
   // tokens [t0, t0 + tokens) and [t0 + tokens, ...) of the sequence; keys from `beg` on, 128 at a time
   const int t0 = it.part * TILES * p.tokens;
   const int beg = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
@@ -667,7 +651,14 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     load(base + L::kv + st * L::kOperand, i & 1 ? &p.v : &p.k, g, it.row0 + beg + (i >> 1) * kPtKeys, kPtHalf, full(st));
     armed.arm(st, ph);
   };
-  if (warp == L::kWarpTma) {
+  if (warp == L::kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // The kernel behind this one may come onto the SMs when every CTA has said so or is done. A CTA says so when it has its tensor memory and not
+    // before: a CTA of that kernel that took the columns first would keep them until this grid is done, and this one would wait for them
+    // without end. (Said at the top, with the allocation before it, every CTA began with the allocation's time: 12 ragged prompts 63.9 us, 62.7.)
+    pdl_launch_dependents();
+  } else if (warp == L::kWarpTma) {
     if (lane == 0) {
       load_queries(0);
       for (int i = 0; i < min(L::kStages, 2 * steps); ++i) {
@@ -914,7 +905,8 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     }
     __syncthreads();
   }
-  give_back();
+  if (warp == L::kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kColumns) : "memory");
 }
 
 static bool encode_heads(CUtensorMap* map, const void* x, size_t ld, size_t hd, int rows, int heads, int dim, int box_heads, int box_rows) {
