@@ -407,8 +407,8 @@ int kdnn_b200_quant_gemv_fp(uint32_t ggml_type, const void* w, size_t rows, size
 
 /* ---- attention: paged 8-bit cache and packed prompts ---------------------------------------------------
  * What stands between the projections of a decoder layer. Rows of a step are PACKED: the new tokens of sequence b are
- * rows row_start[b] .. row_start[b + 1] of q, k, v and out, in order. Rows behind the last sequence are neither read nor
- * written. Lengths, tables and plans live on the device; nothing here waits for the host, so a step can be captured into
+ * rows row_start[b] .. row_start[b + 1] of q, k, v and out, in order. Rows behind the last sequence are not written, and
+ * what they hold reaches no result. Lengths, tables and plans live on the device; nothing here waits for the host, so a step can be captured into
  * a graph once and replayed while lengths change. In the reference: src/KokkosDNN_Attention.hpp (causal grouped-query,
  * sliding window, int8 cache), src/KokkosDNN_KVCache.hpp. */
 

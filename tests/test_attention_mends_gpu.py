@@ -29,3 +29,87 @@ def test_prompts_behind_one_another(kd):
     for q, k, v, _, starts, out in made:
         check_prompt(q, k, v, out, starts, 0, torch.bfloat16)
         assert (out[starts[-1]:] == 777.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,dim,lens,window", [
+    (32, 8, 128, [77], 0), (8, 2, 64, [300, 5, 130], 0), (4, 4, 128, [700], 0), (8, 8, 64, [600, 333], 100), (1, 1, 72, [129, 128, 127], 1),
+    (12, 4, 96, [900], 500), (16, 2, 256, [500, 20], 0), (6, 6, 256, [400], 60), (16, 1, 128, [1500, 300, 800], 0), (64, 1, 64, [100], 7),
+    (32, 8, 128, [2000, 900], 0), (20, 4, 40, [1500], 333),
+])
+def test_prompt_attention_meets_what_is_not_finite_where_it_is_seen_and_nowhere_else(kd, dtype, heads, kv, dim, lens, window):
+    """Every result is what the formula gives: infinities of one sign stay, others are NaN, for the rows that see them; all else is the
+    attention over the finite values. (Scores are ordinary, so every weight is positive in the kernels too.)"""
+    starts = [2]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    rows = starts[-1] + 40
+    q, k, v = rows_of(rows, heads, dim, dtype, 1), rows_of(rows, kv, dim, dtype, 2), rows_of(rows, kv, dim, dtype, 3)
+    g = torch.Generator(device="cuda").manual_seed(dim + len(lens))
+    kind = torch.tensor([float("nan"), float("inf"), float("-inf")], device="cuda", dtype=dtype)
+    few = torch.rand(rows, kv, dim, device="cuda", generator=g) < 4.0 / (sum(lens) * dim)       # about four per head
+    few[starts[-1]:] = True
+    few[:2] = True
+    for s in starts[1:-1]:
+        few[s - 1, 0, 0] = few[s, -1, 3] = True                                                # at the ends of sequences
+    v0 = torch.where(few, 0.0, v)
+    v = torch.where(few, kind[torch.randint(0, 3, v.shape, device="cuda", generator=g)], v)
+    k0 = k.clone()
+    lost = [(b, n - n // 3) for b, n in enumerate(lens) if n > 60]                            # a key that is NaN, of the last head
+    for b, i in lost:
+        k[starts[b] + i, -1, 1] = float("nan")
+    k[starts[-1]:], k[:2], q[starts[-1]:] = float("nan"), float("inf"), float("nan")
+    out = torch.full_like(q, 777.0)
+    kd.prompt_attention(q, k, v, i32(starts), out, window=window)
+    assert (out[:2] == 777.0).all() and (out[starts[-1]:] == 777.0).all()
+    G, clean = heads // kv, out.clone()
+    for b, n in enumerate(lens):
+        part = slice(starts[b], starts[b + 1])
+        i = torch.arange(n, device="cuda")
+        keep = i[None, :] <= i[:, None]
+        if window:
+            keep &= i[None, :] > i[:, None] - window
+        nan, up, down = (torch.einsum("nt,tgd->ngd", keep.float(), m[part].float()) > 0 for m in (torch.isnan(v), v == float("inf"), v == float("-inf")))
+        nan |= up & down
+        for c, at in lost:
+            if c == b:
+                nan[:, -1] |= keep[:, at, None]
+        nan, up, down = (m.repeat_interleave(G, 1) for m in (nan, up, down))
+        got = out[part]
+        assert torch.equal(torch.isnan(got), nan)
+        assert (got[up & ~nan] == float("inf")).all() and (got[down & ~nan] == float("-inf")).all()
+        lone = nan | up | down
+        clean[part] = torch.where(lone, 0.0, got)
+        # the finite ones by the ordinary bound
+        want = torch.empty_like(out[part])
+        kd.prompt_attention(q[part], k0[part], v0[part], i32([0, n]), want, window=window)
+        check_prompt(q[part], k0[part], v0[part], torch.where(lone, want, got), [0, n], window, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prompt_attention_takes_no_longer_for_what_is_not_finite(kd, dtype):
+    """A row that meets NaN or infinity is not computed on another, slower way."""
+    n = 2500
+    q, k, v = rows_of(n + 30, 16, 128, dtype, 1), rows_of(n + 30, 4, 128, dtype, 2), rows_of(n + 30, 4, 128, dtype, 3)
+    out, starts = torch.empty_like(q), i32([0, n])
+
+    def time_of():
+        best = 1e9
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            kd.prompt_attention(q, k, v, starts, out)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    clean = time_of()
+    k[n:], v[n:] = float("nan"), float("inf")
+    behind = time_of()
+    v[n // 2, 1, 7] = float("nan")
+    one = time_of()
+    v[n // 2:] = float("nan")
+    half = time_of()
+    limit = 5 * clean + 0.1      # (fp32 tiles that hold one are computed without tensor cores)
+    assert max(behind, one, half) < limit, (clean, behind, one, half)
