@@ -78,6 +78,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, long long per, int 
 // The order of channels within 16 (of a product over them) and of keys within 8 is such that fragments are 16-byte loads and
 // the scores' accumulators are the weights' operand.
 constexpr int kTileM = 64, kTileN = 32, kTileWarps = kTileM / 16;
+constexpr float kTileDown = 0x1p-40f;
 template <int DM, int GROUPS>
 struct TileShape {
   static constexpr int kKeys = kTileN * GROUPS, kThreads = kTileWarps * 32 * GROUPS;
@@ -150,6 +151,10 @@ __global__ void __launch_bounds__(kTileWarps * 32 * GROUPS, GROUPS == 2 ? 128 / 
   int hi[2], lo[2];
   float m[2], l[2];
   float o[DM / 8][4];          // [4 i + e]: channels 32 i + 8 c + e and + 4 of row g, then of row g + 8
+  // Set by the first tile that holds values from 2^64 on: from there on all weights are kTileDown times as large, so that their sums stay finite.
+  // (Kept here, as there is no register left: 1500 tokens, 16 / 8 heads of 64 151 us, 160 with a flag in one.)
+  __shared__ int s_large;
+  if (threadIdx.x == 0) s_large = 0;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int pos = tok0 + q_at(16 * w + lg + 8 * r) / G;
@@ -219,6 +224,20 @@ __global__ void __launch_bounds__(kTileWarps * 32 * GROUPS, GROUPS == 2 ? 128 / 
       odd |= beyond_parts(*reinterpret_cast<const float4*>(share_v(buf) + RP * i * S::kVPitch));
     }
     odd = __syncthreads_or(odd);
+    if (odd) {
+      const bool first = s_large == 0;
+      __syncthreads();      // everybody has read it
+      s_large = 1;
+      if (first) {
+#pragma unroll
+        for (int i = 0; i < DM / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] *= kTileDown;
+        l[0] *= kTileDown;
+        l[1] *= kTileDown;
+      }
+    }
+    const bool large = s_large != 0;
     const int k0 = at + group * kTileN;      // this group's keys
     if (k0 > w_hi || k0 + kTileN <= see_beg) continue;
     const float *sk = kv + buf * S::kKv + group * kTileN * S::kKPitch;
@@ -318,6 +337,7 @@ __global__ void __launch_bounds__(kTileWarps * 32 * GROUPS, GROUPS == 2 ? 128 / 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[j][e] = exp2f(s[j][e] - ref[e >> 1]);
+        if (large) s[j][e] *= kTileDown;
         l[e >> 1] += s[j][e];
       }
 #pragma unroll
@@ -456,6 +476,9 @@ static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
 
 // ---- tcgen05 tiles ----------------------------------------------------------------------------------------------------------
 constexpr int kPtKeys = 128, kPtEdges = 5;
+// Weights are 2^(score - reference - kPtDown), so that sums of values near the largest number stay finite (up to 2^16 keys whose scores are all
+// 2^8 above the reference, 2^24 at it); in return values below 2^-102 lose bits.
+constexpr float kPtDown = 24.0f;
 constexpr uint32_t kPtHalf = 128 * 128;     // 128 rows of 64 channels, 128-byte swizzle
 
 // TILES: query tiles of a CTA. Two share every key and value and keep the tensor cores busy in turn; one is for calls that would leave SMs idle.
@@ -742,7 +765,7 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
             }
           }
         }
-        const float nm = m == -INFINITY ? 0.0f : -m * c;
+        const float nm = m == -INFINITY ? 0.0f : -m * c - kPtDown;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t w[32];

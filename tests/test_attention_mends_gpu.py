@@ -113,3 +113,19 @@ def test_prompt_attention_takes_no_longer_for_what_is_not_finite(kd, dtype):
     half = time_of()
     limit = 5 * clean + 0.1      # (fp32 tiles that hold one are computed without tensor cores)
     assert max(behind, one, half) < limit, (clean, behind, one, half)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,dim,lens,window", [(8, 2, 128, [20, 300], 0), (8, 8, 64, [2500], 0), (4, 2, 256, [700], 100), (16, 4, 96, [900, 1], 0)])
+@pytest.mark.parametrize("size", [3e38, 1e36, 1e20])
+def test_prompt_attention_of_values_near_the_largest_number(kd, dtype, heads, kv, dim, lens, window, size):
+    """A mean of finite values is finite: of one sign, of both, and of a few large ones among ordinary ones."""
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    rows = starts[-1]
+    q, k, v = rows_of(rows, heads, dim, dtype, 1), rows_of(rows, kv, dim, dtype, 2), rows_of(rows, kv, dim, dtype, 3)
+    out = torch.empty_like(q)
+    for large in (torch.full_like(v, size), torch.where(v > 0, size, -size / 2).to(dtype), torch.where(v > 2.5, size, v).to(dtype)):
+        kd.prompt_attention(q, k, large, i32(starts), out, window=window)
+        check_prompt(q, k, large, out, starts, window, dtype)
