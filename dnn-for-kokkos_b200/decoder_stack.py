@@ -14,7 +14,7 @@ The reference's models run the same order of operators (models/lfm2_5/KokkosDNN_
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, Optional
+from typing import Optional
 
 import torch
 
@@ -35,9 +35,54 @@ class AttentionConfig:
     longest: int = 8192      # tokens of a sequence at most
 
 
+class StepBuffers:
+    """Plan, activations and workspaces of steps of up to ``capacity`` rows of one stack. A captured step has a set of its own, which lives
+    as long as its graph; all others share the stack's. Steps of one stack must not overlap, whatever sets and streams they use: the
+    cache and its bookkeeping are one."""
+
+    def __init__(self, stack: "DecoderStack", capacity: int):
+        kd, a, c, dev = stack.kd, stack.attn, stack.cfg, stack.dev
+        self.kd, self.cfg, self.seqs, self.attn, self.capacity, self.rows = kd, c, a.seqs, stack.attn_workspace, capacity, -1
+        self.stream = torch.cuda.current_stream(dev)
+
+        def rows_of(n, dtype=torch.bfloat16):
+            return torch.empty((capacity, n), dtype=dtype, device=dev)
+        self.plan = kd.KvPlan.empty(a.seqs, capacity, a.page, dev)
+        self.plan.lens, self.plan.state = stack.lens, stack.state     # the pool moves from step to step in place
+        self.qkv, self.o, self.x = rows_of(stack.width), rows_of(a.heads * a.dim), rows_of(c.hidden)
+        self.y, self.zero = rows_of(c.hidden, torch.float32), torch.zeros((capacity, c.hidden), dtype=torch.float32, device=dev)
+        self.gemm = torch.empty(max(kd.quant_gemm_workspace_bytes(capacity, n) for n in (c.hidden, a.heads * a.dim)), dtype=torch.uint8, device=dev)
+        self.moe = torch.zeros(self._moe_bytes(capacity), dtype=torch.uint8, device=dev)
+        self._moe_rows = capacity
+
+    def _moe_bytes(self, rows: int) -> int:
+        c = self.cfg
+        return self.kd.moe_block_workspace_bytes(rows, 1, c.top_k, c.hidden, c.ffn, c.experts, True)
+
+    def tensors(self):
+        p = self.plan
+        return (p.row_start, p.first, p.slots, p.writes, self.qkv, self.o, self.x, self.y, self.zero, self.gemm, self.moe)
+
+    def of(self, rows: int) -> dict:
+        """Views of ``rows`` rows."""
+        if rows > self.capacity:
+            raise ValueError(f"StepBuffers: {rows} rows in buffers of {self.capacity}")
+        if rows != self.rows:
+            p = self.plan
+            plan = p if rows == self.capacity else self.kd.KvPlan(p.row_start, p.first, p.lens, p.state, p.slots[:rows],
+                                                                  p.writes[:self.kd.kv_writes(rows, self.seqs, p.page)], p.page)
+            moe = self.moe[:self._moe_bytes(rows)]
+            if rows != self._moe_rows and rows > 0:      # the counters of the block lie elsewhere for another number of rows, and begin at 0
+                moe.zero_()
+                self._moe_rows = rows
+            self.rows, self._views = rows, dict(plan=plan, qkv=self.qkv[:rows], o=self.o[:rows], x=self.x[:rows], y=self.y[:rows],
+                                                zero=self.zero[:rows], gemm=self.gemm, attn=self.attn, moe=moe)
+        return self._views
+
+
 class DecoderStack:
     """``step`` runs one step of all sequences: prompts of those that begin, one or several tokens of those that go on. The
-    cache's bookkeeping (lengths, block table, free pages) stays on the device."""
+    cache's bookkeeping (lengths, block table, free pages) stays on the device. Steps must not overlap."""
 
     def __init__(self, kd, device, cfg: StackConfig, attn: AttentionConfig):
         if (attn.heads * attn.dim) % 256:
@@ -57,35 +102,36 @@ class DecoderStack:
         self.table = torch.full((a.seqs, -(-a.longest // a.page)), -1, **i32)
         self.ring = torch.arange(a.pages, **i32)
         self.state = torch.tensor([0, a.pages, 0, 0], **i32)
-        self._steps: Dict[int, dict] = {}
+        # (the same size for every number of rows)
+        self.attn_workspace = torch.empty(kd.kv_attention_workspace_bytes(1, a.seqs, a.heads, a.kv_heads, a.dim), dtype=torch.uint8, device=device)
+        self._buffers: Optional[StepBuffers] = None
+        self._captured = []
         torch.cuda.current_stream(device).synchronize()       # packed weights are complete before the first call
 
     def buffers(self, rows: int) -> dict:
-        """Plan, workspaces and activations of a step of `rows` rows, made once per size."""
-        if rows not in self._steps:
-            kd, a, c, dev = self.kd, self.attn, self.cfg, self.dev
+        """Plan, workspaces and activations of a step of ``rows`` rows: views of one set, as large as the largest step so far."""
+        if torch.cuda.is_current_stream_capturing():          # (a set of its own: another step's counters must not lie in it)
+            self._captured.append(StepBuffers(self, rows))
+            return self._captured[-1].of(rows)
+        stream, own = torch.cuda.current_stream(self.dev), self._buffers
+        if own is None or rows > own.capacity:
+            # a quarter more than before at least, so that slowly growing steps do not make a new set each
+            more = max(rows, own.capacity + own.capacity // 4 if own else 0)
+            self._buffers = own = None                        # (the old set goes first)
+            self._buffers = own = StepBuffers(self, -(-more // 64) * 64)
+        if own.stream != stream:
+            for t in own.tensors():
+                t.record_stream(stream)
+        return own.of(rows)
 
-            def rows_of(n, dtype=torch.bfloat16):
-                return torch.empty((rows, n), dtype=dtype, device=dev)
-            plan = kd.KvPlan.empty(a.seqs, rows, a.page, dev)
-            plan.lens, plan.state = self.lens, self.state     # the pool moves from step to step in place
-            self._steps[rows] = dict(
-                plan=plan, qkv=rows_of(self.width), o=rows_of(a.heads * a.dim), y=rows_of(c.hidden, torch.float32), x=rows_of(c.hidden),
-                gemm=torch.empty(max(kd.quant_gemm_workspace_bytes(rows, c.hidden), kd.quant_gemm_workspace_bytes(rows, a.heads * a.dim)),
-                                 dtype=torch.uint8, device=dev),
-                attn=torch.empty(kd.kv_attention_workspace_bytes(rows, a.seqs, a.heads, a.kv_heads, a.dim), dtype=torch.uint8, device=dev),
-                moe=torch.zeros(kd.moe_block_workspace_bytes(rows, 1, c.top_k, c.hidden, c.ffn, c.experts, True), dtype=torch.uint8,
-                                device=dev),
-                zero=torch.zeros((rows, c.hidden), dtype=torch.float32, device=dev))
-        return self._steps[rows]
-
-    def step(self, h: torch.Tensor, fresh: torch.Tensor, begin: bool = False) -> torch.Tensor:
+    def step(self, h: torch.Tensor, fresh: torch.Tensor, begin: bool = False, buffers: Optional[StepBuffers] = None) -> torch.Tensor:
         """The residual stream of the step's rows behind the last layer. ``h`` [rows, hidden], packed in the order of the
         sequences; ``fresh`` int32 [seqs] on the device: rows of each sequence, 0 for one that waits, -1 for one that has ended.
-        ``begin``: every sequence with rows begins with them (its prompt), so attention is among the step's rows alone."""
+        ``begin``: every sequence with rows begins with them (its prompt), so attention is among the step's rows alone.
+        ``buffers``: a set of the caller's own in place of the stack's."""
         kd, a, c = self.kd, self.attn, self.cfg
         rows = h.shape[0]
-        b = self.buffers(rows)
+        b = self.buffers(rows) if buffers is None else buffers.of(rows)
         plan, qkv = b["plan"], b["qkv"].view(rows, a.heads + 2 * a.kv_heads, a.dim)
         q, k, v = qkv[:, :a.heads], qkv[:, a.heads:a.heads + a.kv_heads], qkv[:, a.heads + a.kv_heads:]
         o = b["o"].view(rows, a.heads, a.dim)
@@ -114,11 +160,13 @@ class DecoderStack:
 
 
 def decode_graph(stack: DecoderStack, h: torch.Tensor, fresh: torch.Tensor, stream: Optional[torch.cuda.Stream] = None):
-    """(graph, result): one decode step captured; replay it after writing the next rows into ``h``. The stack must have run a step of
-    this size before (buffers and kernels are set up by it)."""
+    """(graph, result): one decode step captured; replay it after writing the next rows into ``h``. The stack must have run a step
+    before (kernels are set up by it). The graph has buffers of its own, which it keeps alive."""
     stream = stream or torch.cuda.Stream()
+    buffers = StepBuffers(stack, h.shape[0])
     torch.cuda.synchronize(h.device)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=stream):
-        out = stack.step(h, fresh)
+        out = stack.step(h, fresh, buffers=buffers)
+    graph.buffers, graph.inputs = buffers, (stack, h, fresh)
     return graph, out
