@@ -126,7 +126,8 @@ class DecoderStack:
 
     def step(self, h: torch.Tensor, fresh: torch.Tensor, begin: bool = False, buffers: Optional[StepBuffers] = None) -> torch.Tensor:
         """The residual stream of the step's rows behind the last layer. ``h`` [rows, hidden], packed in the order of the
-        sequences; ``fresh`` int32 [seqs] on the device: rows of each sequence, 0 for one that waits, -1 for one that has ended.
+        sequences; ``fresh`` int32 [seqs] on the device: rows of each sequence, 0 for one that waits, -1 for one that has ended. Rows
+        behind the last sequence meet no attention.
         ``begin``: every sequence with rows begins with them (its prompt), so attention is among the step's rows alone.
         ``buffers``: a set of the caller's own in place of the stack's."""
         kd, a, c = self.kd, self.attn, self.cfg
@@ -138,6 +139,7 @@ class DecoderStack:
         kd.kv_plan(fresh, self.lens, self.table, self.ring, self.state, plan)
         x = torch.empty_like(h)
         kd.residual_rmsnorm(h, b["zero"], x)
+        b["o"].zero_()      # rows behind the last sequence: attention leaves them as they are, in every layer
         for l in range(c.layers):
             kd.quant_gemm(x, self.qkv[l], b["qkv"], b["gemm"])
             kd.kv_append(k, v, plan, self.caches[l])

@@ -117,3 +117,21 @@ def test_a_step_captured_by_hand(kd):
         assert torch.equal(got, other.step(h, fresh))
         assert torch.equal(stack.step(rows(9, i), i32([4, 0, 5])), other.step(rows(9, i), i32([4, 0, 5])))
     assert kd.device_status() == 0
+
+
+def test_rows_behind_the_last_sequence_are_not_what_lay_in_memory(kd):
+    """A step with more rows than its sequences have: the rest of the rows meet an attention of 0, whatever steps came before."""
+    results = []
+    for before in (None, float("nan"), 1e30):
+        ds, stack = new_stack(kd)
+        stack.step(rows(40, 1), i32([20, 3, 17]), begin=True)
+        if before is not None:
+            for t in stack._buffers.tensors() if hasattr(stack._buffers, "tensors") else ():
+                if t.dtype == torch.bfloat16:
+                    t.fill_(before)
+        a = stack.step(rows(12, 5), i32([1, 0, 2]))
+        b = stack.step(rows(30, 6), i32([-1, 0, 0]))
+        c = stack.step(rows(50, 7), i32([33, 0, 0]), begin=True)
+        results.append(torch.cat([a, b, c]))
+        assert torch.isfinite(results[-1].float()).all()
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2]) and kd.device_status() == 0
