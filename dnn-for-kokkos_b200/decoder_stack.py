@@ -102,6 +102,7 @@ class DecoderStack:
         self.table = torch.full((a.seqs, -(-a.longest // a.page)), -1, **i32)
         self.ring = torch.arange(a.pages, **i32)
         self.state = torch.tensor([0, a.pages, 0, 0], **i32)
+        self.prefixes = torch.zeros((), **i32)
         # (the same size for every number of rows)
         self.attn_workspace = torch.empty(kd.kv_attention_workspace_bytes(1, a.seqs, a.heads, a.kv_heads, a.dim), dtype=torch.uint8, device=device)
         self._buffers: Optional[StepBuffers] = None
@@ -128,7 +129,8 @@ class DecoderStack:
         """The residual stream of the step's rows behind the last layer. ``h`` [rows, hidden], packed in the order of the
         sequences; ``fresh`` int32 [seqs] on the device: rows of each sequence, 0 for one that waits, -1 for one that has ended. Rows
         behind the last sequence meet no attention.
-        ``begin``: every sequence with rows begins with them (its prompt), so attention is among the step's rows alone.
+        ``begin``: every sequence with rows begins with them (its prompt), so attention is among the step's rows alone; a sequence that
+        holds tokens already would lose them, which ``prefixes_left_out`` counts.
         ``buffers``: a set of the caller's own in place of the stack's."""
         kd, a, c = self.kd, self.attn, self.cfg
         rows = h.shape[0]
@@ -137,6 +139,8 @@ class DecoderStack:
         q, k, v = qkv[:, :a.heads], qkv[:, a.heads:a.heads + a.kv_heads], qkv[:, a.heads + a.kv_heads:]
         o = b["o"].view(rows, a.heads, a.dim)
         kd.kv_plan(fresh, self.lens, self.table, self.ring, self.state, plan)
+        if begin:
+            torch.sum((plan.first > 0) & (fresh > 0), 0, dtype=torch.int32, out=self.prefixes)
         x = torch.empty_like(h)
         kd.residual_rmsnorm(h, b["zero"], x)
         b["o"].zero_()      # rows behind the last sequence: attention leaves them as they are, in every layer
@@ -159,6 +163,10 @@ class DecoderStack:
     def rows_without_place(self) -> int:
         """Rows of the last step that found no page (synchronises)."""
         return int(self.state[2])
+
+    def prefixes_left_out(self) -> int:
+        """Sequences that did not begin with the last ``begin`` step's rows, whose earlier tokens those rows have not met (synchronises)."""
+        return int(self.prefixes)
 
 
 def decode_graph(stack: DecoderStack, h: torch.Tensor, fresh: torch.Tensor, stream: Optional[torch.cuda.Stream] = None):

@@ -135,3 +135,15 @@ def test_rows_behind_the_last_sequence_are_not_what_lay_in_memory(kd):
         results.append(torch.cat([a, b, c]))
         assert torch.isfinite(results[-1].float()).all()
     assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2]) and kd.device_status() == 0
+
+
+def test_a_beginning_step_counts_the_sequences_that_do_not_begin(kd):
+    ds, stack = new_stack(kd)
+    stack.step(rows(40, 1), i32([20, 3, 17]), begin=True)
+    assert stack.prefixes_left_out() == 0
+    stack.step(rows(9, 2), i32([4, 0, 5]))
+    assert stack.prefixes_left_out() == 0                   # (attended to over the cache)
+    stack.step(rows(9, 3), i32([4, -1, 5]), begin=True)
+    assert stack.prefixes_left_out() == 2
+    stack.step(rows(7, 4), i32([0, 7, 0]), begin=True)
+    assert stack.prefixes_left_out() == 0
