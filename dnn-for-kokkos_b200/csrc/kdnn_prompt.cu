@@ -458,8 +458,11 @@ static cudaError_t launch_tile(const AttnArgs& a, unsigned ctas, cudaStream_t st
   if (e != cudaSuccess) return e;
   return launch_chained(prompt_tile_kernel<ST, DM, GROUPS>, dim3(ctas), dim3(S::kThreads), S::kFloats * 4, st, a);
 }
-// Two groups of warps where three CTAs per SM hold the call and its longest rows decide (1500 tokens, 16 / 8 heads of 64, window 512:
-// 72 us, 81 with one group), else one (4096 tokens, 16 / 4 heads of 128: 1323 us, 1569 with two).
+// Two groups of warps share a tile's keys where a call has few CTAs, so that its longest rows decide: up to three per SM for heads of up to 64 (two such
+// CTAs fit an SM), up to two and a half for heads of up to 128 (one fits, two of one group). fp32, us with two groups and with one:
+//   heads of 64: 152 CTAs (600 tokens) 49 and 51, 376 (1500) 143 and 153, 392 (three of 500) 65 and 74, 392 (twelve of 100) 35 and 29, 752 (1500) 219 and 213
+//   heads of 128: 152 CTAs 78 and 89, 304 (2400) 304 and 382, 304 (1200) 173 and 204, 368 (2900) 464 and 478, 376 (1500) 264 and 260,
+//   392 (three of 500) 127 and 115, 416 (four of 200) 78 and 74, 604 (1200) 321 and 282; short prompts alone lose: 240 (twelve of 100) 45 and 39
 template <class ST>
 static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
   const int G = a.heads / a.kv_heads;
@@ -468,7 +471,7 @@ static cudaError_t launch_tiles(const AttnArgs& a, cudaStream_t st) {
   if (all > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const unsigned ctas = static_cast<unsigned>(all);
   if constexpr (sizeof(ST) == 4) {
-    if (a.dim <= 128 && all <= 3LL * device_sm_count()) return a.dim <= 64 ? launch_tile<ST, 64, 2>(a, ctas, st) : launch_tile<ST, 128, 2>(a, ctas, st);
+    if (a.dim <= 128 && 2 * all <= (a.dim <= 64 ? 6LL : 5LL) * device_sm_count()) return a.dim <= 64 ? launch_tile<ST, 64, 2>(a, ctas, st) : launch_tile<ST, 128, 2>(a, ctas, st);
   }
   if (a.dim <= 64) return launch_tile<ST, 64, 1>(a, ctas, st);
   return a.dim <= 128 ? launch_tile<ST, 128, 1>(a, ctas, st) : launch_tile<ST, 256, 1>(a, ctas, st);

@@ -129,3 +129,12 @@ def test_prompt_attention_of_values_near_the_largest_number(kd, dtype, heads, kv
     for large in (torch.full_like(v, size), torch.where(v > 0, size, -size / 2).to(dtype), torch.where(v > 2.5, size, v).to(dtype)):
         kd.prompt_attention(q, k, large, i32(starts), out, window=window)
         check_prompt(q, k, large, out, starts, window, dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("lens", [[700], [720, 20], [850], [60] * 15])
+def test_prompt_attention_fp32_around_the_choice_of_groups(kd, dim, lens):
+    """Calls of 320 to 480 CTAs, on either side of where one or two groups of warps take a tile."""
+    from test_attention_gpu import prompt_case
+    prompt_case(kd, torch.float32, 32, 4, dim, lens, 0, seed=dim)
+    prompt_case(kd, torch.float32, 32, 4, dim, lens, 50, seed=dim + 1)
