@@ -17,10 +17,11 @@
 //    multiple of 2^-24), and the sums start from -128 sum(q); for O, whose sums run over the whole context, codes become
 //    fp16 exactly (1024 + code + 128 by a byte permutation, minus 1152). k order and channel order are permuted the same way on both sides of a product.
 //  * Weights: 2^(s + log2 b - m), one running reference for the values and one for the sum of weights, so that scales
-//    that lie far apart lose neither. References are whole numbers and move only when a score passes them by 8 (weights
-//    stay below 2^15 in fp16, and one below 2^-24, 2^-31 of the row's largest at the most, may vanish; every rescale is exact).
-//  * fp32 activations: q and the weights enter as two fp16 parts each (22 bits), and every tile's product is added to the sums
-//    by fp32 additions (the tensor core cuts instead of rounding).
+//    that lie far apart lose neither sum. References are whole numbers and move only when a score passes them by 8 (every rescale is
+//    exact). The product's weights stay below 2^15 in fp16, whose smallest step is 2^-24: a weight times its page's value scale is off by
+//    2^-31 of the row's largest such product at the most, beside fp16's 11 bits, and vanishes below that.
+//  * fp32 activations: q and the weights enter as two fp16 parts each (22 bits, on the same grid of 2^-24), and every tile's product is
+//    added to the sums by fp32 additions (the tensor core cuts instead of rounding).
 #include "kdnn_common.cuh"
 
 #include <string.h>

@@ -457,7 +457,9 @@ size_t kdnn_b200_kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t h
  * with no such token gives 0. The new rows themselves are read from the cache: append before this call. Tokens on a page
  * that the table does not hold (a number outside [0, pages), or beyond table_cols) are left out.
  * q, out [rows][heads][dim] Scalar with row and head pitches; out may be q. heads is a multiple of kv_heads. Calls that overlap need
- * workspaces of their own. A weight below 2^-31 of its row's largest may count as 0. seqs <= 8192. */
+ * workspaces of their own. Where the pages' value scales are alike, a weight below 2^-31 of its row's largest may count as 0; in general
+ * what is held to a step of 2^-31 of its row's largest is a weight times its page's value scale, so that a token of a page whose scale is
+ * 2^-31 of another visible one's may not count, whatever its weight. seqs <= 8192. */
 int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, size_t rows, size_t heads, const int32_t* row_start,
                            const int32_t* first, const int32_t* lens, size_t seqs, const int32_t* table, size_t ldt,
                            size_t table_cols, const kdnn_b200_kv_cache* cache, void* out, size_t ldo, size_t hdo, float scale,

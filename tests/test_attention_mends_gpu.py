@@ -3,7 +3,7 @@ those of test_attention_gpu.py."""
 import pytest
 import torch
 
-from test_attention_gpu import check_prompt, i32, rows_of
+from test_attention_gpu import F32, OUT, cache_case, check_prompt, i32, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,42 @@ def test_prompt_attention_fp32_around_the_choice_of_groups(kd, dim, lens):
     from test_attention_gpu import prompt_case
     prompt_case(kd, torch.float32, 32, 4, dim, lens, 0, seed=dim)
     prompt_case(kd, torch.float32, 32, 4, dim, lens, 50, seed=dim + 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("apart", [4, 20, 28, 40, 90])
+@pytest.mark.parametrize("heads,kv,dim,page,fresh,lens", [(8, 2, 128, 16, [1, 2], [100, 40]), (4, 1, 64, 64, [1], [3000]), (6, 2, 256, 32, [5], [200])])
+def test_cache_attention_of_scales_that_lie_far_apart(kd, dtype, apart, heads, kv, dim, page, fresh, lens):
+    """Every second page's values are 2^-apart of the others', and the others hold codes of 0 in half of the channels: there the small
+    pages alone are seen. A weight times scale is off by its rounding (fp16 2^-11, in two parts 2^-22) and by 2^-31 of the row's largest
+    one, which meet the codes; a score by the roundings that the ordinary bound counts."""
+    plan, table, cache, q, out, ws = cache_case(kd, dtype, heads, kv, dim, page, fresh, lens, 0)
+    cache.v_scale.fill_(0.5)
+    for row in table.tolist():
+        for i, p in enumerate(row):
+            if 0 <= p < cache.pages:
+                if i % 2:
+                    cache.v_scale[p] = 0.5 * 2.0 ** -apart
+                else:
+                    cache.v[p, :, :, : dim // 2] = 0
+    kd.kv_attention(q, plan, table, cache, out, ws)
+    rs, G = plan.row_start.tolist(), heads // kv
+    for b in range(len(fresh)):
+        n, T = rs[b + 1] - rs[b], plan.lens[b].item()
+        pg = table[b, :-(-T // page)].long()
+        k = (cache.k[pg].double() * cache.k_scale[pg].double()[..., None, None]).transpose(1, 2).reshape(-1, kv, dim)[:T].repeat_interleave(G, 1)
+        code = cache.v[pg].double().transpose(1, 2).reshape(-1, kv, dim)[:T].repeat_interleave(G, 1)
+        scale = cache.v_scale[pg].double().repeat_interleave(page, 0)[:T].repeat_interleave(G, 1)
+        x = q[rs[b]:rs[b + 1]].double()
+        keep = torch.arange(T, device="cuda")[None, :] <= torch.arange(lens[b], lens[b] + n, device="cuda")[:, None]
+        s = (torch.einsum("nhd,thd->hnt", x, k) * dim ** -0.5).masked_fill(~keep, float("-inf"))
+        big = (torch.einsum("nhd,thd->hnt", x.abs(), k.abs()) * dim ** -0.5).masked_fill(~keep, 0.0).amax(-1).T[..., None]
+        p = torch.softmax(s, -1)
+        pb = p * scale.T[:, None]                                                     # weight times scale
+        want, A = torch.einsum("hnt,thd->nhd", pb, code), torch.einsum("hnt,thd->nhd", pb, code.abs())
+        floor = pb.amax(-1).T[..., None] * torch.einsum("nt,thd->nhd", keep.double(), code.abs()) * 2.0 ** -31
+        operand, weight = (0.0, 2.0 ** -11) if dtype == torch.bfloat16 else (2.0 ** -22, 2.0 ** -22)
+        keys = keep.sum(-1).double()[:, None, None]
+        bound = A * (2 * big * (2 * operand + (dim + 8) * F32) + 2 * weight + (8 + keys.sqrt() * 4) * F32) + want.abs() * OUT[dtype] * 1.01 + floor + 1e-38
+        off = (out[rs[b]:rs[b + 1]].double() - want).abs()
+        assert (off <= bound).all(), f"{(off / bound).max().item():.3g} of the bound"
