@@ -127,6 +127,30 @@ void* mapped_host_pointer(const void* host) {
 bool page_ok(size_t page) { return page == 16 || page == 32 || page == 64 || page == 128; }
 // rows of `heads` heads of `dim` elements: nothing of a row lies behind its pitch
 bool heads_fit(size_t ld, size_t hd, size_t heads, size_t dim) { return heads > 0 && hd >= dim && (heads - 1) <= (ld - dim) / hd && ld >= dim; }
+// Rows [rows][heads][dim] of an attention call, and whether two of them have an element in common: a result may lie beside its
+// inputs in one buffer, rows between rows or heads between heads.
+struct HeadRows { const void* p; size_t ld, hd, heads; };
+bool rows_meet(const HeadRows& x, const HeadRows& y, size_t rows, size_t dim, int scalar) {
+  const size_t e = scalar == KDNN_F32 ? 4 : 2, w = dim * e, hx = x.hd * e, hy = y.hd * e, lx = x.ld * e, ly = y.ld * e;
+  const size_t wx = (x.heads - 1) * hx + w, wy = (y.heads - 1) * hy + w;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+  // with one pitch the places repeat from row to row: the first ones that meet tell
+  const size_t from = b > a + wx ? (b - a - wx) / lx : 0, to = lx == ly && rows > from + 4 ? from + 4 : rows;
+  for (size_t r = from; r < to; ++r) {
+    const uintptr_t x0 = a + r * lx;
+    if (x0 >= b + (rows - 1) * ly + wy) break;
+    if (x0 + wx <= b) continue;
+    for (size_t s = x0 >= b + wy ? (x0 - b - wy) / ly + 1 : 0; s < rows && b + s * ly < x0 + wx; ++s) {
+      const uintptr_t y0 = b + s * ly;
+      for (size_t i = 0, j = 0; i < x.heads && j < y.heads;) {
+        const uintptr_t p = x0 + i * hx, q = y0 + j * hy;
+        if (p < q + w && q < p + w) return true;
+        if (p < q) ++i; else ++j;
+      }
+    }
+  }
+  return false;
+}
 const char* cache_fault(const kdnn_b200_kv_cache* c) {
   if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return "null cache";
   if (!page_ok(c->page)) return "pages hold 16, 32, 64 or 128 tokens";
@@ -635,6 +659,8 @@ int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, si
   if (workspace_bytes < kdnn::kv_attention_workspace_bytes(rows, seqs, heads, cache->kv_heads, cache->dim) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(KDNN_ERR_INVALID, "kv_attention: workspace too small or not 256-byte aligned");
+  if (!(out == q && ldo == ldq && hdo == hdq) && rows_meet({out, ldo, hdo, heads}, {q, ldq, hdq, heads}, rows, cache->dim, scalar))
+    return fail(KDNN_ERR_INVALID, "kv_attention: out must be q or not overlap it");
   kdnn::AttnArgs a{};
   a.q = q; a.ldq = ldq; a.hdq = hdq; a.out = out; a.ldo = ldo; a.hdo = hdo; a.scalar = scalar;
   a.rows = static_cast<int>(rows); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(cache->kv_heads);
@@ -656,7 +682,10 @@ int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void
     return fail(KDNN_ERR_INVALID, "prompt_attention: dimension mismatch");
   if (rows > static_cast<size_t>(INT_MAX) / heads || seqs > 8192) return fail(KDNN_ERR_INVALID, "prompt_attention: too many rows or sequences");
   if (!q || !k || !v || !row_start || !out) return fail(KDNN_ERR_INVALID, "prompt_attention: null argument");
-  if (out == q || out == k || out == v) return fail(KDNN_ERR_INVALID, "prompt_attention: out must not overlap q, k or v");
+  const HeadRows to{out, ldo, hdo, heads};
+  if (rows_meet(to, {q, ldq, hdq, heads}, rows, dim, scalar) || rows_meet(to, {k, ldk, hdk, kv_heads}, rows, dim, scalar) ||
+      rows_meet(to, {v, ldv, hdv, kv_heads}, rows, dim, scalar))
+    return fail(KDNN_ERR_INVALID, "prompt_attention: out must not overlap q, k or v");
   kdnn::AttnArgs a{};
   a.q = q; a.ldq = ldq; a.hdq = hdq; a.k = k; a.ldk = ldk; a.hdk = hdk; a.v = v; a.ldv = ldv; a.hdv = hdv;
   a.out = out; a.ldo = ldo; a.hdo = hdo; a.scalar = scalar;

@@ -456,7 +456,7 @@ size_t kdnn_b200_kv_attention_workspace_bytes(size_t rows, size_t seqs, size_t h
  * kv_heads): 0 <= j < lens[b], j <= pos, and j > pos - window where window > 0; pos = first[b] + r - row_start[b]. A row
  * with no such token gives 0. The new rows themselves are read from the cache: append before this call. Tokens on a page
  * that the table does not hold (a number outside [0, pages), or beyond table_cols) are left out.
- * q, out [rows][heads][dim] Scalar with row and head pitches; out may be q. heads is a multiple of kv_heads. Calls that overlap need
+ * q, out [rows][heads][dim] Scalar with row and head pitches; out is q (same pitches) or shares no element with it. heads is a multiple of kv_heads. Calls that overlap need
  * workspaces of their own. Where the pages' value scales are alike, a weight below 2^-31 of its row's largest may count as 0; in general
  * what is held to a step of 2^-31 of its row's largest is a weight times its page's value scale, so that a token of a page whose scale is
  * 2^-31 of another visible one's may not count, whatever its weight. seqs <= 8192. */
@@ -468,8 +468,8 @@ int kdnn_b200_kv_attention(const void* q, size_t ldq, size_t hdq, int scalar, si
 /* Causal grouped attention over packed prompts: row r of sequence b attends to the rows row_start[b] .. r (with window > 0:
  * the last `window` of them). q, out [rows][heads][dim], k, v [rows][kv_heads][dim] Scalar with row and head pitches in
  * elements; dim a multiple of 8 up to 256. Values in masked places (later rows, other sequences) do not reach the result,
- * infinities and NaN included. Rows outside [row_start[0], row_start[seqs]) are left as they were. out must not overlap
- * q, k or v. bf16 rows that are 16-byte aligned (groups of up to 128 heads, scale > 0) run on tcgen05 tiles, weights rounded to bf16, sums
+ * infinities and NaN included. Rows outside [row_start[0], row_start[seqs]) are left as they were. out must share no element with
+ * q, k or v (it may lie between their rows or heads). bf16 rows that are 16-byte aligned (groups of up to 128 heads, scale > 0) run on tcgen05 tiles, weights rounded to bf16, sums
  * fp32; the rest on mma.sync tiles with two tf32 parts of each number (about 2^-21 of a product is left out). seqs <= 8192. */
 int kdnn_b200_prompt_attention(const void* q, size_t ldq, size_t hdq, const void* k, size_t ldk, size_t hdk, const void* v,
                                size_t ldv, size_t hdv, int scalar, size_t rows, size_t heads, size_t kv_heads, size_t dim,

@@ -134,3 +134,38 @@ def test_a_plan_keeps_its_tensors_when_a_new_one_is_refused(kd, name, bad):
         setattr(plan, name, bad())
     assert getattr(plan, name) is before and (plan.seqs, plan.rows) == (seqs, rows)
     plan._check()
+
+
+def attention_calls(kd):
+    """(name, call(out=..., **pitches)) of both attention calls on fake rows: q at 0x100000 [rows 6, heads 4, dim 64] fp32."""
+    def prompt(**kw):
+        a = dict(dict(q=0x100000, ldq=256, hdq=64, k=0x200000, ldk=128, hdk=64, v=0x300000, ldv=128, hdv=64, scalar=0, rows=6, heads=4, kv_heads=2,
+                      dim=64, row_start=P, seqs=2, out=0x400000, ldo=256, hdo=64, scale=0.1, window=0), **kw)
+        return kd.lib.kdnn_b200_prompt_attention(*a.values(), None)
+
+    def cached(**kw):
+        a = dict(dict(q=0x100000, ldq=256, hdq=64, scalar=0, rows=6, heads=4, row_start=P, first=P, lens=P, seqs=2, table=P, ldt=8, cols=8,
+                      cache=C.byref(_cache(kd, dim=64)), out=0x400000, ldo=256, hdo=64, scale=0.1, window=0, ws=P, ws_bytes=1 << 40), **kw)
+        return kd.lib.kdnn_b200_kv_attention(*a.values(), None)
+    return prompt, cached
+
+
+def test_results_that_overlap_their_inputs_are_refused(kd):
+    """Every place of the result that shares an element with an input, by brute force, is refused; what is merely beside one is for the GPU
+    tests, as it would be launched."""
+    q, row, head = 0x100000, 1024, 256
+    prompt, cached = attention_calls(kd)
+    overlaps = [dict(out=q + 4), dict(out=q + head), dict(out=q - 4 * 1), dict(out=q + 5 * row), dict(out=q - 5 * row), dict(out=q + 5 * row + 3 * head),
+                dict(out=q - 3 * row, ldo=512), dict(out=q, ldo=512), dict(out=q - 6 * row + 4), dict(out=q - 8 * 2048 // 2, ldo=2048, hdo=512),
+                # heads twice as far apart, the result half a head off
+                dict(ldq=512, hdq=128, ldo=512, hdo=128, out=q + 128), dict(ldq=512, hdq=128, ldo=512, hdo=128, out=q + 3 * 512 + 384)]
+    for kw in overlaps:
+        a = dict(dict(ldq=256, hdq=64, ldo=256, hdo=64), **kw)
+        mine = {q + 4 * (r * a["ldq"] + h * a["hdq"] + d) for r in range(6) for h in range(4) for d in range(64)}
+        outs = {a["out"] + 4 * (r * a["ldo"] + h * a["hdo"] + d) for r in range(6) for h in range(4) for d in range(64)}
+        if not mine & outs:
+            continue
+        assert prompt(**kw) == kd.KDNN_ERR_INVALID and "overlap" in kd.last_error(), kw
+        assert cached(**kw) == kd.KDNN_ERR_INVALID and "overlap" in kd.last_error(), kw
+    for kw in (dict(out=0x200000 + 512), dict(out=0x300000 - 1024), dict(out=0x300000, ldo=512)):      # k and v
+        assert prompt(**kw) == kd.KDNN_ERR_INVALID and "overlap" in kd.last_error(), kw

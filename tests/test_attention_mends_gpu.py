@@ -177,3 +177,42 @@ def test_cache_attention_of_scales_that_lie_far_apart(kd, dtype, apart, heads, k
         bound = A * (2 * big * (2 * operand + (dim + 8) * F32) + 2 * weight + (8 + keys.sqrt() * 4) * F32) + want.abs() * OUT[dtype] * 1.01 + floor + 1e-38
         off = (out[rs[b]:rs[b + 1]].double() - want).abs()
         assert (off <= bound).all(), f"{(off / bound).max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_results_beside_their_inputs_in_one_buffer(kd, dtype):
+    """Rows between rows and heads between heads: no element is shared, so the calls are taken, and nothing else is written."""
+    n, H, KV, D = 90, 8, 2, 64
+    # q, k, v and the result side by side in every row
+    buf = rows_of(n, 2 * H + 2 * KV, D, dtype, 1)
+    q, k, v, out = buf[:, :H], buf[:, H:H + KV], buf[:, H + KV:H + 2 * KV], buf[:, H + 2 * KV:]
+    kept = buf[:, :H + 2 * KV].clone()
+    kd.prompt_attention(q, k, v, i32([0, 40, n]), out)
+    check_prompt(q, k, v, out, [0, 40, n], 0, dtype)
+    assert torch.equal(kept, buf[:, :H + 2 * KV])
+    # every second head; and rows of the result behind those of q
+    pairs = rows_of(n, 2 * H, D, dtype, 2)
+    q, out = pairs[:, ::2], pairs[:, 1::2]
+    kept = q.clone()
+    k, v = k.contiguous(), v.contiguous()
+    kd.prompt_attention(q, k, v, i32([0, 40, n]), out)
+    check_prompt(kept, k, v, out, [0, 40, n], 0, dtype)
+    assert torch.equal(kept, q)
+    both = rows_of(2 * n, H, D, dtype, 3)
+    kept = both[:n].clone()
+    kd.prompt_attention(both[:n], k, v, i32([0, 40, n]), both[n:])
+    check_prompt(kept, k, v, both[n:], [0, 40, n], 0, dtype)
+    assert torch.equal(kept, both[:n])
+    alternate = rows_of(2 * n, H, D, dtype, 4)
+    kept = alternate[::2].clone()
+    kd.prompt_attention(alternate[::2], k, v, i32([0, 40, n]), alternate[1::2])
+    check_prompt(kept, k, v, alternate[1::2], [0, 40, n], 0, dtype)
+    assert torch.equal(kept, alternate[::2])
+    plan, table, cache, q, out, ws = cache_case(kd, dtype, H, KV, D, 16, [1, 3], [100, 40], 0)
+    want = out.clone()
+    wide = torch.cat([q, q], 1)
+    kd.kv_attention(wide[:, :H], plan, table, cache, wide[:, H:], ws)
+    assert torch.equal(wide[:, H:], want) and torch.equal(wide[:, :H], q)
+    same = torch.cat([q, q], 1)
+    kd.kv_attention(same[:, :H], plan, table, cache, same[:, :H], ws)
+    assert torch.equal(same[:, :H], want) and torch.equal(same[:, H:], q)
