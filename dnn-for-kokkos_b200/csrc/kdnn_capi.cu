@@ -619,6 +619,22 @@ int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, si
     return fail(KDNN_ERR_INVALID, "kv_plan: null or misaligned argument");
   if (writes_entries < kdnn_b200_kv_writes(rows, seqs, page) || writes_entries > static_cast<size_t>(INT_MAX) / 4)
     return fail(KDNN_ERR_INVALID, "kv_plan: writes holds fewer entries than kv_writes() says");
+  // What the call writes is apart from all else it is given, but for lens_out on lens and state_out on state (the CTAs that read lens and state
+  // have to know of their new values). {first byte, bytes of a row, rows, pitch}
+  struct Part { const void* p; size_t bytes, rows, pitch; };
+  const Part parts[] = {{fresh, seqs * 4, 1, 0}, {lens, seqs * 4, 1, 0}, {state, 16, 1, 0},   // read; written from here on
+                        {row_start, (seqs + 1) * 4, 1, 0}, {first, seqs * 4, 1, 0}, {lens_out, seqs * 4, 1, 0}, {state_out, 16, 1, 0},
+                        {slots, rows * 4, 1, 0}, {writes, writes_entries * 16, 1, 0}, {ring, pages * 4, 1, 0}, {table, table_cols * 4, seqs, ldt * 4}};
+  auto meet = [](const Part& x, const Part& y) {      // x has one row
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+    if (x.bytes == 0 || y.bytes == 0 || a >= b + (y.rows - 1) * y.pitch + y.bytes || b >= a + x.bytes) return false;
+    const size_t r = y.rows > 1 && a > b ? (a - b) / y.pitch : 0;      // the row of y that begins last before x, and the next
+    return a < b + r * y.pitch + y.bytes || (r + 1 < y.rows && b + (r + 1) * y.pitch < a + x.bytes);
+  };
+  for (int i = 0; i < 10; ++i)
+    for (int j = i < 3 ? 3 : i + 1; j < 11; ++j)
+      if (!(i == 1 && j == 5) && !(i == 2 && j == 6) && meet(parts[i], parts[j]))
+        return fail(KDNN_ERR_INVALID, "kv_plan: arguments overlap (lens_out may be lens, state_out may be state)");
   return cuda_result(kdnn::kv_plan_launch(fresh, lens, state, table, ldt, table_cols, ring, pages, seqs, page, rows, row_start, first,
                                           lens_out, state_out, slots, writes, writes_entries, static_cast<cudaStream_t>(stream)),
                      "kv_plan");

@@ -435,7 +435,7 @@ size_t kdnn_b200_kv_writes(size_t rows, size_t seqs, size_t page);
  * writes[i] = {first row, rows, page number, first token in the page}, one per page that new rows fall on, the rest zero.
  * Pages go to the sequences in order. Where the ring runs out, or a sequence outgrows table_cols pages, the sequence's last
  * tokens get no slot: lens_out counts what is stored, state_out[2] what is not. More fresh tokens than `rows` are cut at
- * `rows` and counted there too. lens_out may be lens and state_out may be state. Calls that share a pool must not overlap.
+ * `rows` and counted there too. lens_out may be lens and state_out may be state; else nothing written may overlap. Calls that share a pool must not overlap.
  * seqs <= 8192, rows <= 2^30, pages * page <= INT_MAX, table_cols * page <= INT_MAX. */
 int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, size_t page, size_t rows, int32_t* table, size_t ldt,
                       size_t table_cols, int32_t* ring, size_t pages, const int32_t* state, int32_t* row_start, int32_t* first,

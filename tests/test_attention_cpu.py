@@ -169,3 +169,33 @@ def test_results_that_overlap_their_inputs_are_refused(kd):
         assert cached(**kw) == kd.KDNN_ERR_INVALID and "overlap" in kd.last_error(), kw
     for kw in (dict(out=0x200000 + 512), dict(out=0x300000 - 1024), dict(out=0x300000, ldo=512)):      # k and v
         assert prompt(**kw) == kd.KDNN_ERR_INVALID and "overlap" in kd.last_error(), kw
+
+
+def test_plan_arguments_that_overlap_are_refused(kd):
+    """What a plan writes on something else that it reads or writes: other CTAs may still have to read it."""
+    MB = 1 << 20
+    names = ("fresh", "lens", "table", "ring", "state", "row_start", "first", "lens_out", "state_out", "slots", "writes")
+    ok = dict(fresh=1 * MB, lens=2 * MB, seqs=300, page=64, rows=5000, table=3 * MB, ldt=100, cols=90, ring=4 * MB, pages=9000, state=5 * MB,
+              row_start=6 * MB, first=7 * MB, lens_out=8 * MB, state_out=9 * MB, slots=10 * MB, writes=11 * MB, entries=700)
+    size = dict(fresh=300, lens=300, table=299 * 100 + 90, ring=9000, state=4, row_start=301, first=300, lens_out=300, state_out=4, slots=5000,
+                writes=2800)
+
+    def call(**kw):
+        return kd.lib.kdnn_b200_kv_plan(*dict(ok, **kw).values(), None)
+
+    reads = ("fresh", "lens", "state")
+    for a in names:
+        for b in names:
+            if a == b or (a in reads and b in reads) or {a, b} in ({"lens", "lens_out"}, {"state", "state_out"}):
+                continue
+            for at in (ok[b], ok[b] + 4 * (size[b] - 1), ok[b] - 4 * (size[a] - 1)):
+                if a == "writes":
+                    at = at // 16 * 16
+                    if not (at < ok[b] + 4 * size[b] and ok[b] < at + 4 * size[a]):
+                        continue
+                if "table" in (a, b) and at not in (ok[b],) and a != "table":
+                    at = ok[b] + 4 * (17 * 100 + 89)              # the last column of a row
+                    if a == "writes":
+                        at = at // 16 * 16
+                assert call(**{a: at}) == kd.KDNN_ERR_INVALID, (a, b, at)
+                assert "overlap" in kd.last_error(), (a, b, kd.last_error())
