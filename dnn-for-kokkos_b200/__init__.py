@@ -948,6 +948,8 @@ def kv_attention(q: torch.Tensor, plan: KvPlan, table: torch.Tensor, cache: KvCa
     ldt = _table("kv_attention", table, seqs)
     if cache.page != plan.page or window < 0:
         raise ValueError("kv_attention: cache and plan have pages of different size, or the window is negative")
+    if not workspace.is_contiguous():      # (its bytes are counted)
+        raise ValueError("kv_attention: the workspace must be contiguous")
     stream = _stream_of("kv_attention", q, out, table, workspace, plan.first, cache.k)
     _check(lib.kdnn_b200_kv_attention(q.data_ptr(), ldq, hdq, _scalar(q), rows, heads, plan.row_start.data_ptr(), plan.first.data_ptr(),
                                       plan.lens.data_ptr(), seqs, table.data_ptr(), ldt, table.shape[1], C.byref(cache.c_struct()),

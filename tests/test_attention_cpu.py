@@ -199,3 +199,18 @@ def test_plan_arguments_that_overlap_are_refused(kd):
                         at = at // 16 * 16
                 assert call(**{a: at}) == kd.KDNN_ERR_INVALID, (a, b, at)
                 assert "overlap" in kd.last_error(), (a, b, kd.last_error())
+
+
+def test_a_workspace_whose_bytes_are_not_there_is_refused(kd, monkeypatch):
+    """An expanded tensor has more elements than memory."""
+    plan, cache = kd.KvPlan.empty(2, 5, 16, device="cpu"), kd.KvCache.empty(4, 2, 16, 64, device="cpu")
+    q, table = torch.zeros(5, 4, 64), torch.zeros(2, 3, dtype=torch.int32)
+    calls = []
+    monkeypatch.setattr(kd, "_stream_of", lambda *a: 0)
+    monkeypatch.setattr(kd.lib, "kdnn_b200_kv_attention", lambda *a: calls.append(a) or 0)
+    for ws in (torch.zeros(256, dtype=torch.uint8)[:1].expand(1 << 30), torch.zeros(1 << 12, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            kd.kv_attention(q, plan, table, cache, torch.zeros_like(q), ws)
+    assert not calls
+    kd.kv_attention(q, plan, table, cache, torch.zeros_like(q), torch.zeros(64, dtype=torch.float32))
+    assert len(calls) == 1 and calls[0][-2] == 256
