@@ -444,8 +444,8 @@ int kdnn_b200_kv_plan(const int32_t* fresh, const int32_t* lens, size_t seqs, si
 /* New rows into the cache: k, v [rows][kv_heads][dim] Scalar with row and head pitches in elements, places from a plan's
  * `writes`. A page's scale becomes the smallest power of two s >= 2^-100 with max|x| <= 127 s over its new rows, or stays
  * what it was where that is larger; new codes are rint(x / s); older codes of the page are rint(code * old scale / s).
- * A page that is written from its first token on starts over. Infinities take the largest code, NaN takes 0, and neither
- * counts for the scale. An entry of `writes` that names no place of the cache writes nothing. */
+ * A page that is written from its first token on starts over. Infinities take the largest code (0 where the page has no scale yet, its new rows
+ * holding nothing finite but zeros), NaN takes 0, and neither counts for the scale. An entry of `writes` that names no place of the cache writes nothing. */
 int kdnn_b200_kv_append(const void* k, size_t ldk, size_t hdk, const void* v, size_t ldv, size_t hdv, int scalar, size_t rows,
                         const int32_t* writes, size_t writes_entries, const kdnn_b200_kv_cache* cache, void* stream);
 

@@ -3,7 +3,7 @@ those of test_attention_gpu.py."""
 import pytest
 import torch
 
-from test_attention_gpu import F32, OUT, cache_case, check_prompt, i32, rows_of
+from test_attention_gpu import F32, OUT, attend, cache_case, check_prompt, i32, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,52 @@ def test_results_beside_their_inputs_in_one_buffer(kd, dtype):
     same = torch.cat([q, q], 1)
     kd.kv_attention(same[:, :H], plan, table, cache, same[:, :H], ws)
     assert torch.equal(same[:, :H], want) and torch.equal(same[:, H:], q)
+
+
+# ---- errors as a whole: a bound for each element leaves room for errors that grow with the number of keys, the 2-norm does not. A value
+# rounded to bf16 is off by 2^-8 at the most and by 2^-8 (1 / sqrt 3) sqrt(3 / (8 ln 2)) = 1.66e-3 in the mean square (an error uniform within
+# half a step, mantissas evenly over their logarithm); random values make the weights' errors and the result's independent, and a result of
+# random values is off by the mean square of its weights' errors. A tenth is left for the sample (thousands of elements).
+BF16_RMS = 2.0 ** -8 * (1 / 3) ** 0.5 * (3 / (8 * 0.6931471805599453)) ** 0.5
+
+
+def off_by(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [300, 3000, 20000])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_attention_as_a_whole(kd, dtype, n, dim):
+    q, k, v = rows_of(n, 8, dim, dtype, 1), rows_of(n, 2, dim, dtype, 2), rows_of(n, 2, dim, dtype, 3)
+    out = torch.empty_like(q)
+    kd.prompt_attention(q, k, v, i32([0, n]), out)
+    i = torch.arange(n - 24, n, device="cuda")
+    want, _, big, _, _ = attend(q[-24:], k, v, torch.arange(n, device="cuda")[None, :] <= i[:, None], dim ** -0.5)
+    if dtype == torch.bfloat16:
+        limit = 1.1 * BF16_RMS * 2 ** 0.5                                # weights and result
+    else:
+        limit = 2 * big.mean().item() * 8 * F32 + 8 * F32               # a score's eight roundings, twice (its own and the sum's), and the result's
+    assert off_by(out[-24:], want) <= limit
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [300, 3000, 50000])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_cache_attention_as_a_whole(kd, dtype, n, dim):
+    plan, table, cache, q, out, ws = cache_case(kd, dtype, 16, 2, dim, 64, [2, 1], [n, n // 2], 0, seed=n)
+    gots, wants, bigs = [], [], []
+    for b in range(2):
+        r0, r1 = plan.row_start.tolist()[b:b + 2]
+        T = plan.lens[b].item()
+        pg = table[b, :-(-T // 64)].long()
+        k, v = ((c[pg].double() * s[pg].double()[..., None, None]).transpose(1, 2).reshape(-1, 2, dim)[:T]
+                for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        pos = torch.arange(T - (r1 - r0), T, device="cuda")[:, None]
+        want, _, big, _, _ = attend(q[r0:r1], k, v, torch.arange(T, device="cuda")[None, :] <= pos, dim ** -0.5)
+        gots.append(out[r0:r1]), wants.append(want), bigs.append(big.mean().item())
+    if dtype == torch.bfloat16:
+        limit = 1.1 * BF16_RMS * (1 + 2.0 ** -6) ** 0.5                   # fp16 weights have three bits more
+    else:
+        limit = 2 * max(bigs) * 8 * F32 + 8 * F32
+    assert off_by(torch.cat(gots), torch.cat(wants)) <= limit
