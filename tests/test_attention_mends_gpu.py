@@ -265,3 +265,68 @@ def test_cache_attention_as_a_whole(kd, dtype, n, dim):
     else:
         limit = 2 * max(bigs) * 8 * F32 + 8 * F32
     assert off_by(torch.cat(gots), torch.cat(wants)) <= limit
+
+
+def test_prompts_and_products_on_two_streams(kd):
+    """Kernels that take tensor memory, on two streams at once: prompts of several forms on both, packed products behind them on one."""
+    made = []
+    for i, (heads, kv, dim, lens) in enumerate([(16, 16, 64, [40, 3, 500]), (32, 8, 128, [700, 600]), (8, 4, 256, [300]), (32, 8, 128, [77])]):
+        starts = [0]
+        for n in lens:
+            starts.append(starts[-1] + n)
+        q, k, v = (rows_of(starts[-1], h, dim, torch.bfloat16, 10 * i + j) for j, h in enumerate((heads, kv, kv)))
+        made.append((q, k, v, i32(starts), torch.empty_like(q)))
+    packed = kd.ggml_pack.synth_weight(kd.Q4_K, 1024, 2048, seed=3)
+    w = kd.QuantWeight.from_numpy(packed, kd.Q4_K, 1024, 2048, torch.device("cuda"))
+    x = rows_of(200, 1, 2048, torch.bfloat16, 77)[:, 0].contiguous()
+    ws = torch.empty(kd.quant_gemm_workspace_bytes(200, 2048), dtype=torch.uint8, device="cuda")
+    y = torch.empty(200, 1024, dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    kd.quant_gemm(x, w, y, ws)
+    for q, k, v, rs, out in made:
+        kd.prompt_attention(q, k, v, rs, out)
+    torch.cuda.synchronize()
+    want, product = [m[4].clone() for m in made], y.clone()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[torch.empty_like(m[4]) for m in made] for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(25):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for m, out in zip(made, outs[s]):
+                    kd.prompt_attention(*m[:4], out)
+                    if s == 0:
+                        kd.quant_gemm(x, w, y, ws)
+    torch.cuda.synchronize()
+    assert kd.device_status() == 0 and torch.equal(y, product)
+    for got in outs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_captured_prompt_whose_values_change(kd, dtype):
+    """Replays of one captured call over values that hold infinities, NaN and numbers near the largest, and over ordinary ones again."""
+    n, starts = 500, [0, 300, 500]
+    q, k, v = rows_of(n, 8, 128, dtype, 1), rows_of(n, 2, 128, dtype, 2), rows_of(n, 2, 128, dtype, 3)
+    out, rs, plain = torch.empty_like(q), i32(starts), v.clone()
+    kd.prompt_attention(q, k, v, rs, out)
+    torch.cuda.synchronize()
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        kd.prompt_attention(q, k, v, rs, out)
+    for kind in ("nan", "plain", "large", "inf", "plain"):
+        v.copy_(plain)
+        if kind == "large":
+            v[::3] = 2e38
+        elif kind != "plain":
+            v[290, 1, 5] = v[450, 0, 9] = float(kind)
+        graph.replay()
+        torch.cuda.synchronize()
+        if kind == "plain":
+            assert torch.equal(out, first)
+        elif kind == "large":
+            check_prompt(q, k, v, out, starts, 0, dtype)
+        else:
+            hit = ~torch.isfinite(out)
+            assert hit[290:300, 4:, 5].all() and hit[450:, :4, 9].all() and hit.sum() == 10 * 4 + 50 * 4
