@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   bool ok = true;
 
   // Registers go where the scores are: 2 x 128 threads of 224 and 128 of 56 are the 64512 that the launch holds (168 each). (One tile alone
-  // needs no split: 219 a thread, 255 for wide heads.)
+  // needs no split: 217 a thread, 255 for wide heads.)
   if (warp < L::kWarpTma) {
     if (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------------ scores -> weights (a thread owns a row)
