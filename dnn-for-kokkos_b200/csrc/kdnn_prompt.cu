@@ -609,9 +609,9 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
   auto p_full  = [&](int x) { return bars + 112u + 8u * x; };
   auto o_full  = [&](int x) { return bars + 128u + 8u * x; };
   const uint32_t mma_end = bars + 144u;
-  // v_clean: the values of the e-th step with masked places have been looked through; v_asked: the later ones of these steps are near. One phase each.
-  const uint32_t v_asked = bars + 176u;
-  auto v_clean = [&](int e) { return bars + 184u + 8u * e; };
+  // The e-th step with masked places: its values come next to their stage (v_asked), and have been looked through (v_clean). One phase each.
+  auto v_asked = [&](int e) { return bars + 176u + 8u * e; };
+  auto v_clean = [&](int e) { return bars + 216u + 8u * e; };
   uint32_t* tmem_slot      = reinterpret_cast<uint32_t*>(smem + L::bar + 152);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::bar + 156);
   RingArmed* ring_end      = reinterpret_cast<RingArmed*>(smem + L::bar + 160);   // what the TMA warp armed last
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     fence_barrier_init();
     fence_proxy_async();
   } else if (warp == 1) {
-    if (lane <= kPtEdges) mbar_init(v_asked + 8u * lane, lane == 0 ? 1 : 2);      // (v_clean right behind)
+    if (lane < 2 * kPtEdges) mbar_init(v_asked(lane), lane < kPtEdges ? 1 : 2);      // (v_clean right behind)
     if (lane <= 4 * kPtEdges) odd_any[lane] = 0u;
     fence_barrier_init();
   }
@@ -875,8 +875,9 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     int cleaned = 0;
     for (int j = 0; j < steps && ok; ++j) {
       if (!(ok = wait(full(vs.at), vs.ph))) break;
-      if (j + 1 == high && lane == 0) mbar_arrive(v_asked);
-      if ((j < low || j >= high) && !(ok = wait(v_clean(cleaned++), 0))) break;
+      const bool here = j < low || j >= high;
+      if ((j + 1 < low || j + 1 >= high) && j + 1 < steps && lane == 0) mbar_arrive(v_asked(cleaned + here));
+      if (here && !(ok = wait(v_clean(cleaned++), 0))) break;
       bool keys = false;       // the next step's keys are there
       for (int x = 0; x < TILES && ok; ++x) {
         const int n = x ? n1 : n0;
@@ -902,13 +903,14 @@ __global__ void __launch_bounds__(128 * TILES + 128, 1) prompt_tc_kernel(const _
     constexpr int HALVES = DM / 64;
     const int tid = static_cast<int>(threadIdx.x) - (L::kWarpMma + 1) * 32, last = max(end0, end1) - 1;
     for (int e = 0; e < edges; ++e) {
-      // The phase that is waited for is the one that comes next, so that its parity says it: what was in the stage before had to land for the
-      // products that came before v_asked, or before the step that was looked through last.
+      // A parity tells a stage's next copy from the one before it, not from the one before that: the wait for the values of step j begins when the
+      // product warp is at step j - 1, which has used what lay in their stage before them (the keys of step j - 2, with two stages the values of
+      // j - 1), and they stay until they have been looked through.
       const int j = step_of(e), fill = 2 * j + 1, st = fill % L::kStages, k0 = beg + j * kPtKeys;
-      if (j == high && high > low) {      // behind all the steps between, each of which has the time of a wait: parked, so that two warps do not
-        ok = false;                         // poll beside the exponentials all that time
+      if (j > 0) {      // behind all the steps between, each of which has the time of a wait: parked, so that two warps do not poll beside the exponentials
+        ok = false;
         for (long long i = 0; i < (j + 1LL) << 16; ++i) {
-          if ((ok = __all_sync(0xffffffffu, mbar_try_wait_hint(v_asked, 0, 20000u)))) break;
+          if ((ok = __all_sync(0xffffffffu, mbar_try_wait_hint(v_asked(e), 0, 20000u)))) break;
           if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
         }
         if (!ok) *abort_flag = 1;
