@@ -330,3 +330,42 @@ def test_a_captured_prompt_whose_values_change(kd, dtype):
         else:
             hit = ~torch.isfinite(out)
             assert hit[290:300, 4:, 5].all() and hit[450:, :4, 9].all() and hit.sum() == 10 * 4 + 50 * 4
+
+
+def test_cache_beyond_two_to_the_31_bytes(kd):
+    """Pages whose codes lie behind 2^31 bytes: written, read, and nothing near 2^31 or 2^32 less is."""
+    page, kv, dim, pages, heads = 64, 8, 128, 66000, 32
+    cache = kd.KvCache(*(torch.zeros((pages, kv, page, dim), dtype=torch.int8, device="cuda") for _ in range(2)),
+                       *(torch.zeros((pages, kv), device="cuda") for _ in range(2)))
+    assert cache.k.numel() > 2 ** 32
+    top = [pages - 1, 32768 + 5, 65536 + 7, 32767, 40000]            # (a page is 2^16 bytes)
+    plan = kd.KvPlan.empty(2, 200, page)
+    ring = torch.full((pages,), -1, dtype=torch.int32, device="cuda")
+    ring[:5] = i32(top)
+    table = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+    kd.kv_plan(i32([130, 70]), i32([0, 0]), table, ring, i32([0, 5, 0, 0]), plan)
+    assert table.tolist() == [top[:3] + [-1], top[3:] + [-1, -1]]
+    k, v, q = (rows_of(200, h, dim, torch.bfloat16, s) for s, h in enumerate((kv, kv, heads)))
+    kd.kv_append(k, v, plan, cache)
+    touched = cache.k_scale.amax(1).nonzero()[:, 0].tolist()
+    assert touched == sorted(top) and not any(cache.k[p - 32768 if p >= 32768 else p + 32768].any() for p in (32768 + 5, 40000))
+    out = torch.full_like(q, 777.0)
+    ws = torch.empty(kd.kv_attention_workspace_bytes(200, 2, heads, kv, dim), dtype=torch.uint8, device="cuda")
+    kd.kv_attention(q, plan, table, cache, out, ws)
+    from test_attention_gpu import check_cache
+    check_cache(plan, table, cache, q, out, [0, 0], [130, 70], 0, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,heads,dim", [(torch.bfloat16, 128, 128), (torch.float32, 64, 256), (torch.bfloat16, 64, 256)])
+def test_prompts_beyond_two_to_the_31_elements(kd, dtype, heads, dim):
+    n = 2 ** 31 // (heads * dim) + 700
+    q, k, v = (torch.zeros((n, h, dim), dtype=dtype, device="cuda") for h in (heads, 2, 2))
+    tail = 600
+    for i, t in enumerate((q, k, v)):
+        t[-tail:] = rows_of(tail, t.shape[1], dim, dtype, i)
+    out = torch.full_like(q, 777.0)
+    starts = [n - 590, n - 400, n - 13]
+    kd.prompt_attention(q, k, v, i32(starts), out)
+    part = slice(n - 590, n)
+    check_prompt(q[part], k[part], v[part], out[part], [0, 190, 577], 0, dtype)
+    assert (out[n - 13:] == 777.0).all() and (out[n - 700:n - 590] == 777.0).all() and (out[:1000] == 777.0).all()
